@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libammon_amd.so")
 
 OK, E_VALIDATION, E_HIP, E_OOM, E_NO_DEVICE = 0, 1, 2, 3, 4
 F32, BF16 = 0, 1
+KV4 = 4  # KV caches only
 COPY_H2D, COPY_D2H, COPY_D2D = 1, 2, 3
 STREAM_VALIDATE = ctypes.c_void_p(1)
 
@@ -77,6 +78,7 @@ SIGNATURES = {
     "ammon_rope_table_host": (_ST, [_F, _U32, _U32, _P]),
     "ammon_kv_unpermute": (_ST, [_P, _P, _U32, _U32, _U32, _U32]),
     "ammon_kv_permute": (_ST, [_P, _P, _U32, _U32, _U32, _U32]),
+    "ammon_kv_cache_bytes": (_SZ, [_DT, _U32, _U32, _U32]),
     "ammon_attention_splits": (_U32, [_U32, _U32]),
     "ammon_attention_scratch_bytes": (_SZ, [_U32, _U32, _U32, _U32]),
     "ammon_attention_default_split": (_U32, [_P, _U32, _U32]),
@@ -87,6 +89,8 @@ SIGNATURES = {
     "ammon_rope_store": (_ST, [_P, _P, _P, _U32, _P, _U32, _U32, _P, _DT, _U32, _P, _P]),
     "ammon_rope": (_ST, [_P, _P, _P, _U32, _U32, _U32, _P, _DT, _U32, _P, _P]),
     "ammon_cache_store": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT, _U32, _P]),
+    "ammon_kv4_store": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _U32, _P]),
+    "ammon_kv4_load": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _DT]),
     "ammon_attention_partial": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _U32, _P,
                                       _U32, _P]),
     "ammon_attention_combine": (_ST, [_P, _P, _P, _U32, _U32, _U32, _P, _U32, _P]),
@@ -94,6 +98,10 @@ SIGNATURES = {
                                            _U32, _U32, _U32, _U32]),
     "ammon_attention_decode": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _U32, _P,
                                      _U32, _P, _SZ, _P]),
+    "ammon_attention_partial_append": (_ST, [_P, _P, _P, _U32, _P, _P, _P, _P, _DT, _U32, _U32,
+                                             _U32, _P, _U32, _P]),
+    "ammon_attention_decode_append": (_ST, [_P, _P, _P, _U32, _P, _P, _P, _P, _DT, _U32, _U32,
+                                            _U32, _P, _U32, _P, _SZ, _P]),
     "ammon_attention_decode_noalloc": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _U32,
                                              _P, _U32, _P]),
     "ammon_swiglu": (_ST, [_P, _P, _P, _P, _U32]),

@@ -18,6 +18,7 @@ extern "C" {
 /* Storage type codes; match ammon_dtype in include/ammon/ammon.h. */
 #define AMMON_K_F32 0
 #define AMMON_K_BF16 1
+#define AMMON_K_KV4 4 /* KV caches only: kernels/kv4_impl.h */
 
 /* Device-resident control parcel: same layout as ammon_decode_step. */
 typedef struct {
@@ -88,7 +89,22 @@ typedef struct {
   uint32_t pair;            /* prefill tiles: workgroups per XCD of which every CU
                                gets one, where a second one per CU takes the
                                rest, in reverse order (0: order as launched) */
+  const float *k_new;       /* KV4 pass 1, append: the position's own key and value */
+  const float *v_new;       /* rows [kv_heads, head], stored by the unit that has it */
 } ammon_k_attention;
+
+/* KV4 rows stored and read back. */
+typedef struct {
+  const float *k, *v;       /* store: [tokens, kv_heads, head] */
+  void *k_cache, *v_cache;  /* codes, then scales: kernels/kv4_impl.h */
+  const ammon_k_step *step; /* store: row t goes to position step->position + t */
+  void *k_out, *v_out;      /* load: [kv_heads, tokens, head] fp32 or bf16 */
+  float *q;                 /* rope_store: [q_numel], rotated in place */
+  const float *table;       /* rope_store: cos/sin [seq, head/2, 2] */
+  uint32_t tokens, kv_heads, head, seq;
+  uint32_t first;           /* load: positions first.. */
+  uint32_t out_dtype, q_numel;
+} ammon_k_kv4;
 
 typedef struct {
   float *hb;                /* [n] in/out (swiglu) or out (add) */

@@ -1,0 +1,107 @@
+// kv4.hip -- kernels of the 4-bit KV cache: rows stored and read back, and split-K
+// decode attention (units of kv4_attention_impl.h; pass 2 is attention.hip's).
+#include "kv4_attention_impl.h"
+
+// Rows [tokens, kv_heads, head] (fp32) into the cache at position step->position + t:
+// 16 lanes a row, 16 rows a workgroup, blockIdx.y 0 the keys, 1 the values.  Bytes
+// bound it: 4 head read and 20 NG written per row.
+extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_store(ammon_k_kv4 p) {
+  const uint32_t r = blockIdx.x * (AMMON_WG / 16) + threadIdx.x / 16, i = threadIdx.x & 15;
+  if (r >= p.tokens * p.kv_heads) return;  // (a row's 16 lanes go together)
+  const uint32_t t = r / p.kv_heads, g = r - t * p.kv_heads;
+  const uint64_t pos = (uint64_t)p.step->position + t;
+  if (pos >= p.seq) return;  // out of range: the cache stays as it is
+  const float *src = blockIdx.y ? p.v : p.k;
+  void *cache = blockIdx.y ? p.v_cache : p.k_cache;
+  float x[8];
+  kv4_row(src + (size_t)r * p.head, i, p.head, x);
+  kv4_put(cache, p.kv_heads, p.seq, p.head, g, (uint32_t)pos, i, x);
+}
+
+// rope_store (rope.hip) into a KV4 cache: q rotated in place, a lane per pair, by the
+// first ceil(q_numel / 2 / 256) workgroups; the rest rotate and store the rows of k
+// [kv_heads, head], 16 lanes each.  The rotation's products round before the sum, as
+// there.
+extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_rope_store(ammon_k_kv4 p) {
+#pragma clang fp contract(off)
+  const uint32_t pos = p.step->position;
+  if (pos >= p.seq) return;
+  const float *cs = p.table + (size_t)pos * p.head;
+  const uint32_t qblocks = (p.q_numel / 2 + AMMON_WG - 1) / AMMON_WG;
+  if (blockIdx.x < qblocks) {
+    const uint32_t i = 2 * (blockIdx.x * AMMON_WG + threadIdx.x);
+    if (i >= p.q_numel) return;
+    const float fcr = cs[i % p.head], fci = cs[i % p.head + 1];
+    const float q0 = p.q[i], q1 = p.q[i + 1];
+    p.q[i] = q0 * fcr - q1 * fci;
+    p.q[i + 1] = q0 * fci + q1 * fcr;
+    return;
+  }
+  const uint32_t g = (blockIdx.x - qblocks) * (AMMON_WG / 16) + threadIdx.x / 16;
+  if (g >= p.kv_heads) return;
+  const uint32_t i = threadIdx.x & 15;
+  float x[8];
+  kv4_row(p.k + (size_t)g * p.head, i, p.head, x);
+#pragma unroll
+  for (uint32_t e = 0; e < 8; e += 2) {
+    const uint32_t d = 8 * i + e;
+    const float fcr = d < p.head ? cs[d] : 0.f, fci = d < p.head ? cs[d + 1] : 0.f;
+    const float a = x[e] * fcr - x[e + 1] * fci, b = x[e] * fci + x[e + 1] * fcr;
+    x[e] = a;
+    x[e + 1] = b;
+  }
+  kv4_put(p.k_cache, p.kv_heads, p.seq, p.head, g, pos, i, x);
+}
+
+// Positions first.. of the cache as numbers [kv_heads, tokens, head], fp32 or bf16: 16
+// lanes a row, 8 numbers each.  Bytes bound it.
+extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_load(ammon_k_kv4 p) {
+  const uint64_t r = (uint64_t)blockIdx.x * (AMMON_WG / 16) + threadIdx.x / 16;
+  const uint32_t i = threadIdx.x & 15, j = i >> 2, piece = i & 3, ng = kv4_groups(p.head);
+  if (r >= (uint64_t)p.tokens * p.kv_heads || 8 * i >= p.head) return;
+  const uint32_t g = (uint32_t)(r / p.tokens), t = (uint32_t)(r - (uint64_t)g * p.tokens) + p.first;
+  const void *cache = blockIdx.y ? p.v_cache : p.k_cache;
+  void *out = blockIdx.y ? p.v_out : p.k_out;
+  const uint32_t w = kv4_codes(cache, p.seq, ng, g, t)[piece * ng + j];
+  const uint32_t sb = kv4_scales(cache, p.kv_heads, p.seq, ng, g, t)[j];
+  const f16x8 v = kv4_numbers(w, sb);
+  const size_t at = (size_t)r * p.head + 8 * i;
+  if (p.head % 8 == 0 && p.out_dtype == AMMON_K_F32) {
+    float *to = (float *)out + at;
+    *(float4 *)to = make_float4(v[0], v[1], v[2], v[3]);
+    *(float4 *)(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else if (p.head % 8 == 0) {
+    u32x4 b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      b[e] = (uint32_t)f32_to_bf16(v[2 * e]) | (uint32_t)f32_to_bf16(v[2 * e + 1]) << 16;
+    *(u32x4 *)((uint16_t *)out + at) = b;
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e)
+      if (8 * i + e < p.head) store_elem(out, p.out_dtype, at + e, v[e]);
+  }
+}
+
+// Pass 1 on a (splits, kv heads, tokens) grid.
+#define KV4_PARTIAL(NAME, NG, NCH, APPEND)                                            \
+  extern "C" __global__ __launch_bounds__(AMMON_WG, 2) void NAME(const ammon_k_step *step, \
+                                                                ammon_k_attention p_) { \
+    using Unit = Kv4Partial<NG, NCH, APPEND>;                                          \
+    __shared__ u32x4 lds[Unit::LDS_BYTES / 16];                                        \
+    ammon_k_attention p0 = p_;                                                         \
+    p0.step = step;                                                                    \
+    const ammon_k_attention p = attention_token(p0, blockIdx.z);                       \
+    Unit unit;                                                                         \
+    if (unit.begin(p, blockIdx.x, blockIdx.y, (char *)lds))                            \
+      unit.run(p, (char *)lds);                                                        \
+    else                                                                               \
+      direct_out_nan(p, blockIdx.y);                                                   \
+  }
+#define KV4_PARTIAL_NG(NG)                                      \
+  KV4_PARTIAL(ammon_kv4_partial_n##NG, NG, 3, false)            \
+  KV4_PARTIAL(ammon_kv4_partial_append_n##NG, NG, 3, true)
+KV4_PARTIAL_NG(1)
+KV4_PARTIAL_NG(2)
+KV4_PARTIAL_NG(3)
+KV4_PARTIAL_NG(4)

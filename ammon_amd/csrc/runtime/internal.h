@@ -21,6 +21,10 @@ constexpr int kAttChunks = 4;  // CH = 8, 4, 2, 1
 constexpr int kAttGroups = 4;  // GMAX = 1, 2, 4, 8
 // GEMV variants: [weight dtype][vector?][mode].
 constexpr int kGemvModes = 4;
+// KV4 variants: ceil(head / 32).
+constexpr int kKv4Groups = 4;
+// Bytes of a KV4 row per group of 32 numbers: 16 of codes, 4 of scale and bias.
+constexpr size_t kKv4RowBytes = 20;
 
 struct Kernels {
   hipFunction_t embed = nullptr;
@@ -58,6 +62,11 @@ struct Kernels {
   // bf16, register-blocked tiles: [64 tokens, 32 tokens][RT 4, RT 2][mode]
   hipFunction_t gemm_big[2][2][kGemvModes] = {};
   hipFunction_t gemm_big_t16[kGemvModes] = {};  // 16 tokens, RT 2
+  // 4-bit KV cache: rows written and read back, decode pass 1 [plain / append][groups - 1]
+  hipFunction_t kv4_store = nullptr;
+  hipFunction_t kv4_rope_store = nullptr;
+  hipFunction_t kv4_load = nullptr;
+  hipFunction_t kv4_partial[2][kKv4Groups] = {};
 };
 
 // LDS per compute unit on gfx950 (bytes); bounds resident GEMV workgroups.

@@ -22,6 +22,7 @@ using DeviceGuard = ammon_rt::DeviceScope;
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 inline bool valid_dtype(ammon_dtype d) { return d == AMMON_F32 || d == AMMON_BF16; }
+inline bool valid_kv(ammon_dtype d) { return valid_dtype(d) || d == AMMON_KV4; }
 inline size_t dsize(ammon_dtype d) { return d == AMMON_BF16 ? 2 : 4; }
 
 inline bool overlaps(const void *a, size_t abytes, const void *b, size_t bbytes) {
@@ -257,12 +258,16 @@ int att_group_index(uint32_t g) {
   return -1;
 }
 
-// Pass-1 variant for a cache layout, or NULL when no chunk width fits.
+// Pass-1 variant for a cache layout, or NULL when no chunk width fits (KV4: when the
+// caches are not aligned).
 // split_len 0: the kernel a split of 128 positions would take (occupancy
 // queries before the split is chosen).
 hipFunction_t attention_kernel(ammon_runtime *rt, ammon_dtype kv_dtype, uint32_t q_heads,
                                uint32_t kv_heads, uint32_t head, const void *k, const void *v,
-                               uint32_t split_len) {
+                               uint32_t split_len, bool append = false) {
+  if (kv_dtype == AMMON_KV4)
+    return (((uintptr_t)k | (uintptr_t)v) & 15u) == 0 ? rt->k.kv4_partial[append][(head - 1) / 32]
+                                                      : nullptr;
   const int ci = att_chunk_index(kv_dtype, head, k, v);
   if (ci < 0) return nullptr;
   const int gi = att_group_index(q_heads / kv_heads);
@@ -310,6 +315,7 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
                          uint32_t head, uint32_t ctx, uint32_t scratch_splits, ammon_dtype kv_dtype,
                          bool aligned) {
   PrefillPlan plan;
+  if (kv_dtype == AMMON_KV4) return plan;
   const bool bf = kv_dtype == AMMON_BF16;
   const uint32_t g = q_heads / kv_heads;
   const uint64_t rows = (uint64_t)tokens * g, krow = head * dsize(kv_dtype);
@@ -421,6 +427,104 @@ ammon_status ammon_rmsnorm(ammon_runtime *rt, ammon_stream stream, const float *
   return launch(rt, stream, rt->k.rmsnorm, rows, 1, 0, p, "rmsnorm");
 }
 
+// ---- 4-bit KV cache ------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+// What every call on KV4 caches asks of them (v NULL: of one).
+ammon_status kv4_check(const char *what, uint32_t kv_heads, uint32_t head, uint32_t seq, const void *k,
+                       const void *v) {
+  AMMON_CHECK(kv_heads > 0 && head > 0 && seq > 0, "%s: empty shape (kv_heads=%u, head=%u, seq=%u)",
+              what, kv_heads, head, seq);
+  AMMON_CHECK(head <= AMMON_ATTENTION_MAX_HEAD, "%s: head size %u exceeds %u", what, head,
+              AMMON_ATTENTION_MAX_HEAD);
+  AMMON_CHECK((((uintptr_t)k | (uintptr_t)v) & 15u) == 0, "%s: KV4 caches must be 16-byte aligned",
+              what);
+  const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
+  AMMON_CHECK(!v || !overlaps(k, bytes, v, bytes), "%s: key and value caches overlap", what);
+  return AMMON_OK;
+}
+
+// Rows k (and v unless v_cache is NULL) into KV4 caches at step->position + t.
+ammon_status kv4_store(ammon_runtime *rt, ammon_stream stream, const float *k, const float *v,
+                       uint32_t tokens, uint32_t kv_heads, uint32_t head, void *k_cache,
+                       void *v_cache, uint32_t seq, const ammon_decode_step *step,
+                       const char *what) {
+  ammon_status st = kv4_check(what, kv_heads, head, seq, k_cache, v_cache);
+  if (st != AMMON_OK) return st;
+  AMMON_CHECK((uint64_t)tokens * kv_heads < (1ull << 31), "%s: too many rows", what);
+  const size_t rows = (size_t)tokens * kv_heads * head * 4;
+  const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
+  for (const float *src : {k, v})
+    AMMON_CHECK(!src || (!overlaps(src, rows, k_cache, bytes) &&
+                         !(v_cache && overlaps(src, rows, v_cache, bytes))),
+                "%s: rows overlap a cache", what);
+  VALIDATE_ONLY();
+  ammon_k_kv4 p = {};
+  p.k = k;
+  p.v = v;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.step = (const ammon_k_step *)step;
+  p.tokens = tokens;
+  p.kv_heads = kv_heads;
+  p.head = head;
+  p.seq = seq;
+  return launch(rt, stream, rt->k.kv4_store, cdiv((uint64_t)tokens * kv_heads, kWorkgroup / 16),
+                v_cache ? 2 : 1, 0, p, what);
+}
+}  // namespace
+
+extern "C" {
+
+ammon_status ammon_kv4_store(ammon_runtime *rt, ammon_stream stream, const float *k,
+                             const float *v, uint32_t tokens, uint32_t kv_heads, uint32_t head,
+                             void *k_cache, void *v_cache, uint32_t seq,
+                             const ammon_decode_step *step) {
+  REQUIRE_RT();
+  AMMON_CHECK(k && v && k_cache && v_cache && step, "kv4_store: NULL rows, cache or step");
+  return kv4_store(rt, stream, k, v, tokens, kv_heads, head, k_cache, v_cache, seq, step,
+                   "kv4_store");
+}
+
+ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *k_cache,
+                            const void *v_cache, uint32_t kv_heads, uint32_t head, uint32_t seq,
+                            uint32_t first, uint32_t count, void *k_out, void *v_out,
+                            ammon_dtype out_dtype) {
+  REQUIRE_RT();
+  AMMON_CHECK(k_cache && k_out, "kv4_load: NULL cache or output");
+  AMMON_CHECK(!v_cache == !v_out, "kv4_load: a value cache and its output go together");
+  AMMON_CHECK(valid_dtype(out_dtype), "kv4_load: unknown output dtype %d", (int)out_dtype);
+  ammon_status st = kv4_check("kv4_load", kv_heads, head, seq, k_cache, v_cache);
+  if (st != AMMON_OK) return st;
+  AMMON_CHECK((uint64_t)first + count <= seq, "kv4_load: positions [%u, %u + %u) exceed %u", first,
+              first, count, seq);
+  AMMON_CHECK((((uintptr_t)k_out | (uintptr_t)v_out) & 15u) == 0,
+              "kv4_load: outputs must be 16-byte aligned");
+  AMMON_CHECK((uint64_t)count * kv_heads < (1ull << 34), "kv4_load: too many rows");
+  const size_t rows = (size_t)count * kv_heads * head * dsize(out_dtype);
+  const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
+  for (const void *out : {k_out, v_out})
+    AMMON_CHECK(!out || (!overlaps(out, rows, k_cache, bytes) &&
+                         !(v_cache && overlaps(out, rows, v_cache, bytes))),
+                "kv4_load: an output overlaps a cache");
+  AMMON_CHECK(!v_out || !overlaps(k_out, rows, v_out, rows), "kv4_load: the outputs overlap");
+  VALIDATE_ONLY();
+  ammon_k_kv4 p = {};
+  p.k_cache = (void *)k_cache;
+  p.v_cache = (void *)v_cache;
+  p.k_out = k_out;
+  p.v_out = v_out;
+  p.tokens = count;
+  p.kv_heads = kv_heads;
+  p.head = head;
+  p.seq = seq;
+  p.first = first;
+  p.out_dtype = (uint32_t)out_dtype;
+  return launch(rt, stream, rt->k.kv4_load, cdiv((uint64_t)count * kv_heads, kWorkgroup / 16),
+                v_out ? 2 : 1, 0, p, "kv4_load");
+}
+
 // ---- rope / cache store ----------------------------------------------------------------
 static ammon_status rope_impl(ammon_runtime *rt, ammon_stream stream, float *q, uint32_t q_heads,
                               const float *k_proj, uint32_t kv_heads, uint32_t head,
@@ -429,11 +533,29 @@ static ammon_status rope_impl(ammon_runtime *rt, ammon_stream stream, float *q, 
                               const char *what) {
   REQUIRE_RT();
   AMMON_CHECK(q && k_cache && step && table, "%s: NULL q, k cache, step or table", what);
-  AMMON_CHECK(valid_dtype(kv_dtype), "%s: unknown kv dtype %d", what, (int)kv_dtype);
+  AMMON_CHECK(valid_kv(kv_dtype), "%s: unknown kv dtype %d", what, (int)kv_dtype);
   AMMON_CHECK(head >= 2 && head % 2 == 0, "%s: head size %u must be even", what, head);
   AMMON_CHECK(q_heads > 0 && kv_heads > 0 && seq > 0, "%s: empty shape", what);
   const uint64_t q_numel = (uint64_t)q_heads * head, kv_dim = (uint64_t)kv_heads * head;
   AMMON_CHECK(kv_dim <= q_numel, "%s: kv width must be even and no wider than q", what);
+  if (kv_dtype == AMMON_KV4) {
+    AMMON_CHECK(k_proj, "%s: a KV4 row cannot be rotated in place", what);
+    ammon_status st = kv4_check(what, kv_heads, head, seq, k_cache, nullptr);
+    if (st != AMMON_OK) return st;
+    VALIDATE_ONLY();
+    ammon_k_kv4 p = {};
+    p.k = k_proj;
+    p.k_cache = k_cache;
+    p.step = (const ammon_k_step *)step;
+    p.q = q;
+    p.table = table;
+    p.kv_heads = kv_heads;
+    p.head = head;
+    p.seq = seq;
+    p.q_numel = (uint32_t)q_numel;
+    return launch(rt, stream, rt->k.kv4_rope_store,
+                  cdiv(q_numel / 2, kWorkgroup) + cdiv(kv_heads, kWorkgroup / 16), 1, 0, p, what);
+  }
   VALIDATE_ONLY();
   ammon_k_rope p = {q, k_proj, k_cache, (const ammon_k_step *)step, table,
                     (uint32_t)q_numel, (uint32_t)kv_dim, head, seq, (uint32_t)kv_dtype};
@@ -462,8 +584,11 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
                                const ammon_decode_step *step) {
   REQUIRE_RT();
   AMMON_CHECK(src && cache && step, "cache_store: NULL src, cache or step");
-  AMMON_CHECK(valid_dtype(kv_dtype), "cache_store: unknown dtype %d", (int)kv_dtype);
+  AMMON_CHECK(valid_kv(kv_dtype), "cache_store: unknown dtype %d", (int)kv_dtype);
   AMMON_CHECK(kv_heads > 0 && head > 0 && seq > 0, "cache_store: empty shape");
+  if (kv_dtype == AMMON_KV4)
+    return kv4_store(rt, stream, src, nullptr, 1, kv_heads, head, cache, nullptr, seq, step,
+                     "cache_store");
   VALIDATE_ONLY();
   const uint32_t kv_dim = kv_heads * head;
   ammon_k_cache_store p = {src, cache, (const ammon_k_step *)step, kv_dim, head, seq,
@@ -481,21 +606,41 @@ ammon_status attention_pass1(ammon_runtime *rt, ammon_stream stream, const float
                              uint32_t q_heads, const void *k_cache, const void *v_cache,
                              ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t head, uint32_t seq,
                              const ammon_decode_step *step, uint32_t split_len, float *partial,
-                             float *single_out) {
+                             float *single_out, const float *k_new = nullptr,
+                             const float *v_new = nullptr) {
   AMMON_CHECK(q && k_cache && v_cache && step && partial,
               "attention_partial: NULL q, cache, step or partial");
-  AMMON_CHECK(valid_dtype(kv_dtype), "attention_partial: unknown kv dtype %d", (int)kv_dtype);
+  AMMON_CHECK(valid_kv(kv_dtype), "attention_partial: unknown kv dtype %d", (int)kv_dtype);
   ammon_status st = attention_check(rt, "attention_partial", q_heads, kv_heads, head, seq, split_len);
   if (st != AMMON_OK) return st;
-  hipFunction_t f =
-      attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache, split_len);
+  hipFunction_t f = attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache,
+                                     split_len, k_new != nullptr);
+  AMMON_CHECK(f || kv_dtype != AMMON_KV4, "attention_partial: KV4 caches must be 16-byte aligned");
   AMMON_CHECK(f, "attention_partial: head %u needs an even width above 64", head);
   VALIDATE_ONLY();
   const uint32_t splits = ammon_attention_splits(seq, split_len);
   ammon_k_attention p = {q, k_cache, v_cache, (const ammon_k_step *)step, partial, single_out,
                          q_heads, kv_heads, head, seq, split_len, splits, 0, seq,
-                         single_out ? 1u : 0u, nullptr, 0, 0, 0, 0, 0, 1, 0};
+                         single_out ? 1u : 0u, nullptr, 0, 0, 0, 0, 0, 1, 0, k_new, v_new};
   return launch_att(rt, stream, f, splits, kv_heads, 1, p, "attention_partial");
+}
+
+// What an append asks beyond pass 1's own checks.
+ammon_status append_check(const char *what, const float *q, uint32_t q_heads, const float *k,
+                          const float *v, const void *k_cache, const void *v_cache,
+                          ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t head, uint32_t seq) {
+  AMMON_CHECK(kv_dtype == AMMON_KV4,
+              "%s: only a KV4 cache is appended to (qkv_rope_store stores the rows of others)", what);
+  AMMON_CHECK(k && v && k_cache && v_cache, "%s: NULL rows or cache", what);
+  ammon_status st = kv4_check(what, kv_heads, head, seq, k_cache, v_cache);
+  if (st != AMMON_OK) return st;
+  const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
+  const size_t row = (size_t)kv_heads * head * 4, qrow = (size_t)q_heads * head * 4;
+  for (const void *cache : {k_cache, v_cache})
+    AMMON_CHECK(!overlaps(k, row, cache, bytes) && !overlaps(v, row, cache, bytes) &&
+                    !overlaps(q, qrow, cache, bytes),
+                "%s: q or the rows overlap a cache", what);
+  return AMMON_OK;
 }
 }  // namespace
 
@@ -509,6 +654,21 @@ ammon_status ammon_attention_partial(ammon_runtime *rt, ammon_stream stream, con
   REQUIRE_RT();
   return attention_pass1(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head, seq,
                          step, split_len, partial, nullptr);
+}
+
+ammon_status ammon_attention_partial_append(ammon_runtime *rt, ammon_stream stream,
+                                            const float *q, uint32_t q_heads, const float *k,
+                                            const float *v, void *k_cache, void *v_cache,
+                                            ammon_dtype kv_dtype, uint32_t kv_heads,
+                                            uint32_t head, uint32_t seq,
+                                            const ammon_decode_step *step, uint32_t split_len,
+                                            float *partial) {
+  REQUIRE_RT();
+  ammon_status st = append_check("attention_partial_append", q, q_heads, k, v, k_cache, v_cache,
+                                 kv_dtype, kv_heads, head, seq);
+  if (st != AMMON_OK) return st;
+  return attention_pass1(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head, seq,
+                         step, split_len, partial, nullptr, k, v);
 }
 
 ammon_status ammon_attention_combine(ammon_runtime *rt, ammon_stream stream,
@@ -547,7 +707,8 @@ ammon_status ammon_attention_combine_warm(ammon_runtime *rt, ammon_stream stream
   VALIDATE_ONLY();
   ammon_k_attention p = {nullptr, nullptr, nullptr, (const ammon_k_step *)step, (float *)partial,
                          out, q_heads, 1, head, seq, split_len,
-                         ammon_attention_splits(seq, split_len), 0, seq, 0, nullptr, 0, 0, 0, 0, 0, 1, 0};
+                         ammon_attention_splits(seq, split_len), 0, seq, 0, nullptr, 0, 0, 0, 0, 0, 1, 0,
+                         nullptr, nullptr};
   const uint32_t grid = q_heads * cdiv(head, 8);
   if (next_w) {
     // The next GEMV (a RESIDUAL-mode ammon_gemv of next_rows x next_n) gives
@@ -603,16 +764,50 @@ uint32_t ammon_attention_default_split_for(ammon_runtime *rt, uint32_t q_heads,
   // 16; 2048: 9.7 against 10.6 at 32).
   uint32_t per_cu = 2, min_split = 16;
   if (rt && kv_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 8 && head > 0 &&
-      head <= AMMON_ATTENTION_MAX_HEAD && valid_dtype(kv_dtype)) {
+      head <= AMMON_ATTENTION_MAX_HEAD && valid_kv(kv_dtype)) {
     DeviceGuard guard(rt->device);
     hipFunction_t f =
         attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, nullptr, nullptr, 0);
     if (f) per_cu = std::min<uint32_t>(occupancy(rt, f, 0), 2);
     const uint32_t g = q_heads / kv_heads;
     if (kv_dtype == AMMON_BF16 && head == 128 && (g & (g - 1)) == 0) min_split = 64;
+    if (kv_dtype == AMMON_KV4) min_split = 128;  // its units' chunk
   }
   return default_split(rt, kv_heads, seq, per_cu, min_split);
 }
+
+}  // extern "C"
+
+namespace {
+// Both passes; with rows k and v, the append.
+ammon_status attention_decode(ammon_runtime *rt, ammon_stream stream, const float *q,
+                              uint32_t q_heads, const float *k, const float *v,
+                              const void *k_cache, const void *v_cache, ammon_dtype kv_dtype,
+                              uint32_t kv_heads, uint32_t head, uint32_t seq,
+                              const ammon_decode_step *step, uint32_t split_len, float *partial,
+                              size_t partial_bytes, float *out) {
+  AMMON_CHECK(partial_bytes >= ammon_attention_scratch_bytes(q_heads, head, seq, split_len),
+              "attention: partial scratch must be %zu bytes ([%u, %u, %u] fp32)",
+              ammon_attention_scratch_bytes(q_heads, head, seq, split_len), q_heads,
+              ammon_attention_splits(seq, split_len), head + 2);
+  ammon_status st = attention_pass1(rt, AMMON_STREAM_VALIDATE, q, q_heads, k_cache, v_cache,
+                                    kv_dtype, kv_heads, head, seq, step, split_len, partial,
+                                    nullptr, k, v);
+  if (st != AMMON_OK) return st;
+  st = ammon_attention_combine(rt, AMMON_STREAM_VALIDATE, partial, q_heads, head, seq, step,
+                               split_len, out);
+  if (st != AMMON_OK) return st;
+  VALIDATE_ONLY();
+  // one split covers the cache: one launch, pass 1 writes out
+  const bool single = ammon_attention_splits(seq, split_len) == 1;
+  st = attention_pass1(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head, seq,
+                       step, split_len, partial, single ? out : nullptr, k, v);
+  if (st != AMMON_OK || single) return st;
+  return ammon_attention_combine(rt, stream, partial, q_heads, head, seq, step, split_len, out);
+}
+}  // namespace
+
+extern "C" {
 
 ammon_status ammon_attention_decode(ammon_runtime *rt, ammon_stream stream, const float *q,
                                     uint32_t q_heads, const void *k_cache, const void *v_cache,
@@ -621,25 +816,23 @@ ammon_status ammon_attention_decode(ammon_runtime *rt, ammon_stream stream, cons
                                     uint32_t split_len, float *partial, size_t partial_bytes,
                                     float *out) {
   REQUIRE_RT();
-  AMMON_CHECK(partial_bytes >= ammon_attention_scratch_bytes(q_heads, head, seq, split_len),
-              "attention: partial scratch must be %zu bytes ([%u, %u, %u] fp32)",
-              ammon_attention_scratch_bytes(q_heads, head, seq, split_len), q_heads,
-              ammon_attention_splits(seq, split_len), head + 2);
-  ammon_status st = ammon_attention_partial(rt, AMMON_STREAM_VALIDATE, q, q_heads, k_cache,
-                                            v_cache, kv_dtype, kv_heads, head, seq, step,
-                                            split_len, partial);
+  return attention_decode(rt, stream, q, q_heads, nullptr, nullptr, k_cache, v_cache, kv_dtype,
+                          kv_heads, head, seq, step, split_len, partial, partial_bytes, out);
+}
+
+ammon_status ammon_attention_decode_append(ammon_runtime *rt, ammon_stream stream,
+                                           const float *q, uint32_t q_heads, const float *k,
+                                           const float *v, void *k_cache, void *v_cache,
+                                           ammon_dtype kv_dtype, uint32_t kv_heads,
+                                           uint32_t head, uint32_t seq,
+                                           const ammon_decode_step *step, uint32_t split_len,
+                                           float *partial, size_t partial_bytes, float *out) {
+  REQUIRE_RT();
+  ammon_status st = append_check("attention_append", q, q_heads, k, v, k_cache, v_cache, kv_dtype,
+                                 kv_heads, head, seq);
   if (st != AMMON_OK) return st;
-  st = ammon_attention_combine(rt, AMMON_STREAM_VALIDATE, partial, q_heads, head, seq, step,
-                               split_len, out);
-  if (st != AMMON_OK) return st;
-  VALIDATE_ONLY();
-  if (ammon_attention_splits(seq, split_len) == 1)  // one launch: pass 1 writes out
-    return attention_pass1(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head,
-                           seq, step, split_len, partial, out);
-  st = ammon_attention_partial(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head,
-                               seq, step, split_len, partial);
-  if (st != AMMON_OK) return st;
-  return ammon_attention_combine(rt, stream, partial, q_heads, head, seq, step, split_len, out);
+  return attention_decode(rt, stream, q, q_heads, k, v, k_cache, v_cache, kv_dtype, kv_heads, head,
+                          seq, step, split_len, partial, partial_bytes, out);
 }
 
 // ---- prompt prefill ---------------------------------------------------------------------
@@ -657,7 +850,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
   REQUIRE_RT();
   AMMON_CHECK(q && k_cache && v_cache && step && partial && out,
               "attention_prefill: NULL q, cache, step, partial or out");
-  AMMON_CHECK(valid_dtype(kv_dtype), "attention_prefill: unknown kv dtype %d", (int)kv_dtype);
+  AMMON_CHECK(valid_kv(kv_dtype), "attention_prefill: unknown kv dtype %d", (int)kv_dtype);
   AMMON_CHECK(tokens > 0, "attention_prefill: no query tokens");
   ammon_status st = attention_check(rt, "attention_prefill", q_heads, kv_heads, head, seq, split_len);
   if (st != AMMON_OK) return st;
@@ -670,6 +863,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
               "attention_prefill: q, partial and out must not overlap");
   hipFunction_t f =
       attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache, split_len);
+  AMMON_CHECK(f || kv_dtype != AMMON_KV4, "attention_prefill: KV4 caches must be 16-byte aligned");
   AMMON_CHECK(f, "attention_prefill: head %u needs an even width above 64", head);
   VALIDATE_ONLY();
   // the partial layout and the grid cover ctx positions: [tokens][q_heads][splits][head + 2];
@@ -678,7 +872,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
   const uint32_t splits = ammon_attention_splits(ctx, split_len);
   ammon_k_attention p = {q, k_cache, v_cache, (const ammon_k_step *)step, partial, out,
                          q_heads, kv_heads, head, seq, split_len, splits, 0, ctx, 0, nullptr, 0, 0, 0, 0, 0,
-                         tokens, 0};
+                         tokens, 0, nullptr, nullptr};
   const uintptr_t bits = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache;
   const PrefillPlan plan = prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, kv_dtype,
                                         (bits & 15u) == 0 && ((uintptr_t)partial & 7u) == 0);

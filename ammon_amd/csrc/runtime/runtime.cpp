@@ -28,6 +28,7 @@ AMMON_BLOB(attention)
 AMMON_BLOB(gemv)
 AMMON_BLOB(misc)
 AMMON_BLOB(prefill)
+AMMON_BLOB(kv4)
 
 namespace ammon_rt {
 
@@ -80,7 +81,7 @@ static ammon_status load_kernels(ammon_runtime *rt) {
   } blobs[] = {{"embed", ammon_co_embed}, {"norm", ammon_co_norm},
                {"rope", ammon_co_rope},   {"attention", ammon_co_attention},
                {"gemv", ammon_co_gemv},   {"misc", ammon_co_misc},
-               {"prefill", ammon_co_prefill}};
+               {"prefill", ammon_co_prefill}, {"kv4", ammon_co_kv4}};
   constexpr int kModules = (int)(sizeof(blobs) / sizeof(blobs[0]));
   hipModule_t mods[kModules];
   for (int i = 0; i < kModules; ++i) {
@@ -177,6 +178,15 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_gemm_bf16_%s_t16_r2", modes[m]);
     R(6, name, k.gemm_big_t16[m]);
   }
+  R(7, "ammon_kv4_store", k.kv4_store);
+  R(7, "ammon_kv4_rope_store", k.kv4_rope_store);
+  R(7, "ammon_kv4_load", k.kv4_load);
+  for (int a = 0; a < 2; ++a)
+    for (int n = 0; n < kKv4Groups; ++n) {
+      char name[96];
+      snprintf(name, sizeof name, "ammon_kv4_partial_%sn%d", a ? "append_" : "", n + 1);
+      R(7, name, k.kv4_partial[a][n]);
+    }
 #undef R
   return AMMON_OK;
 }
@@ -495,6 +505,16 @@ ammon_status ammon_kv_unpermute(const void *head_major, void *pos_major, uint32_
 ammon_status ammon_kv_permute(const void *pos_major, void *head_major, uint32_t kv_heads,
                               uint32_t seq, uint32_t head, uint32_t elem_bytes) {
   return kv_move(pos_major, head_major, kv_heads, seq, head, elem_bytes, false);
+}
+
+size_t ammon_kv_cache_bytes(ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t seq, uint32_t head) {
+  const size_t rows = (size_t)kv_heads * seq;
+  switch (kv_dtype) {
+    case AMMON_F32: return rows * head * 4;
+    case AMMON_BF16: return rows * head * 2;
+    case AMMON_KV4: return rows * kKv4RowBytes * (((size_t)head + 31) / 32);
+  }
+  return 0;
 }
 
 uint32_t ammon_attention_splits(uint32_t seq, uint32_t split_len) {

@@ -17,7 +17,8 @@
  *   - Every call returns an ammon_status.  On failure nothing is launched and
  *     ammon_last_error() returns a message on the calling thread.
  *   - Storage dtypes: AMMON_F32, or AMMON_BF16 (bit patterns, round to nearest
- *     even when written).  Activations are always fp32.
+ *     even when written); KV caches also AMMON_KV4 (4 bits a number, below).
+ *     Activations are always fp32.
  *   - KV caches are head-major per layer: [kv_heads, seq, head].  The
  *     reference is position-major [seq, kv_heads, head]
  *     (reference src/modules.rs:37-71); ammon_kv_unpermute converts.
@@ -48,7 +49,9 @@ typedef enum ammon_status {
   AMMON_E_NO_DEVICE = 4   /* no usable gfx950 device */
 } ammon_status;
 
-typedef enum ammon_dtype { AMMON_F32 = 0, AMMON_BF16 = 1 } ammon_dtype;
+/* AMMON_KV4 is a storage type of KV caches alone (2 and 3 are left to the C++
+ * layer's index types). */
+typedef enum ammon_dtype { AMMON_F32 = 0, AMMON_BF16 = 1, AMMON_KV4 = 4 } ammon_dtype;
 
 typedef enum ammon_copy_kind {
   AMMON_COPY_H2D = 1,
@@ -167,6 +170,8 @@ ammon_status ammon_kv_unpermute(const void *head_major, void *pos_major, uint32_
                                 uint32_t seq, uint32_t head, uint32_t elem_bytes);
 ammon_status ammon_kv_permute(const void *pos_major, void *head_major, uint32_t kv_heads,
                               uint32_t seq, uint32_t head, uint32_t elem_bytes);
+/* Bytes of one layer's key (or value) cache; 0 for an unknown dtype. */
+size_t ammon_kv_cache_bytes(ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t seq, uint32_t head);
 /* Flash-decoding split count and scratch size ([q_heads, splits, head + 2]
  * fp32; reference src/blocks.rs:317-320 with a caller-chosen split length). */
 uint32_t ammon_attention_splits(uint32_t seq, uint32_t split_len);
@@ -224,6 +229,44 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
                                ammon_dtype kv_dtype, uint32_t seq,
                                const ammon_decode_step *step);
 
+/* ---- 4-bit KV cache (AMMON_KV4) -------------------------------------------
+ * No counterpart in the reference.  A row (one kv head, one position; head at
+ * most 128) holds its numbers in groups of 32, the last one shorter where
+ * head is no multiple of 32.  A group has a scale s and a bias b (fp16) and a
+ * code c in 0..15 per number, which stands for fp16(s (16 + c) + b).  Storing
+ * fp32 numbers x (each step rounds to fp32):
+ *   x = min(max(x, -16384), 16384)
+ *   s = fp16((max x - min x) / 15),  b = fp16(min x - 16 s)
+ *   c = clamp(rint((x - b) (1 / s) - 16), 0, 15), 0 where s = 0
+ * A group with a number that is not finite reads back as NaN.  A stored number
+ * is off by at most about half a step s, i.e. 1/30 of its group's range.
+ *
+ * Memory of one cache (20 ceil(head / 32) bytes a row, 16-byte aligned): the
+ * codes as 32-bit words [kv_heads, seq, 4, ceil(head / 32)], word (p, j) with
+ * numbers 32 j + 8 p .. + 7, number + e in bits 4 n .. 4 n + 3, n = e / 2 for
+ * even e and 4 + e / 2 for odd e; then words s | b << 16 [kv_heads, seq,
+ * ceil(head / 32)].
+ *
+ * ammon_rope_store and ammon_cache_store write rows of such a cache, the
+ * attention entries read it (16 query heads' width is always computed, so any
+ * group up to 8 costs the same); ammon_rope, ammon_qkv_rope_store and its
+ * prefill form do not take it: ammon_qkv_rope and ammon_prefill_qkv_rope give
+ * the rows, ammon_attention_decode_append and ammon_kv4_store take them. */
+
+/* Rows k, v [tokens, kv_heads, head] into the caches at positions
+ * step->position + t; a position at or past seq is left out. */
+ammon_status ammon_kv4_store(ammon_runtime *rt, ammon_stream stream, const float *k,
+                             const float *v, uint32_t tokens, uint32_t kv_heads, uint32_t head,
+                             void *k_cache, void *v_cache, uint32_t seq,
+                             const ammon_decode_step *step);
+/* The numbers of positions [first, first + count), first + count <= seq, as
+ * [kv_heads, count, head] fp32 or bf16 (16-byte aligned).  v_cache and v_out
+ * may both be NULL. */
+ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *k_cache,
+                            const void *v_cache, uint32_t kv_heads, uint32_t head, uint32_t seq,
+                            uint32_t first, uint32_t count, void *k_out, void *v_out,
+                            ammon_dtype out_dtype);
+
 /* attention_partial (reference src/kernels.rs:228-345): split-K pass over
  * the head-major cache, one workgroup per (split, kv head) serving all
  * q_heads / kv_heads query heads.  partial is [q_heads, splits, head + 2]
@@ -270,6 +313,26 @@ ammon_status ammon_attention_decode(ammon_runtime *rt, ammon_stream stream, cons
                                     uint32_t seq, const ammon_decode_step *step,
                                     uint32_t split_len, float *partial, size_t partial_bytes,
                                     float *out);
+
+/* The decode step of a KV4 cache (kv_dtype AMMON_KV4; others' rows are stored
+ * by ammon_qkv_rope_store): the position's own rows k, v [kv_heads, head] are
+ * stored at step->position, as ammon_kv4_store stores them, and attended to
+ * with the positions before, in the launches of ammon_attention_decode (or
+ * ammon_attention_partial): the unit that has the position stores its row. */
+ammon_status ammon_attention_partial_append(ammon_runtime *rt, ammon_stream stream,
+                                            const float *q, uint32_t q_heads, const float *k,
+                                            const float *v, void *k_cache, void *v_cache,
+                                            ammon_dtype kv_dtype, uint32_t kv_heads,
+                                            uint32_t head, uint32_t seq,
+                                            const ammon_decode_step *step, uint32_t split_len,
+                                            float *partial);
+ammon_status ammon_attention_decode_append(ammon_runtime *rt, ammon_stream stream,
+                                           const float *q, uint32_t q_heads, const float *k,
+                                           const float *v, void *k_cache, void *v_cache,
+                                           ammon_dtype kv_dtype, uint32_t kv_heads,
+                                           uint32_t head, uint32_t seq,
+                                           const ammon_decode_step *step, uint32_t split_len,
+                                           float *partial, size_t partial_bytes, float *out);
 
 /* No counterpart in the reference.  For callers that cannot allocate device
  * memory (code under HIP graph capture, tight serving loops, harnesses that
