@@ -76,7 +76,9 @@ typedef struct {
                                NaN output, no partial (seq for decode; the
                                positions the grid and scratch cover for prefill) */
   uint32_t single_out;      /* pass 1 with splits == 1 writes out (the merge's
-                               result) instead of the partial; no pass 2 */
+                               result) instead of the partial; no pass 2.  KV4
+                               prefill tiles: a row with one live split, which the
+                               merge then leaves alone */
   /* Merge only, optional (NULL: none): the next GEMV's weights.  Merge
    * workgroup i reads one dword of every 128-byte line of row block i
    * (rows [i warm_rows, +warm_rows), bytes [0, warm_bytes) of each, rows

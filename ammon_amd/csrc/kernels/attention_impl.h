@@ -888,6 +888,7 @@ AMMON_DEV void attention_combine_wave(const ammon_k_attention &p, uint32_t h) {
     return;
   }
   const uint32_t live = min(pos / p.split_len + 1, p.splits);
+  if (live == 1 && p.single_out) return;  // written by pass 1
   const float *base = p.partial + (size_t)h * p.splits * slot;
   float m = -INFINITY;
   for (uint32_t s = lane; s < live; s += COMB_SPLIT_LANES) m = fmaxf(m, base[(size_t)s * slot + head]);

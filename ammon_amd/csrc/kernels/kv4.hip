@@ -1,6 +1,8 @@
-// kv4.hip -- kernels of the 4-bit KV cache: rows stored and read back, and split-K
-// decode attention (units of kv4_attention_impl.h; pass 2 is attention.hip's).
+// kv4.hip -- kernels of the 4-bit KV cache: rows stored and read back, split-K decode
+// attention (units of kv4_attention_impl.h) and prefill attention (tiles of
+// kv4_prefill_impl.h); the merges are attention.hip's.
 #include "kv4_attention_impl.h"
+#include "kv4_prefill_impl.h"
 
 // Rows [tokens, kv_heads, head] (fp32) into the cache at position step->position + t:
 // 16 lanes a row, 16 rows a workgroup, blockIdx.y 0 the keys, 1 the values.  Bytes
@@ -64,7 +66,7 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_load(ammon_k_kv
   void *out = blockIdx.y ? p.v_out : p.k_out;
   const uint32_t w = kv4_codes(cache, p.seq, ng, g, t)[piece * ng + j];
   const uint32_t sb = kv4_scales(cache, p.kv_heads, p.seq, ng, g, t)[j];
-  const f16x8 v = kv4_numbers(w, sb);
+  const f16x8 v = kv4_numbers(w, sb, Kv4Bits());
   const size_t at = (size_t)r * p.head + 8 * i;
   if (p.head % 8 == 0 && p.out_dtype == AMMON_K_F32) {
     float *to = (float *)out + at;
@@ -105,3 +107,20 @@ KV4_PARTIAL_NG(1)
 KV4_PARTIAL_NG(2)
 KV4_PARTIAL_NG(3)
 KV4_PARTIAL_NG(4)
+
+// Prefill tiles: one workgroup of two groups of four waves per (256 query rows, split,
+// kv head), one per CU.
+#define KV4_PREFILL(NG)                                                                     \
+  extern "C" __global__ __launch_bounds__(KV4_PF_WG, 2) void ammon_kv4_prefill_n##NG(       \
+      const ammon_k_step *step, ammon_k_attention p_) {                                     \
+    using Tile = Kv4PrefillTile<NG>;                                                        \
+    __shared__ u32x4 lds[Tile::LDS_BYTES / 16];                                             \
+    ammon_k_attention p = p_;                                                               \
+    p.step = step;                                                                          \
+    Tile unit;                                                                              \
+    unit.run(p, (char *)lds);                                                               \
+  }
+KV4_PREFILL(1)
+KV4_PREFILL(2)
+KV4_PREFILL(3)
+KV4_PREFILL(4)

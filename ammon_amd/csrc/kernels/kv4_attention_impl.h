@@ -158,6 +158,8 @@ struct Kv4Partial {
     float *s_L = s_M + KV4_MAX_GROUP;                    // [8] workgroup sums
     const uint32_t h = lane & 15, grp = lane >> 4, head = p.head;
 
+    const Kv4Bits bits;
+    const float minus1 = kv4_minus1();
     // q^T as the B operand, fp16 hi + lo of q 2^(14 - e), |q| < 2^e
     float qmax = 0.f;
 #pragma unroll
@@ -170,10 +172,11 @@ struct Kv4Partial {
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = ldexpf(qraw[j][e], 14 - qe);
-        qhi[j][e] = (_Float16)x;
-        qlo[j][e] = (_Float16)(x - (float)qhi[j][e]);
+      for (int e = 0; e < 8; e += 2) {
+        f16x2 hi, lo;
+        kv4_parts(ldexpf(qraw[j][e], 14 - qe), ldexpf(qraw[j][e + 1], 14 - qe), minus1, hi, lo);
+        qhi[j][e] = hi[0], qhi[j][e + 1] = hi[1];
+        qlo[j][e] = lo[0], qlo[j][e + 1] = lo[1];
       }
     // log2(e) / sqrt(head), and q's scale back
     const float scale2 = ldexpf(1.4426950408889634f / sqrtf((float)head), qe - 14);
@@ -228,7 +231,7 @@ struct Kv4Partial {
         f32x4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          const f16x8 a = kv4_numbers(w[j], ps[j]);
+          const f16x8 a = kv4_numbers(w[j], ps[j], bits);
           hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qhi[j], hi, 0, 0, 0);
           lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qlo[j], lo, 0, 0, 0);
         }
@@ -254,10 +257,13 @@ struct Kv4Partial {
       f16x8 ph, pl;
       float pw[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pw[e] = __builtin_amdgcn_exp2f(sc[e / 4][e % 4] - mu);
-        ph[e] = (_Float16)pw[e];
-        pl[e] = (_Float16)(pw[e] - (float)ph[e]);
+      for (int e = 0; e < 8; ++e) pw[e] = __builtin_amdgcn_exp2f(sc[e / 4][e % 4] - mu);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        f16x2 hi, lo;
+        kv4_parts(pw[e], pw[e + 1], minus1, hi, lo);
+        ph[e] = hi[0], ph[e + 1] = hi[1];
+        pl[e] = lo[0], pl[e + 1] = lo[1];
       }
       l += ((pw[0] + pw[1]) + (pw[2] + pw[3])) + ((pw[4] + pw[5]) + (pw[6] + pw[7]));
       // values: words of positions e = 4 T + r, row 16 T + 4 r + grp
@@ -294,7 +300,7 @@ struct Kv4Partial {
         f16x8 a;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const f16x2 v = __builtin_elementwise_fma(kv4_pair<decltype(nib)::value>(x[u]), vs2[u], vb2[u]);
+          const f16x2 v = __builtin_elementwise_fma(kv4_pair<decltype(nib)::value>(x[u], bits), vs2[u], vb2[u]);
           a[2 * u] = v[0];
           a[2 * u + 1] = v[1];
         }

@@ -38,21 +38,42 @@ AMMON_DEV uint32_t kv4_groups(uint32_t head) { return (head + 31) / 32; }
 // Number + e of a word: its code's place.
 constexpr int kv4_nibble(int e) { return e / 2 + 4 * (e & 1); }
 
-// Codes `shift` nibbles up of a word's low and high half, as 16 + c.
-template <int NIB> AMMON_DEV f16x2 kv4_pair(uint32_t w) {
+// The mask of a code's bits in an fp16 mantissa and the fp16 number 16, twice, in
+// registers of the two kinds that one v_and_or_b32 takes (as literals they were two
+// instructions).
+struct Kv4Bits {
+  uint32_t mask = 0x03c003c0u, base = 0x4c004c00u;
+  AMMON_DEV Kv4Bits() { asm("" : "+s"(mask), "+v"(base)); }
+};
+
+// Codes NIB nibbles up of a word's low and high half, as 16 + c.
+template <int NIB> AMMON_DEV f16x2 kv4_pair(uint32_t w, const Kv4Bits &k) {
   const uint32_t at = NIB == 0 ? w << 6 : NIB == 1 ? w << 2 : NIB == 2 ? w >> 2 : w >> 6;
-  return __builtin_bit_cast(f16x2, (at & 0x03c003c0u) | 0x4c004c00u);
+  return __builtin_bit_cast(f16x2, (at & k.mask) | k.base);
 }
 
 // The eight numbers of a word with scale | bias sb, in order.
-AMMON_DEV f16x8 kv4_numbers(uint32_t w, uint32_t sb) {
+AMMON_DEV f16x8 kv4_numbers(uint32_t w, uint32_t sb, const Kv4Bits &k) {
   const f16x2 p = __builtin_bit_cast(f16x2, sb);
   const f16x2 s = {p[0], p[0]}, b = {p[1], p[1]};
-  const f16x2 v0 = __builtin_elementwise_fma(kv4_pair<0>(w), s, b);
-  const f16x2 v1 = __builtin_elementwise_fma(kv4_pair<1>(w), s, b);
-  const f16x2 v2 = __builtin_elementwise_fma(kv4_pair<2>(w), s, b);
-  const f16x2 v3 = __builtin_elementwise_fma(kv4_pair<3>(w), s, b);
+  const f16x2 v0 = __builtin_elementwise_fma(kv4_pair<0>(w, k), s, b);
+  const f16x2 v1 = __builtin_elementwise_fma(kv4_pair<1>(w, k), s, b);
+  const f16x2 v2 = __builtin_elementwise_fma(kv4_pair<2>(w, k), s, b);
+  const f16x2 v3 = __builtin_elementwise_fma(kv4_pair<3>(w, k), s, b);
   return f16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+
+// Two floats as fp16 hi + lo, 22 bits: lo by one mixed-precision multiply-add each (the
+// factor is hidden from the compiler, which would make a conversion and a subtraction).
+AMMON_DEV void kv4_parts(float a, float b, float minus1, f16x2 &hi, f16x2 &lo) {
+  hi = __builtin_convertvector(f32x2{a, b}, f16x2);
+  lo = __builtin_convertvector(
+      f32x2{__builtin_fmaf((float)hi[0], minus1, a), __builtin_fmaf((float)hi[1], minus1, b)}, f16x2);
+}
+AMMON_DEV float kv4_minus1() {
+  float f = -1.f;
+  asm("" : "+s"(f));
+  return f;
 }
 
 // A row as 16 lanes quantise it: lane i (of aligned 16) has numbers 8 i .. + 7 in x

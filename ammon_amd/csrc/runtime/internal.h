@@ -63,10 +63,12 @@ struct Kernels {
   hipFunction_t gemm_big[2][2][kGemvModes] = {};
   hipFunction_t gemm_big_t16[kGemvModes] = {};  // 16 tokens, RT 2
   // 4-bit KV cache: rows written and read back, decode pass 1 [plain / append][groups - 1]
+  // and prefill [groups - 1]
   hipFunction_t kv4_store = nullptr;
   hipFunction_t kv4_rope_store = nullptr;
   hipFunction_t kv4_load = nullptr;
   hipFunction_t kv4_partial[2][kKv4Groups] = {};
+  hipFunction_t kv4_prefill[kKv4Groups] = {};  // prefill tiles
 };
 
 // LDS per compute unit on gfx950 (bytes); bounds resident GEMV workgroups.

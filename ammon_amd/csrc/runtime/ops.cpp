@@ -51,11 +51,12 @@ ammon_status launch(ammon_runtime *rt, ammon_stream s, hipFunction_t f, uint32_t
 // The attention kernels take the DecodeStep pointer as a leading scalar
 // argument (preloaded into SGPRs), then the parameter struct.
 ammon_status launch_att(ammon_runtime *rt, ammon_stream s, hipFunction_t f, uint32_t gx,
-                        uint32_t gy, uint32_t gz, ammon_k_attention &params, const char *what) {
+                        uint32_t gy, uint32_t gz, ammon_k_attention &params, const char *what,
+                        uint32_t threads = kWorkgroup) {
   DeviceGuard guard(rt->device);
   hipStream_t st = s ? (hipStream_t)s : rt->stream;
   void *args[] = {&params.step, &params};
-  hipError_t e = hipModuleLaunchKernel(f, gx, gy, gz, kWorkgroup, 1, 1, 0, st, args, nullptr);
+  hipError_t e = hipModuleLaunchKernel(f, gx, gy, gz, threads, 1, 1, 0, st, args, nullptr);
   if (e != hipSuccess) return hip_error(e, what);
   return AMMON_OK;
 }
@@ -294,6 +295,8 @@ struct PrefillPlan {
   hipFunction_t f = nullptr;  // NULL: decode's units
   uint32_t split_len = 0, splits = 0, grid = 0;
   uint32_t pair = 0;  // ammon_k_attention::pair
+  uint32_t threads = kWorkgroup;
+  uint32_t whole_rows = 0;  // rows with one live split write their result themselves
 };
 
 // Tiles need whole 16-byte pieces of cache rows.  Their splits fill the
@@ -315,7 +318,6 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
                          uint32_t head, uint32_t ctx, uint32_t scratch_splits, ammon_dtype kv_dtype,
                          bool aligned) {
   PrefillPlan plan;
-  if (kv_dtype == AMMON_KV4) return plan;
   const bool bf = kv_dtype == AMMON_BF16;
   const uint32_t g = q_heads / kv_heads;
   const uint64_t rows = (uint64_t)tokens * g, krow = head * dsize(kv_dtype);
@@ -351,6 +353,55 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
   if (per_cu >= 2 && cus % 8 == 0 && plan.grid > cus && plan.grid <= 2 * cus) plan.pair = cus / 8;
   plan.split_len = split_len;
   plan.splits = splits;
+  return plan;
+}
+
+// The same for a KV4 cache (kv4_prefill_impl.h): tiles of 256 rows, one workgroup per
+// CU.  The number of splits is the one with the least estimated time, of
+//   chunks  the longest workgroup's, or what each CU gets of all of them (with causal
+//           masking a tile sees half of its prompt: splits even that out),
+//   ends    a workgroup's first and last steps; workgroups of a second round have theirs
+//           after the first's,
+//   merge   a launch, and the partials written and read; rows of which one split sees
+//           anything write their result themselves.
+// Measured at 32 q / 8 kv heads of 128 (units, tiles, us): 64 tokens after 500: 15, 32; 64
+// after 4000: 78, 43 (16 kv heads, 40 tokens: 84, 43); 300 after 3000: 314, 50; 2048: 852,
+// 98 in one split, 101 in two; heads of 64: 64 after 500: 12, 22; 64 after 4000: 52, 36.
+PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                             uint32_t head, uint32_t ctx, uint32_t scratch_splits, bool aligned) {
+  PrefillPlan plan;
+  const uint32_t g = q_heads / kv_heads, ng = cdiv(head, 32);
+  const uint64_t rows = (uint64_t)tokens * g, tiles = cdiv(rows, 256);
+  if (!aligned || rows >= (1ull << 31)) return plan;
+  const double chunk_ns = 500 + 560 * ng;
+  const double seen = ctx - tokens / 2.0;  // positions a token sees, on average
+  const double unit_ns = 6e3 + tokens * kv_heads * seen * (0.015 + 0.007 * ng);
+  if (10e3 + chunk_ns >= unit_ns) return plan;  // (the shortest tiles: a small call asks no further)
+  const double cus = std::max(rt->info.compute_units, 1);
+  double best = unit_ns;
+  for (uint32_t n = 1; n <= std::min<uint32_t>(scratch_splits, 64); ++n) {
+    const uint32_t len = cdiv(cdiv(ctx, n), 64) * 64;
+    if (len > kPrefillMaxSplit) continue;
+    if (n > 1 && len < 256) break;
+    const uint32_t splits = cdiv(ctx, len);
+    const double units = (double)tiles * kv_heads * splits;
+    if (units >= (1u << 30)) break;
+    const double longest = cdiv(std::min(len, ctx), 64);
+    const double all = (double)tiles * kv_heads * (seen / 64 + 0.5 * splits) / cus;
+    // (a second round of workgroups starts where the first's end, from its beginning)
+    double ns = 10e3 + chunk_ns * std::max(longest, all + (units > cus ? 0.15 * longest : 0)) +
+                (units > cus ? 8e3 : 0);
+    if (splits > 1)
+      ns += 5e3 + tokens * q_heads * (head + 2.0) * 8 * (splits * seen / ctx) / 3e3;
+    if (ns >= best) continue;
+    best = ns;
+    plan.f = rt->k.kv4_prefill[ng - 1];
+    plan.split_len = len;
+    plan.splits = splits;
+    plan.grid = cdiv((uint64_t)tiles * kv_heads * splits, 8) * 8;
+    plan.threads = 2 * kWorkgroup;
+    plan.whole_rows = 1;
+  }
   return plan;
 }
 
@@ -874,13 +925,17 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
                          q_heads, kv_heads, head, seq, split_len, splits, 0, ctx, 0, nullptr, 0, 0, 0, 0, 0,
                          tokens, 0, nullptr, nullptr};
   const uintptr_t bits = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache;
-  const PrefillPlan plan = prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, kv_dtype,
-                                        (bits & 15u) == 0 && ((uintptr_t)partial & 7u) == 0);
+  const bool aligned = (bits & 15u) == 0 && ((uintptr_t)partial & 7u) == 0;
+  const PrefillPlan plan =
+      kv_dtype == AMMON_KV4
+          ? kv4_prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, aligned)
+          : prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, kv_dtype, aligned);
   if (plan.f) {
     p.split_len = plan.split_len;
     p.splits = plan.splits;
     p.pair = plan.pair;
-    st = launch_att(rt, stream, plan.f, plan.grid, 1, 1, p, "attention_prefill");
+    p.single_out = plan.whole_rows;
+    st = launch_att(rt, stream, plan.f, plan.grid, 1, 1, p, "attention_prefill", plan.threads);
     if (st != AMMON_OK || p.splits == 1) return st;
   } else {
     // one split: the units write the merge's result themselves, as in decode

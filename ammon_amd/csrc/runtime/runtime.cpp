@@ -187,6 +187,11 @@ static ammon_status load_kernels(ammon_runtime *rt) {
       snprintf(name, sizeof name, "ammon_kv4_partial_%sn%d", a ? "append_" : "", n + 1);
       R(7, name, k.kv4_partial[a][n]);
     }
+  for (int n = 0; n < kKv4Groups; ++n) {
+    char name[96];
+    snprintf(name, sizeof name, "ammon_kv4_prefill_n%d", n + 1);
+    R(7, name, k.kv4_prefill[n]);
+  }
 #undef R
   return AMMON_OK;
 }

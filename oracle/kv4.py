@@ -110,13 +110,16 @@ def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, first: int) -> np.nda
     [kv_heads, >= first + tokens, head]."""
     q = np.asarray(q, np.float64)
     tokens, heads, head = q.shape
-    g = heads // k.shape[0]
+    g, ctx = heads // k.shape[0], first + tokens
+    seen = np.arange(ctx)[None, :] <= first + np.arange(tokens)[:, None]
     out = np.empty_like(q)
     with np.errstate(invalid="ignore"):
-        for t in range(tokens):
-            for h in range(heads):
-                kk, vv = k[h // g, :first + t + 1], v[h // g, :first + t + 1]
-                s = kk @ q[t, h] / np.sqrt(head)
-                p = np.exp(s - s.max())
-                out[t, h] = p @ vv / p.sum()
+        for h in range(heads):
+            kk, vv = k[h // g, :ctx], v[h // g, :ctx]
+            s = np.where(seen, q[:, h] @ kk.T / np.sqrt(head), -np.inf)
+            p = np.exp(s - s.max(-1, keepdims=True))  # NaN where a seen score is
+            bad = ~np.isfinite(vv)
+            o = p @ np.where(bad, 0, vv) / p.sum(-1, keepdims=True)
+            # a number that is not finite is NaN (a group is), and so is its sum wherever it is seen
+            out[:, h] = np.where(seen.astype(np.float64) @ bad > 0, np.nan, o)
     return out

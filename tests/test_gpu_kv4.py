@@ -357,16 +357,97 @@ def test_decode_steps_in_a_graph(rt):
     call("ammon_stream_destroy", rt.handle, stream)
 
 
+def prefill(rt, q, c, start, split, ctx=None, pad=64):
+    tokens, heads = q.shape[:2]
+    ctx = ctx or start + tokens
+    nbytes = int(lib.ammon_attention_prefill_scratch_bytes(tokens, heads, c.head, ctx, split))
+    part, out = rt.alloc(nbytes + pad * 4), rt.alloc(q.nbytes + pad * 4)
+    for buf, n in ((part, nbytes // 4), (out, q.size)):
+        rt.fill(buf, F32, n + pad, 7.0)
+    call("ammon_attention_prefill", rt.handle, None, up(rt, q), tokens, heads, *c.dev, KV4,
+         c.kv_heads, c.head, c.seq, rt.step(0, start), ctx, split, part, nbytes, out)
+    got = out.download(q.size + pad)
+    assert np.all(got[q.size:] == 7.0) and np.all(part.download(nbytes // 4 + pad)[nbytes // 4:] == 7.0)
+    return got[:q.size].reshape(q.shape)
+
+
 @pytest.mark.parametrize("heads,kv_heads,head", SHAPES)
 @pytest.mark.parametrize("start,tokens", [(0, 1), (0, 5), (0, 70), (61, 40), (300, 3)])
 def test_prefill(rt, heads, kv_heads, head, start, tokens):
-    seq, ctx = 400, start + tokens
-    c = Cache(rt, kv_heads, seq, head, filled=ctx)
+    c = Cache(rt, kv_heads, 400, head, filled=start + tokens)
     q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
-    want = kv4.attention(q, *c.numbers(ctx), start)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
     for split in (16, 512):
-        nbytes = int(lib.ammon_attention_prefill_scratch_bytes(tokens, heads, head, ctx, split))
-        part, out = rt.alloc(nbytes), rt.alloc(q.nbytes)
-        call("ammon_attention_prefill", rt.handle, None, up(rt, q), tokens, heads, *c.dev, KV4,
-             kv_heads, head, seq, rt.step(0, start), ctx, split, part, nbytes, out)
-        assert off(out.download(q.shape), want) <= TOL
+        assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+# long enough for the tiles: one and several splits, rows that end inside a tile, a wave and a
+# chunk, every number of groups, heads that are no multiple of 4
+LONG = [(32, 8, 128, 0, 300), (32, 8, 128, 1500, 131), (8, 8, 128, 63, 1000), (16, 2, 128, 2500, 77),
+        (8, 4, 64, 129, 700), (18, 6, 96, 1000, 200), (6, 6, 48, 1, 999), (5, 5, 32, 2000, 250),
+        (12, 6, 100, 500, 333), (9, 3, 127, 700, 301), (12, 12, 30, 400, 500), (24, 3, 80, 64, 640)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,head,start,tokens", LONG)
+def test_prefill_long(rt, heads, kv_heads, head, start, tokens):
+    c = Cache(rt, kv_heads, 3000, head, filled=start + tokens)
+    q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
+    for split in (1024, 256, 64):
+        assert off(prefill(rt, q, c, start, split), want) <= TOL, split
+
+
+@pytest.mark.parametrize("head", [128, 80])
+def test_prefill_numbers_that_are_not_finite(rt, head):
+    """A later token's NaN does not reach an earlier one; a value's stays in its group."""
+    heads, kv_heads, start, tokens = 8, 4, 700, 400
+    for side in (0, 1):
+        c = Cache(rt, kv_heads, 2000, head, filled=start + tokens)
+        for at, g, d, bad in ((900, 0, 40, np.inf), (start + tokens - 1, 1, head - 1, np.nan), (5, 2, 0, -np.inf)):
+            row = c.numbers(1, at)[side].astype(np.float32)
+            row[g, 0, d] = bad
+            kv4.pack(c.host[side], kv_heads, 2000, head, at, row)
+        c.dev[side].upload(c.host[side])
+        q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+        want = kv4.attention(q, *c.numbers(start + tokens), start)
+        assert np.isnan(want[200:, 0]).any() and not np.isnan(want[:200, :2]).any()
+        assert not np.isnan(want[:, 6:]).any() and np.isnan(want[:, 4:6]).any()
+        for split in (1024, 64):
+            assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+@pytest.mark.parametrize("tokens", [20, 700])
+def test_prefill_positions_out_of_range(rt, tokens):
+    # the last tokens are past ctx: NaN, and the others as they are
+    c = Cache(rt, 4, 1000, 64, filled=1000)
+    q = oracle.normal(tokens * 8 * 64, 9).reshape(tokens, 8, 64)
+    start, ctx = 250, 250 + tokens - 7
+    want = kv4.attention(q[:-7], *c.numbers(ctx), start)
+    for split in (1024, 100):
+        got = prefill(rt, q, c, start, split, ctx=ctx)
+        assert off(got[:-7], want) <= TOL and np.all(np.isnan(got[-7:]))
+    got = prefill(rt, q, c, 5000, 1024, ctx=ctx)
+    assert np.all(np.isnan(got))
+
+
+def test_prefill_in_a_graph(rt):
+    c = Cache(rt, 8, 1500, 128, filled=1500)
+    tokens, heads = 301, 32
+    q = oracle.normal(tokens * heads * 128, 9).reshape(tokens, heads, 128)
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    call("ammon_stream_create", rt.handle, ctypes.byref(stream))
+    nbytes = int(lib.ammon_attention_prefill_scratch_bytes(tokens, heads, 128, 1500, 256))
+    dq, part, out, step = up(rt, q), rt.alloc(nbytes), rt.alloc(q.nbytes), rt.step(0, 0)
+    rt.synchronize()
+    call("ammon_capture_begin", rt.handle, stream)
+    call("ammon_attention_prefill", rt.handle, stream, dq, tokens, heads, *c.dev, KV4, 8, 128, 1500,
+         step, 1500, 256, part, nbytes, out)
+    call("ammon_capture_end", rt.handle, stream, ctypes.byref(graph))
+    for start in (0, 700, 1199, 3):
+        rt.deposit(step, 0, start, stream)
+        call("ammon_graph_launch", rt.handle, graph, stream)
+        got = out.download(q.shape, stream=stream)
+        assert off(got, kv4.attention(q, *c.numbers(start + tokens), start)) <= TOL
+        np.testing.assert_array_equal(got, prefill(rt, q, c, start, 256, ctx=1500))
+    call("ammon_graph_destroy", rt.handle, graph)
+    call("ammon_stream_destroy", rt.handle, stream)
