@@ -111,6 +111,8 @@ SIGNATURES = {
     "ammon_gemv_rmsnorm": (_ST, [_P, _P, _P, _P, _DT, _F, _P, _DT, _U32, _U32, _P]),
     "ammon_qkv_rope_store": (_ST, [_P, _P, _P, _P, _DT, _F, _P, _P, _P, _DT, _U32, _U32, _U32,
                                    _U32, _P, _P, _P, _DT, _U32, _P, _P]),
+    "ammon_qkv_rope": (_ST, [_P, _P, _P, _P, _DT, _F, _P, _P, _P, _DT, _U32, _U32, _U32, _U32, _P,
+                             _P, _P, _U32, _P, _P]),
     "ammon_gate_up_swiglu": (_ST, [_P, _P, _P, _P, _DT, _F, _P, _P, _DT, _U32, _U32, _P]),
     "ammon_argmax_scratch_bytes": (_SZ, [_U32]),
     "ammon_argmax": (_ST, [_P, _P, _P, _U32, _P, _P]),
@@ -125,6 +127,8 @@ SIGNATURES = {
                                               _U32, _P, _P, _P, _DT, _U32, _P, _P, _P, _SZ]),
     "ammon_prefill_qkv_rope_store": (_ST, [_P, _P, _P, _U32, _P, _P, _P, _DT, _U32, _U32, _U32,
                                            _U32, _P, _P, _P, _DT, _U32, _P, _P]),
+    "ammon_prefill_qkv_rope": (_ST, [_P, _P, _P, _U32, _P, _P, _P, _DT, _U32, _U32, _U32, _U32, _P,
+                                     _P, _P, _U32, _P, _P, _P, _SZ]),
     "ammon_prefill_gate_up_swiglu": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _P]),
     "ammon_attention_prefill_scratch_bytes": (_SZ, [_U32, _U32, _U32, _U32, _U32]),
     "ammon_attention_prefill": (_ST, [_P, _P, _P, _U32, _U32, _P, _P, _DT, _U32, _U32, _U32, _P,

@@ -1,5 +1,6 @@
 // core.cpp -- runtime handle, tensors, DecodeStep parcel and Scheme of the
 // C++ host layer.  Uses only the public C ABI (ammon.h).
+#include <algorithm>
 #include <cstring>
 #include <sstream>
 
@@ -13,7 +14,20 @@ void check(ammon_status st, const std::string &context) {
   throw Error(st, context.empty() ? msg : context + ": " + msg);
 }
 
-size_t dtype_size(DType d) { return d == DType::BF16 ? 2 : 4; }
+size_t dtype_size(DType d) {
+  if (d == DType::KV4) throw Error(AMMON_E_VALIDATION, "KV4 elements have no size of their own");
+  return d == DType::BF16 ? 2 : 4;
+}
+
+size_t storage_bytes(const Shape &shape, DType dtype) {
+  if (dtype != DType::KV4) return shape.numel() * dtype_size(dtype);
+  const size_t r = shape.rank();
+  if (r < 3) throw Error(AMMON_E_VALIDATION, "a KV4 tensor is [.., kv_heads, seq, head], not " + shape.str());
+  size_t bytes =
+      ammon_kv_cache_bytes(AMMON_KV4, shape.dims[r - 3], shape.dims[r - 2], shape.dims[r - 1]);
+  for (size_t i = 0; i + 3 < r; ++i) bytes *= shape.dims[i];
+  return bytes;
+}
 
 // ---- runtime -------------------------------------------------------------------
 Runtime Runtime::create(int device) {
@@ -70,16 +84,21 @@ TensorView TensorView::narrow(size_t axis, uint32_t start, uint32_t len) const {
        << shape_.str();
     throw Error(AMMON_E_VALIDATION, os.str());
   }
-  uint64_t inner = 1;
-  for (size_t i = axis + 1; i < shape_.rank(); ++i) inner *= shape_.dims[i];
+  if (dtype_ == DType::KV4 && axis + 3 >= shape_.rank())
+    throw Error(AMMON_E_VALIDATION, "narrow: a KV4 cache " + shape_.str() + " is not divisible");
+  const Shape inner = Shape{{shape_.dims.begin() + axis + 1, shape_.dims.end()}};
   Shape s = shape_;
   s.dims[axis] = len;
-  return TensorView((char *)ptr_ + (size_t)start * inner * dtype_size(dtype_), s, dtype_);
+  return TensorView((char *)ptr_ + (size_t)start * storage_bytes(inner, dtype_), s, dtype_);
 }
 
 TensorView TensorView::reshape(std::vector<uint32_t> dims) const {
   Shape s = Shape::from_dims(std::move(dims));
-  if (s.numel() != numel()) {
+  const size_t r = shape_.rank(), t = s.rank();
+  const bool same_caches =
+      dtype_ != DType::KV4 ||
+      (r >= 3 && t >= 3 && std::equal(shape_.dims.end() - 3, shape_.dims.end(), s.dims.end() - 3));
+  if (s.numel() != numel() || !same_caches) {
     throw Error(AMMON_E_VALIDATION, "cannot reshape " + shape_.str() + " to " + s.str());
   }
   return TensorView(ptr_, s, dtype_);

@@ -40,6 +40,11 @@ void expect_float(const std::string &k, const TensorView &v, const char *param) 
     fail(k + ": parameter `" + std::string(param) + "` must be f32 or bf16");
 }
 
+// A KV cache's storage.
+void expect_cache(const std::string &k, const TensorView &v, const char *param) {
+  if (v.dtype() != DType::KV4) expect_float(k, v, param);
+}
+
 void expect_f32(const std::string &k, const TensorView &v, const char *param) {
   if (v.dtype() != DType::F32) fail(k + ": parameter `" + std::string(param) + "` must be f32");
 }
@@ -137,7 +142,7 @@ static void check_rope(const std::string &k, const TensorView &q, const TensorVi
   expect_dim(k, table, "table", 1, "head / 2", head / 2);
   expect_f32(k, q, "q");
   expect_f32(k, table, "table");
-  expect_float(k, cache, "k");
+  expect_cache(k, cache, "k");
 }
 
 void rope(Scheme &s, const std::string &label, TensorView q, TensorView kc, const Tensor &step,
@@ -181,7 +186,7 @@ void cache_store(Scheme &s, const std::string &label, TensorView src, TensorView
   expect_rank(k, dst, "dst", 3);
   expect_dim(k, src, "src", 0, "kv_dim", dst.shape().dim(0) * dst.shape().dim(2));
   expect_f32(k, src, "src");
-  expect_float(k, dst, "dst");
+  expect_cache(k, dst, "dst");
   expect_step(k, step);
   ammon_runtime *rt = s.runtime().raw();
   const auto *st = step_ptr(step);

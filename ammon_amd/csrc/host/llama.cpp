@@ -79,7 +79,7 @@ class LlamaModel : public AutoregressiveModel {
   std::vector<float> host_logits_;
   // prompt prefill scratch, [capacity, width] rows
   uint32_t pf_cap_ = 0;
-  Tensor pf_ids_, pf_x_, pf_xn_, pf_q_, pf_att_, pf_hb_, pf_partial_, pf_ws_;
+  Tensor pf_ids_, pf_x_, pf_xn_, pf_q_, pf_k_, pf_v_, pf_att_, pf_hb_, pf_partial_, pf_ws_;
 };
 
 DType dt(ammon_dtype d) { return (DType)d; }
@@ -297,6 +297,10 @@ void LlamaModel::ensure_prefill(uint32_t n) {
   pf_x_ = Tensor::zeros(rt_, Shape::from_dims({cap, c_.dim}), DType::F32);
   pf_xn_ = Tensor::zeros(rt_, Shape::from_dims({cap, c_.dim}), DType::F32);
   pf_q_ = Tensor::zeros(rt_, Shape::from_dims({cap, q_dim_}), DType::F32);
+  if (c_.kv_dtype == AMMON_KV4) {  // rows for the cache
+    pf_k_ = Tensor::zeros(rt_, Shape::from_dims({cap, kv_dim_}), DType::F32);
+    pf_v_ = Tensor::zeros(rt_, Shape::from_dims({cap, kv_dim_}), DType::F32);
+  }
   pf_att_ = Tensor::zeros(rt_, Shape::from_dims({cap, q_dim_}), DType::F32);
   pf_hb_ = Tensor::zeros(rt_, Shape::from_dims({cap, c_.hidden}), DType::F32);
   // split-reduction partial sums of the QKV, wo and w2 GEMMs
@@ -308,7 +312,8 @@ void LlamaModel::ensure_prefill(uint32_t n) {
 }
 
 // Positions start..start+n-1 through every layer at once: embed rows, then
-// per layer rmsnorm rows, QKV GEMM (RoPE + cache stores at start + t),
+// per layer rmsnorm rows, QKV GEMM (RoPE + cache stores at start + t; KV4: rows,
+// then their stores),
 // token-batched attention, wo GEMM + residual, rmsnorm rows, gate/up GEMM +
 // SwiGLU, w2 GEMM + residual; the final norm and LM head for the last row.
 void LlamaModel::prefill(const int32_t *tokens, uint32_t n, uint32_t start, float *logits) {
@@ -351,11 +356,23 @@ void LlamaModel::prefill(const int32_t *tokens, uint32_t n, uint32_t start, floa
     KvLayer kv = cache_.layer(l);
     check(ammon_rmsnorm(rt, st, x, aw.norm.data(), AMMON_F32, xn, n, c_.dim, c_.eps),
           "prefill rmsnorm");
-    check(ammon_prefill_qkv_rope_store_ws(rt, st, xn, n, aw.query.data(), aw.key.data(),
-                                          aw.value.data(), wd, c_.dim, c_.n_heads, c_.n_kv_heads,
-                                          head_, q, kv.key.data(), kv.value.data(), kvd,
-                                          c_.max_seq, step, table, pf_ws_.data(), pf_ws_.nbytes()),
-          "prefill qkv");
+    if (kvd == AMMON_KV4) {
+      float *kn = (float *)pf_k_.data(), *vn = (float *)pf_v_.data();
+      check(ammon_prefill_qkv_rope(rt, st, xn, n, aw.query.data(), aw.key.data(), aw.value.data(),
+                                   wd, c_.dim, c_.n_heads, c_.n_kv_heads, head_, q, kn, vn,
+                                   c_.max_seq, step, table, pf_ws_.data(), pf_ws_.nbytes()),
+            "prefill qkv");
+      check(ammon_kv4_store(rt, st, kn, vn, n, c_.n_kv_heads, head_, kv.key.data(),
+                            kv.value.data(), c_.max_seq, step),
+            "prefill store");
+    } else {
+      check(ammon_prefill_qkv_rope_store_ws(rt, st, xn, n, aw.query.data(), aw.key.data(),
+                                            aw.value.data(), wd, c_.dim, c_.n_heads,
+                                            c_.n_kv_heads, head_, q, kv.key.data(),
+                                            kv.value.data(), kvd, c_.max_seq, step, table,
+                                            pf_ws_.data(), pf_ws_.nbytes()),
+            "prefill qkv");
+    }
     check(ammon_attention_prefill(rt, st, q, n, c_.n_heads, kv.key.data(), kv.value.data(), kvd,
                                   c_.n_kv_heads, head_, c_.max_seq, step, ctx, split,
                                   (float *)pf_partial_.data(), part_bytes, att),

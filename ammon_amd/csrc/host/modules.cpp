@@ -9,6 +9,7 @@
 // Blocks::record_attention / record_ffn (src/blocks.rs:172-278):
 //   attention: [rmsnorm + wq|wk|wv + rope_store + cache_store] -> attn_partial
 //              -> attn_combine -> [wo + residual]            (10 -> 4 launches)
+//              (KV4 cache: [rmsnorm + wq|wk|wv + rope] -> [stores + attn_partial] -> ..)
 //   SwiGLU:    [rmsnorm + w1|w3 + swiglu] -> [w2 + residual]  (6 -> 2 launches)
 #include <sstream>
 
@@ -34,7 +35,11 @@ KvCache::KvCache(const Runtime &rt, uint32_t layers, uint32_t seq_len, uint32_t 
                  uint32_t head_size, DType dtype)
     : rt_(rt), layers_(layers), seq_(seq_len), kv_heads_(kv_heads), head_(head_size),
       dtype_(dtype) {
-  need(dtype == DType::F32 || dtype == DType::BF16, "KvCache: dtype must be f32 or bf16");
+  need(dtype == DType::F32 || dtype == DType::BF16 || dtype == DType::KV4,
+       "KvCache: dtype must be f32, bf16 or kv4");
+  need(dtype != DType::KV4 || head_size <= AMMON_ATTENTION_MAX_HEAD,
+       "KvCache: head size " + std::to_string(head_size) + " exceeds " +
+           std::to_string(AMMON_ATTENTION_MAX_HEAD));
   const Shape shape = Shape::from_dims({layers, kv_heads, seq_len, head_size});
   key_ = Tensor::zeros(rt, shape, dtype);
   value_ = Tensor::zeros(rt, shape, dtype);
@@ -52,6 +57,19 @@ std::vector<uint8_t> KvCache::layer_to_host_reference_order(uint32_t layer, bool
   need(layer < layers_, "KvCache: layer " + std::to_string(layer) + " of " +
                             std::to_string(layers_));
   const Tensor &src = value ? value_ : key_;
+  if (dtype_ == DType::KV4) {
+    const KvLayer l = KvCache::layer(layer);
+    Tensor numbers = Tensor::zeros(rt_, Shape::from_dims({kv_heads_, seq_, head_}), DType::F32);
+    check(ammon_kv4_load(rt_.raw(), nullptr, (value ? l.value : l.key).data(), nullptr, kv_heads_,
+                         head_, seq_, 0, seq_, numbers.data(), nullptr, AMMON_F32),
+          "KvCache load");
+    const std::vector<float> head_major = numbers.to_f32();
+    std::vector<uint8_t> pos_major(head_major.size() * sizeof(float));
+    check(ammon_kv_unpermute(head_major.data(), pos_major.data(), kv_heads_, seq_, head_,
+                             sizeof(float)),
+          "KvCache unpermute");
+    return pos_major;
+  }
   const size_t layer_bytes = (size_t)kv_heads_ * seq_ * head_ * dtype_size(dtype_);
   std::vector<uint8_t> head_major(layer_bytes), pos_major(layer_bytes);
   check(ammon_memcpy(rt_.raw(), head_major.data(), (const char *)src.data() + layer * layer_bytes,
@@ -131,6 +149,8 @@ CausalAttentionBlock::CausalAttentionBlock(const Runtime &rt, uint32_t hidden, u
   need(head_ % 2 == 0, "attention: head size " + std::to_string(head_) + " must be even for RoPE");
   xb_ = Tensor::zeros(rt, Shape::from_dims({query_heads, head_}), DType::F32);
   q_ = Tensor::zeros(rt, Shape::from_dims({query_heads, head_}), DType::F32);
+  k_ = Tensor::zeros(rt, Shape::from_dims({query_heads, head_}), DType::F32);
+  v_ = Tensor::zeros(rt, Shape::from_dims({query_heads, head_}), DType::F32);
   // Scratch for the most splits any shape will use: the split length grows
   // with kv_heads and with fewer units per CU, so kv_heads = 1 at two units
   // per CU bounds the count.
@@ -188,27 +208,45 @@ void CausalAttentionBlock::record(Scheme &s, TensorView x, const CausalAttention
   const auto *st = (const ammon_decode_step *)step.data();
   const uint32_t hidden = hidden_, q_heads = q_heads_, head = head_, seq = seq_;
   const float eps = opts_.eps;
-  float *q = (float *)q_.data();
+  float *q = (float *)q_.data(), *kn = (float *)k_.data(), *vn = (float *)v_.data();
   float *xb = (float *)xb_.data();
   float *partial = (float *)partial_.data();
   const size_t partial_bytes = partial_.nbytes();
   const float *table = (const float *)table_->data();
-  s.record("qkv_rope_store", [=](ammon_stream stream) {
-    return ammon_qkv_rope_store(rt, stream, (const float *)x.data(), w.norm.data(),
-                                abi(w.norm.dtype()), eps, w.query.data(), w.key.data(),
-                                w.value.data(), abi(w.query.dtype()), hidden, q_heads, kv_heads,
-                                head, q, cache.key.data(), cache.value.data(),
-                                abi(cache.key.dtype()), seq, st, table);
-  });
+  // a KV4 row is quantised whole: the attention pass stores it
+  const bool append = cache.key.dtype() == DType::KV4;
+  if (append)
+    s.record("qkv_rope", [=](ammon_stream stream) {
+      return ammon_qkv_rope(rt, stream, (const float *)x.data(), w.norm.data(), abi(w.norm.dtype()),
+                            eps, w.query.data(), w.key.data(), w.value.data(),
+                            abi(w.query.dtype()), hidden, q_heads, kv_heads, head, q, kn, vn, seq,
+                            st, table);
+    });
+  else
+    s.record("qkv_rope_store", [=](ammon_stream stream) {
+      return ammon_qkv_rope_store(rt, stream, (const float *)x.data(), w.norm.data(),
+                                  abi(w.norm.dtype()), eps, w.query.data(), w.key.data(),
+                                  w.value.data(), abi(w.query.dtype()), hidden, q_heads, kv_heads,
+                                  head, q, cache.key.data(), cache.value.data(),
+                                  abi(cache.key.dtype()), seq, st, table);
+    });
   if (ammon_attention_splits(seq, split) == 1) {
     // one split covers the cache: pass 1 writes the output, no merge launch
     s.record("attention", [=](ammon_stream stream) {
+      if (append)
+        return ammon_attention_decode_append(rt, stream, q, q_heads, kn, vn, cache.key.data(),
+                                             cache.value.data(), AMMON_KV4, kv_heads, head, seq, st,
+                                             split, partial, partial_bytes, xb);
       return ammon_attention_decode(rt, stream, q, q_heads, cache.key.data(), cache.value.data(),
                                     abi(cache.key.dtype()), kv_heads, head, seq, st, split,
                                     partial, partial_bytes, xb);
     });
   } else {
     s.record("attn_partial", [=](ammon_stream stream) {
+      if (append)
+        return ammon_attention_partial_append(rt, stream, q, q_heads, kn, vn, cache.key.data(),
+                                              cache.value.data(), AMMON_KV4, kv_heads, head, seq,
+                                              st, split, partial);
       return ammon_attention_partial(rt, stream, q, q_heads, cache.key.data(), cache.value.data(),
                                      abi(cache.key.dtype()), kv_heads, head, seq, st, split,
                                      partial);

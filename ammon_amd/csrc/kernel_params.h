@@ -142,6 +142,7 @@ typedef struct {
   uint32_t norm_dtype;
   float eps;
   uint32_t kv_dim, head, seq, kv_dtype; /* QKV */
+  uint32_t kv_rows;         /* QKV: k_cache / v_cache are fp32 rows [kv_dim] */
   float *cand_v;            /* PLAIN_ARGMAX: [gridDim.x] (value, index) of the */
   uint32_t *cand_i;         /* first maximum over the workgroup's rows */
 } ammon_k_gemv;
@@ -160,6 +161,7 @@ typedef struct {
   const float *table;       /* QKV: rope cos/sin [seq, head/2, 2] */
   uint32_t d, n, rows, tokens;
   uint32_t kv_dim, head, seq, kv_dtype; /* QKV */
+  uint32_t kv_rows;         /* QKV: k_cache / v_cache are fp32 rows [tokens, kv_dim] */
   /* PLAIN / RESIDUAL, register-blocked tiles: the reduction split into
    * ksplit ranges of kchunks 64-wide chunks; range s writes its partial
    * sums to ws[s][tokens][d], summed in order by ammon_gemm_reduce */

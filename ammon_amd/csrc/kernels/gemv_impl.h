@@ -28,7 +28,7 @@
 //   QKV       rows run over [Wq; Wk; Wv]; (2i, 2i+1) pairs of q and k rows are
 //             rotated with the cos/sin table at step->position; q goes to y,
 //             rotated k and raw v go to the head-major caches at that position
-//             (src/kernels.rs:174-226).
+//             (src/kernels.rs:174-226), or with kv_rows to fp32 rows [kv_dim].
 //
 // The pass runs in two steps: begin() requests the first two tiles (weights
 // only, which depend on nothing an earlier kernel wrote), run() stages x,
@@ -431,6 +431,11 @@ struct GemvPass {
             if (vr < p.d) {
               st_out(p.y + vr, __uint_as_float(0x7fc00000u));
               st_out(p.y + vr + 1, __uint_as_float(0x7fc00000u));
+            } else if (p.kv_rows) {
+              const uint32_t rr = vr - p.d;
+              float *to = (float *)(rr < p.kv_dim ? p.k_cache : p.v_cache);
+              st_out(to + rr % p.kv_dim, __uint_as_float(0x7fc00000u));
+              st_out(to + rr % p.kv_dim + 1, __uint_as_float(0x7fc00000u));
             }
             continue;
           }
@@ -444,12 +449,14 @@ struct GemvPass {
               st_out(p.y + vr, o0);
               st_out(p.y + vr + 1, o1);
             } else {
-              const size_t dst = ((size_t)(rr / p.head) * p.seq + pos) * p.head + hd;
+              const size_t dst =
+                  p.kv_rows ? rr : ((size_t)(rr / p.head) * p.seq + pos) * p.head + hd;
               store_pair_out(p.k_cache, p.kv_dtype, dst, o0, o1);
             }
           } else {
             const uint32_t rv = vr - p.d - p.kv_dim;
-            const size_t dst = ((size_t)(rv / p.head) * p.seq + pos) * p.head + rv % p.head;
+            const size_t dst =
+                p.kv_rows ? rv : ((size_t)(rv / p.head) * p.seq + pos) * p.head + rv % p.head;
             store_pair_out(p.v_cache, p.kv_dtype, dst, a0, a1);
           }
         }

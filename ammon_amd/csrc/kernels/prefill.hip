@@ -63,8 +63,9 @@ template <> struct GemmTraits<float> {
 
 // QKV epilogue of virtual rows (v, v + 1) of token t: rotate q and k pairs
 // with the cos/sin table at position step->position + t; q to y, k and raw
-// v rows to the head-major caches (src/kernels.rs:174-226); a position past
-// the cache poisons q and touches no cache.  fcr, fci: the pair's cos and sin
+// v rows to the head-major caches (src/kernels.rs:174-226), or with kv_rows to
+// fp32 rows [tokens, kv_dim]; a position past the cache poisons q (and such
+// rows) and touches no cache.  fcr, fci: the pair's cos and sin
 // (unused for v rows and positions past the cache).
 AMMON_DEV void qkv_store_pair(const ammon_k_gemm &p, uint32_t t, uint32_t v, float a0, float a1,
                               float fcr, float fci) {
@@ -75,6 +76,10 @@ AMMON_DEV void qkv_store_pair(const ammon_k_gemm &p, uint32_t t, uint32_t v, flo
     if (v < p.d) {
       p.y[(size_t)t * p.d + v] = __uint_as_float(0x7fc00000u);
       p.y[(size_t)t * p.d + v + 1] = __uint_as_float(0x7fc00000u);
+    } else if (p.kv_rows) {
+      const uint32_t rr = v - p.d;
+      const float nan = __uint_as_float(0x7fc00000u);
+      store_pair_out(rr < kvd ? p.k_cache : p.v_cache, AMMON_K_F32, (size_t)t * kvd + rr % kvd, nan, nan);
     }
     return;
   }
@@ -87,12 +92,16 @@ AMMON_DEV void qkv_store_pair(const ammon_k_gemm &p, uint32_t t, uint32_t v, flo
       p.y[(size_t)t * p.d + v + 1] = o1;
     } else {
       store_pair_out(p.k_cache, p.kv_dtype,
-                     ((size_t)(rr / p.head) * p.seq + pos) * p.head + rr % p.head, o0, o1);
+                     p.kv_rows ? (size_t)t * kvd + rr
+                               : ((size_t)(rr / p.head) * p.seq + pos) * p.head + rr % p.head,
+                     o0, o1);
     }
   } else {
     const uint32_t rv = v - p.d - kvd;
     store_pair_out(p.v_cache, p.kv_dtype,
-                   ((size_t)(rv / p.head) * p.seq + pos) * p.head + rv % p.head, a0, a1);
+                   p.kv_rows ? (size_t)t * kvd + rv
+                             : ((size_t)(rv / p.head) * p.seq + pos) * p.head + rv % p.head,
+                   a0, a1);
   }
 }
 

@@ -88,6 +88,7 @@ struct GemvArgs {
   const float *table;
   uint32_t kv_dim, head, seq;
   ammon_dtype kv_dtype;
+  bool kv_rows;        // QKV: k and v as fp32 rows, not cache rows
   float *cand_v;       // PLAIN_ARGMAX: candidate arrays of cand_cap entries
   uint32_t *cand_i;
   uint32_t cand_cap;
@@ -153,6 +154,7 @@ ammon_status gemv_pack(ammon_runtime *rt, const GemvArgs &a, const char *what, a
   p.head = a.head;
   p.seq = a.seq;
   p.kv_dtype = (uint32_t)a.kv_dtype;
+  p.kv_rows = a.kv_rows;
   p.cand_v = a.cand_v;
   p.cand_i = a.cand_i;
   *lds_out = shmem;
@@ -963,6 +965,7 @@ struct GemmArgs {
   const float *table;
   uint32_t kv_dim, head, seq;
   ammon_dtype kv_dtype;
+  bool kv_rows;  // QKV: k and v as fp32 rows, not cache rows
   void *ws;  // PLAIN / RESIDUAL: optional workspace for a split reduction
   size_t ws_bytes;
 };
@@ -1009,6 +1012,7 @@ ammon_status gemm_check_and_launch(ammon_runtime *rt, ammon_stream stream, const
   p.head = a.head;
   p.seq = a.seq;
   p.kv_dtype = (uint32_t)a.kv_dtype;
+  p.kv_rows = a.kv_rows;
   // bf16 W: register-blocked tiles of 64 or 32 tokens (16 for up to 16) x 4
   // waves x 4 or 2 (2) 16-row tiles per wave, the reduction optionally split
   // into 2..8 ranges of at least 8 chunks (plain / residual / QKV with a
@@ -1170,17 +1174,22 @@ ammon_status ammon_prefill_qkv_rope_store(ammon_runtime *rt, ammon_stream stream
                                          table, nullptr, 0);
 }
 
-ammon_status ammon_prefill_qkv_rope_store_ws(ammon_runtime *rt, ammon_stream stream, const float *x,
-                                          uint32_t tokens, const void *wq, const void *wk,
-                                          const void *wv, ammon_dtype w_dtype, uint32_t dim,
-                                          uint32_t q_heads, uint32_t kv_heads, uint32_t head,
-                                          float *q, void *k_cache, void *v_cache,
-                                          ammon_dtype kv_dtype, uint32_t seq,
-                                          const ammon_decode_step *step, const float *table,
-                                             void *workspace, size_t workspace_bytes) {
-  REQUIRE_RT();
+}  // extern "C"
+
+namespace {
+// The QKV GEMM into caches [kv_heads, seq, head], or (rows) into fp32 rows [tokens,
+// kv_heads * head].
+ammon_status prefill_qkv(ammon_runtime *rt, ammon_stream stream, const float *x, uint32_t tokens,
+                         const void *wq, const void *wk, const void *wv, ammon_dtype w_dtype,
+                         uint32_t dim, uint32_t q_heads, uint32_t kv_heads, uint32_t head, float *q,
+                         void *k, void *v, ammon_dtype kv_dtype, bool rows, uint32_t seq,
+                         const ammon_decode_step *step, const float *table, void *workspace,
+                         size_t workspace_bytes, const char *what) {
   AMMON_CHECK(wq && wk && wv, "prefill_qkv: NULL wq, wk or wv");
-  AMMON_CHECK(k_cache && v_cache && step && table, "prefill_qkv: NULL cache, step or table");
+  AMMON_CHECK(k && v && step && table, "prefill_qkv: NULL %s, step or table",
+              rows ? "row buffer" : "cache");
+  AMMON_CHECK(kv_dtype != AMMON_KV4,
+              "prefill_qkv: a KV4 cache takes rows (prefill_qkv_rope, then kv4_store)");
   AMMON_CHECK(valid_dtype(kv_dtype), "prefill_qkv: unknown kv dtype %d", (int)kv_dtype);
   AMMON_CHECK(head >= 16 && head % 16 == 0, "prefill_qkv: head size %u must be a multiple of 16",
               head);
@@ -1188,9 +1197,9 @@ ammon_status ammon_prefill_qkv_rope_store_ws(ammon_runtime *rt, ammon_stream str
   const uint64_t q_dim = (uint64_t)q_heads * head, kv_dim = (uint64_t)kv_heads * head;
   AMMON_CHECK(kv_dim <= q_dim, "attention: kv width must be even and no wider than q");
   AMMON_CHECK(q_dim + 2 * kv_dim < (1ull << 31), "prefill_qkv: too many rows");
-  AMMON_CHECK(!overlaps(k_cache, (size_t)kv_dim * seq * dsize(kv_dtype), v_cache,
-                        (size_t)kv_dim * seq * dsize(kv_dtype)),
-              "prefill_qkv: key and value caches overlap");
+  const size_t kv_bytes = (size_t)kv_dim * (rows ? tokens : seq) * dsize(kv_dtype);
+  AMMON_CHECK(!overlaps(k, kv_bytes, v, kv_bytes), "prefill_qkv: key and value %s overlap",
+              rows ? "rows" : "caches");
   GemmArgs a = {};
   a.mode = AMMON_GEMV_QKV;
   a.w0 = wq;
@@ -1204,21 +1213,108 @@ ammon_status ammon_prefill_qkv_rope_store_ws(ammon_runtime *rt, ammon_stream str
   a.x = x;
   a.y = q;
   a.y_bytes = (size_t)tokens * q_dim * 4;
-  a.k_cache = k_cache;
-  a.v_cache = v_cache;
+  a.k_cache = k;
+  a.v_cache = v;
   a.step = step;
   a.table = table;
   a.kv_dim = (uint32_t)kv_dim;
   a.head = head;
   a.seq = seq;
   a.kv_dtype = kv_dtype;
+  a.kv_rows = rows;
   a.ws = workspace;
   a.ws_bytes = workspace ? workspace_bytes : 0;
-  const size_t cache_bytes = (size_t)kv_dim * seq * dsize(kv_dtype);
-  AMMON_CHECK(!workspace || (!overlaps(workspace, workspace_bytes, k_cache, cache_bytes) &&
-                             !overlaps(workspace, workspace_bytes, v_cache, cache_bytes)),
-              "prefill_qkv: workspace overlaps a cache");
-  return gemm_check_and_launch(rt, stream, a, "prefill_qkv_rope_store");
+  AMMON_CHECK(!workspace || (!overlaps(workspace, workspace_bytes, k, kv_bytes) &&
+                             !overlaps(workspace, workspace_bytes, v, kv_bytes)),
+              "prefill_qkv: workspace overlaps %s", rows ? "the rows" : "a cache");
+  if (rows) {
+    const size_t xbytes = (size_t)tokens * dim * 4;
+    for (const void *to : {k, v})
+      AMMON_CHECK(!overlaps(to, kv_bytes, x, xbytes) && !overlaps(to, kv_bytes, q, a.y_bytes),
+                  "prefill_qkv: the rows overlap x or q");
+    AMMON_CHECK((((uintptr_t)k | (uintptr_t)v) & 7u) == 0, "prefill_qkv: rows must be 8-byte aligned");
+  }
+  return gemm_check_and_launch(rt, stream, a, what);
+}
+
+// The QKV GEMV into caches, or (rows) into fp32 rows [kv_heads * head].
+ammon_status qkv(ammon_runtime *rt, ammon_stream stream, const float *x, const void *norm_weight,
+                 ammon_dtype norm_dtype, float eps, const void *wq, const void *wk, const void *wv,
+                 ammon_dtype w_dtype, uint32_t dim, uint32_t q_heads, uint32_t kv_heads,
+                 uint32_t head, float *q, void *k, void *v, ammon_dtype kv_dtype, bool rows,
+                 uint32_t seq, const ammon_decode_step *step, const float *table, const char *what) {
+  AMMON_CHECK(wq && wk && wv, "qkv: NULL wq, wk or wv");
+  AMMON_CHECK(k && v && step && table, "qkv: NULL %s, step or table", rows ? "row buffer" : "cache");
+  AMMON_CHECK(kv_dtype != AMMON_KV4,
+              "qkv: a KV4 cache takes rows (qkv_rope, then attention_decode_append or kv4_store)");
+  AMMON_CHECK(valid_dtype(kv_dtype), "qkv: unknown kv dtype %d", (int)kv_dtype);
+  AMMON_CHECK(head >= 2 && head % 2 == 0, "qkv: head size %u must be even", head);
+  AMMON_CHECK(q_heads > 0 && kv_heads > 0 && seq > 0, "qkv: empty shape");
+  const uint64_t q_dim = (uint64_t)q_heads * head, kv_dim = (uint64_t)kv_heads * head;
+  AMMON_CHECK(kv_dim <= q_dim, "attention: kv width must be even and no wider than q");
+  AMMON_CHECK(q_dim + 2 * kv_dim < (1ull << 31), "qkv: too many rows");
+  const size_t kv_bytes = (size_t)kv_dim * (rows ? 1 : seq) * dsize(kv_dtype);
+  AMMON_CHECK(!overlaps(k, kv_bytes, v, kv_bytes), "qkv: key and value %s overlap",
+              rows ? "rows" : "caches");
+  if (rows) {
+    for (const void *to : {k, v})
+      AMMON_CHECK(!overlaps(to, kv_bytes, x, (size_t)dim * 4) && !overlaps(to, kv_bytes, q, q_dim * 4),
+                  "qkv: the rows overlap x or q");
+    AMMON_CHECK((((uintptr_t)k | (uintptr_t)v) & 7u) == 0, "qkv: rows must be 8-byte aligned");
+  }
+  GemvArgs a = {};
+  a.mode = AMMON_GEMV_QKV;
+  a.w0 = wq;
+  a.w1 = wk;
+  a.w2 = wv;
+  a.w_dtype = w_dtype;
+  a.d = (uint32_t)q_dim;
+  a.n = dim;
+  a.rows = (uint32_t)(q_dim + 2 * kv_dim);
+  a.x = x;
+  a.norm_w = norm_weight;
+  a.norm_dtype = norm_dtype;
+  a.eps = eps;
+  a.y = q;
+  a.k_cache = k;
+  a.v_cache = v;
+  a.step = step;
+  a.table = table;
+  a.kv_dim = (uint32_t)kv_dim;
+  a.head = head;
+  a.seq = seq;
+  a.kv_dtype = kv_dtype;
+  a.kv_rows = rows;
+  return gemv_check_and_launch(rt, stream, a, what);
+}
+}  // namespace
+
+extern "C" {
+
+ammon_status ammon_prefill_qkv_rope_store_ws(ammon_runtime *rt, ammon_stream stream, const float *x,
+                                          uint32_t tokens, const void *wq, const void *wk,
+                                          const void *wv, ammon_dtype w_dtype, uint32_t dim,
+                                          uint32_t q_heads, uint32_t kv_heads, uint32_t head,
+                                          float *q, void *k_cache, void *v_cache,
+                                          ammon_dtype kv_dtype, uint32_t seq,
+                                          const ammon_decode_step *step, const float *table,
+                                             void *workspace, size_t workspace_bytes) {
+  REQUIRE_RT();
+  return prefill_qkv(rt, stream, x, tokens, wq, wk, wv, w_dtype, dim, q_heads, kv_heads, head, q,
+                     k_cache, v_cache, kv_dtype, false, seq, step, table, workspace,
+                     workspace_bytes, "prefill_qkv_rope_store");
+}
+
+ammon_status ammon_prefill_qkv_rope(ammon_runtime *rt, ammon_stream stream, const float *x,
+                                    uint32_t tokens, const void *wq, const void *wk, const void *wv,
+                                    ammon_dtype w_dtype, uint32_t dim, uint32_t q_heads,
+                                    uint32_t kv_heads, uint32_t head, float *q, float *k, float *v,
+                                    uint32_t seq, const ammon_decode_step *step, const float *table,
+                                    void *workspace, size_t workspace_bytes) {
+  REQUIRE_RT();
+  return prefill_qkv(rt, stream, x, tokens, wq, wk, wv, w_dtype, dim, q_heads, kv_heads, head, q, k,
+                     v, AMMON_F32, true, seq, step, table, workspace, workspace_bytes,
+                     "prefill_qkv_rope");
 }
 
 ammon_status ammon_prefill_gate_up_swiglu(ammon_runtime *rt, ammon_stream stream, const float *x,
@@ -1331,40 +1427,19 @@ ammon_status ammon_qkv_rope_store(ammon_runtime *rt, ammon_stream stream, const 
                                   void *v_cache, ammon_dtype kv_dtype, uint32_t seq,
                                   const ammon_decode_step *step, const float *table) {
   REQUIRE_RT();
-  AMMON_CHECK(wq && wk && wv, "qkv: NULL wq, wk or wv");
-  AMMON_CHECK(k_cache && v_cache && step && table, "qkv: NULL cache, step or table");
-  AMMON_CHECK(valid_dtype(kv_dtype), "qkv: unknown kv dtype %d", (int)kv_dtype);
-  AMMON_CHECK(head >= 2 && head % 2 == 0, "qkv: head size %u must be even", head);
-  AMMON_CHECK(q_heads > 0 && kv_heads > 0 && seq > 0, "qkv: empty shape");
-  const uint64_t q_dim = (uint64_t)q_heads * head, kv_dim = (uint64_t)kv_heads * head;
-  AMMON_CHECK(kv_dim <= q_dim, "attention: kv width must be even and no wider than q");
-  AMMON_CHECK(q_dim + 2 * kv_dim < (1ull << 31), "qkv: too many rows");
-  AMMON_CHECK(!overlaps(k_cache, (size_t)kv_dim * seq * dsize(kv_dtype), v_cache,
-                        (size_t)kv_dim * seq * dsize(kv_dtype)),
-              "qkv: key and value caches overlap");
-  GemvArgs a = {};
-  a.mode = AMMON_GEMV_QKV;
-  a.w0 = wq;
-  a.w1 = wk;
-  a.w2 = wv;
-  a.w_dtype = w_dtype;
-  a.d = (uint32_t)q_dim;
-  a.n = dim;
-  a.rows = (uint32_t)(q_dim + 2 * kv_dim);
-  a.x = x;
-  a.norm_w = norm_weight;
-  a.norm_dtype = norm_dtype;
-  a.eps = eps;
-  a.y = q;
-  a.k_cache = k_cache;
-  a.v_cache = v_cache;
-  a.step = step;
-  a.table = table;
-  a.kv_dim = (uint32_t)kv_dim;
-  a.head = head;
-  a.seq = seq;
-  a.kv_dtype = kv_dtype;
-  return gemv_check_and_launch(rt, stream, a, "qkv_rope_store");
+  return qkv(rt, stream, x, norm_weight, norm_dtype, eps, wq, wk, wv, w_dtype, dim, q_heads, kv_heads,
+             head, q, k_cache, v_cache, kv_dtype, false, seq, step, table, "qkv_rope_store");
+}
+
+ammon_status ammon_qkv_rope(ammon_runtime *rt, ammon_stream stream, const float *x,
+                            const void *norm_weight, ammon_dtype norm_dtype, float eps,
+                            const void *wq, const void *wk, const void *wv, ammon_dtype w_dtype,
+                            uint32_t dim, uint32_t q_heads, uint32_t kv_heads, uint32_t head,
+                            float *q, float *k, float *v, uint32_t seq,
+                            const ammon_decode_step *step, const float *table) {
+  REQUIRE_RT();
+  return qkv(rt, stream, x, norm_weight, norm_dtype, eps, wq, wk, wv, w_dtype, dim, q_heads, kv_heads,
+             head, q, k, v, AMMON_F32, true, seq, step, table, "qkv_rope");
 }
 
 ammon_status ammon_gate_up_swiglu(ammon_runtime *rt, ammon_stream stream, const float *x,

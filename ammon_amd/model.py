@@ -15,7 +15,7 @@ import ctypes
 import numpy as np
 
 from . import _abi
-from ._abi import BF16, F32, call
+from ._abi import BF16, F32, KV4, call
 from .runtime import Runtime
 
 WEIGHT_NAMES = ("tok_emb", "rms_att", "rms_ffn", "wq", "wk", "wv", "wo", "w1", "w2", "w3",
@@ -250,7 +250,8 @@ class LlamaModel:
         self.rt.synchronize(self.stream)
 
     def kv_layer(self, layer: int):
-        """(key, value) of `layer` in the reference order [seq, kv_heads, head]."""
+        """(key, value) of `layer` in the reference order [seq, kv_heads, head] (a KV4 cache: the
+        fp32 numbers it stands for)."""
         from .runtime import kv_unpermute
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
         call("ammon_llama_kv_layer", self.handle, layer, ctypes.byref(k), ctypes.byref(v))
@@ -259,6 +260,12 @@ class LlamaModel:
         shape = (c.n_kv_heads, c.max_seq, self.head)
         out = []
         self.synchronize()
+        if c.kv_dtype == KV4:
+            bufs = [self.rt.alloc(4 * int(np.prod(shape))) for _ in range(2)]
+            call("ammon_kv4_load", self.rt.handle, None, k, v, c.n_kv_heads, self.head, c.max_seq,
+                 0, c.max_seq, *bufs, F32)
+            return tuple(kv_unpermute(b.download(shape), c.n_kv_heads, c.max_seq, self.head)
+                         for b in bufs)
         for ptr in (k, v):
             a = np.empty(shape, dt)
             call("ammon_memcpy", self.rt.handle, a.ctypes.data, ptr, a.nbytes, _abi.COPY_D2H,

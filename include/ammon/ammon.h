@@ -391,6 +391,16 @@ ammon_status ammon_qkv_rope_store(ammon_runtime *rt, ammon_stream stream, const 
                                   void *v_cache, ammon_dtype kv_dtype, uint32_t seq,
                                   const ammon_decode_step *step, const float *table);
 
+/* ... with the rows as fp32, k, v [kv_heads * head] (8-byte aligned), and no
+ * cache: for caches that take whole rows (AMMON_KV4).  A position >= seq
+ * writes NaN to q, k and v. */
+ammon_status ammon_qkv_rope(ammon_runtime *rt, ammon_stream stream, const float *x,
+                            const void *norm_weight, ammon_dtype norm_dtype, float eps,
+                            const void *wq, const void *wk, const void *wv, ammon_dtype w_dtype,
+                            uint32_t dim, uint32_t q_heads, uint32_t kv_heads, uint32_t head,
+                            float *q, float *k, float *v, uint32_t seq,
+                            const ammon_decode_step *step, const float *table);
+
 /* Fused SwiGLU-block front (reference src/blocks.rs:267-272: rmsnorm, w1,
  * w3, swiglu) in one launch: hb = silu(W1 xn) * (W3 xn). */
 ammon_status ammon_gate_up_swiglu(ammon_runtime *rt, ammon_stream stream, const float *x,
@@ -471,6 +481,15 @@ ammon_status ammon_prefill_qkv_rope_store_ws(ammon_runtime *rt, ammon_stream str
                                           ammon_dtype kv_dtype, uint32_t seq,
                                           const ammon_decode_step *step, const float *table,
                                              void *workspace, size_t workspace_bytes);
+/* ammon_qkv_rope over rows of an already normalised x: q [tokens, q_heads *
+ * head], k, v [tokens, kv_heads * head] (8-byte aligned); workspace may be
+ * NULL. */
+ammon_status ammon_prefill_qkv_rope(ammon_runtime *rt, ammon_stream stream, const float *x,
+                                    uint32_t tokens, const void *wq, const void *wk, const void *wv,
+                                    ammon_dtype w_dtype, uint32_t dim, uint32_t q_heads,
+                                    uint32_t kv_heads, uint32_t head, float *q, float *k, float *v,
+                                    uint32_t seq, const ammon_decode_step *step, const float *table,
+                                    void *workspace, size_t workspace_bytes);
 /* ammon_gate_up_swiglu over rows of an already normalised x: hb [tokens,
  * hidden]. */
 ammon_status ammon_prefill_gate_up_swiglu(ammon_runtime *rt, ammon_stream stream, const float *x,

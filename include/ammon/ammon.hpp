@@ -45,9 +45,10 @@ class Error : public std::runtime_error {
 // Throws ammon::Error with the library's message when `st` is not AMMON_OK.
 void check(ammon_status st, const std::string &context = {});
 
-// Storage dtypes.  F32 / BF16 are the ABI's ammon_dtype values; U32 / I32
+// Storage dtypes.  F32 / BF16 / KV4 are the ABI's ammon_dtype values; U32 / I32
 // are host-layer index types (DecodeStep parcels, token ids).
-enum class DType { F32 = AMMON_F32, BF16 = AMMON_BF16, U32 = 2, I32 = 3 };
+enum class DType { F32 = AMMON_F32, BF16 = AMMON_BF16, U32 = 2, I32 = 3, KV4 = AMMON_KV4 };
+// Bytes of an element; KV4 has none (throws): its rows are 20 bytes per 32 numbers.
 size_t dtype_size(DType d);
 
 // ---- runtime -----------------------------------------------------------------
@@ -82,6 +83,9 @@ struct Shape {
   bool operator==(const Shape &o) const { return dims == o.dims; }
 };
 
+// Bytes of a contiguous tensor.  KV4 tensors are stacked caches [.., kv_heads, seq, head].
+size_t storage_bytes(const Shape &shape, DType dtype);
+
 // Non-owning device view: pointer, shape, storage dtype.
 class TensorView {
  public:
@@ -92,11 +96,12 @@ class TensorView {
   DType dtype() const { return dtype_; }
   uint64_t numel() const { return shape_.numel(); }
   uint32_t numel_u32() const;
-  size_t nbytes() const { return numel() * dtype_size(dtype_); }
+  size_t nbytes() const { return storage_bytes(shape_, dtype_); }
   // Sub-range [start, start + len) along `axis` of a contiguous view
-  // (Goldy TensorView::narrow).
+  // (Goldy TensorView::narrow).  KV4: of whole caches only.
   TensorView narrow(size_t axis, uint32_t start, uint32_t len) const;
   // Same storage, new dims with the same element count (TensorView::reshape).
+  // KV4: the caches' own [kv_heads, seq, head] stay.
   TensorView reshape(std::vector<uint32_t> dims) const;
 
  private:
@@ -123,7 +128,7 @@ class Tensor {
   void *data() const { return ptr_; }
   const Shape &shape() const { return shape_; }
   DType dtype() const { return dtype_; }
-  size_t nbytes() const { return shape_.numel() * dtype_size(dtype_); }
+  size_t nbytes() const { return storage_bytes(shape_, dtype_); }
   // Synchronous copies (the reference's submit + host take).
   std::vector<float> to_f32() const;
   void to_host(void *dst) const;
@@ -276,7 +281,8 @@ class KvCache {  // src/modules.rs:37-71
   uint32_t kv_heads() const { return kv_heads_; }
   uint32_t head_size() const { return head_; }
   DType dtype() const { return dtype_; }
-  // Host copy of one layer in the reference's [seq, kv_heads, head] order.
+  // Host copy of one layer in the reference's [seq, kv_heads, head] order
+  // (KV4: the fp32 numbers it stands for).
   std::vector<uint8_t> layer_to_host_reference_order(uint32_t layer, bool value) const;
 
  private:
@@ -330,7 +336,8 @@ struct AttentionOptions {
 // RoPE, attention, output projection, residual into x.  Recorded as four
 // launches: norm+QKV+RoPE+KV store, split attention, LSE merge, wo +
 // residual (three when one split covers the cache: the attention pass then
-// writes the merged output).
+// writes the merged output).  With a KV4 cache the first gives the rows and the
+// attention pass stores them.
 class CausalAttentionBlock {
  public:
   CausalAttentionBlock(const Runtime &rt, uint32_t hidden, uint32_t query_heads, uint32_t seq_len,
@@ -347,7 +354,7 @@ class CausalAttentionBlock {
   Runtime rt_;
   uint32_t hidden_, q_heads_, head_, seq_;
   AttentionOptions opts_;
-  Tensor xb_, q_, partial_;
+  Tensor xb_, q_, k_, v_, partial_;  // k_, v_: a KV4 cache's new rows
   std::shared_ptr<Tensor> table_;
   uint32_t max_splits_;
 };

@@ -27,7 +27,7 @@ typedef struct ammon_llama_config {
   float theta; /* RoPE base; the reference's default is 10000 */
   float eps;   /* RMSNorm epsilon; the reference's literal is 1e-5 */
   ammon_dtype w_dtype;  /* embedding table and projection matrices */
-  ammon_dtype kv_dtype; /* KV cache storage */
+  ammon_dtype kv_dtype; /* KV cache storage: AMMON_F32, AMMON_BF16 or AMMON_KV4 */
   uint32_t use_graph;   /* replay each token as a captured HIP graph */
   uint32_t split_len;   /* attention split length; 0 picks one sized to the
                            device and the shape's kernel
@@ -109,7 +109,7 @@ ammon_status ammon_llama_decode(ammon_llama *m, uint32_t token, uint32_t start_p
 ammon_status ammon_llama_tokens(ammon_llama *m, uint32_t start, uint32_t n, int32_t *tokens);
 
 /* Device pointers of layer `layer`'s key and value caches ([kv_heads, seq,
- * head] in kv_dtype), the model's stream, and its logits buffer. */
+ * head] in kv_dtype; ammon_kv_cache_bytes each), the model's stream, and its logits buffer. */
 ammon_status ammon_llama_kv_layer(ammon_llama *m, uint32_t layer, void **key, void **value);
 ammon_status ammon_llama_stream(ammon_llama *m, ammon_stream *stream);
 ammon_status ammon_llama_logits(ammon_llama *m, float **device_logits);
