@@ -101,8 +101,8 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_load(ammon_k_kv
       direct_out_nan(p, blockIdx.y);                                                   \
   }
 #define KV4_PARTIAL_NG(NG)                                      \
-  KV4_PARTIAL(ammon_kv4_partial_n##NG, NG, 3, false)            \
-  KV4_PARTIAL(ammon_kv4_partial_append_n##NG, NG, 3, true)
+  KV4_PARTIAL(ammon_kv4_partial_n##NG, NG, 2, false)            \
+  KV4_PARTIAL(ammon_kv4_partial_append_n##NG, NG, 2, true)
 KV4_PARTIAL_NG(1)
 KV4_PARTIAL_NG(2)
 KV4_PARTIAL_NG(3)

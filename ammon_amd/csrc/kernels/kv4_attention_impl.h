@@ -2,14 +2,16 @@
 //
 // Pass 1 of attention_impl.h's pair, any head up to 128 and up to 8 query heads per
 // kv head: one workgroup per (split, kv head), on matrix cores; the partials have
-// the other units' format, so pass 2 is theirs.  Chunks of 128 positions, 32 per
+// the other units' format, so pass 2 is theirs.  Chunks of 256 positions, 64 per
 // wave; NCH chunks are requested ahead into a ring in LDS of which every wave reads
 // back only its own rows, so the chunk loop has no barrier.
 //
 //   scores  S[t][h] = K[t] . q[h] on v_mfma_f32_16x16x32_f16, one per group of 32
-//           numbers: A = K rows as kv4_numbers gives them, B = q as fp16 hi + lo: 22
-//           bits (q is scaled by a power of two to at most 2^13..2^14 first, so that
-//           lo is no subnormal where it matters).
+//           numbers and 16 positions: A = K rows as kv4_numbers gives them, B = q as
+//           fp16, hi in columns 0..7 and lo in 8..15: 22 bits (q is scaled by a power
+//           of two to at most 2^13..2^14 first, so that lo is no subnormal where it
+//           matters).  The halves' sum is a rotation by 8 columns; columns 0..7 then
+//           go on with the first 32 positions' scores, 8..15 with the others'.
 //   weights P = 2^(s log2e / sqrt(head) - m), fp32; m is a running maximum less
 //           KV4_BITS, so that the fp16 parts of small weights are no subnormals
 //           either, and moves only when a chunk exceeds that maximum by KV4_SLACK.
@@ -18,10 +20,16 @@
 //           positions, joined half by half in pairs, and nibble n of the words is
 //           value tile n.  Row 4 a + r of a score tile is position 4 r + a, so that
 //           the four rows of V that a wave reads at a time are neighbours.
+//           Above head 64 a product takes 32 positions, hi in one half of the columns
+//           and lo in the other.  Up to head 64 a row has at most 8 words, and a
+//           product takes 64 positions: lanes 0..7 of A and columns 0..7 are the first
+//           32, the others the second, and the two blocks in which they meet are not
+//           used.
 //
-// What bounds it: HBM where the context is long.  Per 32 positions a wave issues some
-// 270 VALU instructions and 32 MFMA (head 128) for 5 KiB, which take a CU's share of
-// 5.5 TB/s as long as 570 VALU instructions on each SIMD.
+// What bounds it: HBM where the context is long, the two launches where it is short.
+// (Hi and lo in two products of one column half, and 32 positions per wave, took twice
+// the matrix instructions, and up to head 64 twice the vector ones: then these
+// bounded it.)
 #pragma once
 
 #include "attention_impl.h"
@@ -30,26 +38,33 @@
 #define KV4_BITS 10.0f
 #define KV4_SLACK 4.0f
 #define KV4_MAX_GROUP 8  // query heads per kv head
+#define KV4_DPP_ROR8 0x128  // rows of 16 lanes by 8
 
-// What one wave stages of a chunk: 32 positions' codes, K's then V's, in 16-byte
-// pieces, and their scales, K's then V's: whole requests of 64 lanes each.
+// What one wave stages of a chunk: 64 positions' codes of K, their scales, then V's
+// alike: whole requests of 64 lanes each, 16 bytes a lane for codes.
 template <int NG> struct Kv4Stage {
-  static constexpr uint32_t CODES = 512 * NG, SCALES = 128 * NG;  // bytes of K (or V)
-  static constexpr uint32_t WAVE = 2 * (CODES + SCALES);
+  static constexpr uint32_t ROWS = 64;
+  static constexpr uint32_t CODES = 16 * NG * ROWS, SCALES = 4 * NG * ROWS;  // bytes of K (or V)
+  static constexpr uint32_t HALF = CODES + SCALES, WAVE = 2 * HALF;
   static constexpr uint32_t CHUNK = AMMON_WAVES * WAVE;
   static constexpr int SREQ = NG == 4 ? 1 : NG;  // a row's scales: 16 bytes, or NG words
-  static constexpr int VREQ = NG / 2;            // requests of V's codes alone, the last ones
-  static constexpr int REQ = NG + SREQ;
+  static constexpr int VREQ = NG + SREQ;         // V's requests, the last ones
+  static constexpr int REQ = 2 * VREQ;
 };
 
 template <int NG, int NCH, bool APPEND>
 struct Kv4Partial {
   using S = Kv4Stage<NG>;
-  static constexpr uint32_t WROWS = 32, CROWS = AMMON_WAVES * WROWS;
-  static constexpr uint32_t MERGE = AMMON_WAVES * KV4_MAX_GROUP * ATT_STAGED_OROW * 4;
-  static constexpr uint32_t RING = S::CHUNK * NCH > MERGE ? S::CHUNK * NCH : MERGE;
-  static constexpr uint32_t LDS_BYTES = RING + (2 * AMMON_WAVES + 2) * KV4_MAX_GROUP * 4;
-  static_assert(NCH >= 1 && NCH <= 4, "chunk buffers");
+  static constexpr uint32_t WROWS = S::ROWS, CROWS = AMMON_WAVES * WROWS;
+  static constexpr bool PAIRED = NG <= 2;              // 64 positions a value product
+  static constexpr uint32_t OROW = 32 * NG + 4;        // merge row: banks spread
+  static constexpr uint32_t MROWS = 2 * AMMON_WAVES;   // merge rows per query head
+  static constexpr uint32_t MERGE = MROWS * KV4_MAX_GROUP * OROW * 4;
+  static constexpr uint32_t LDS_BYTES = S::CHUNK * NCH;
+  // A wave's maxima and sums wait for the merge in its part of the last ring buffer,
+  // past the merge's rows.
+  static constexpr uint32_t STATS = S::CHUNK * (NCH - 1);
+  static_assert(NCH >= 2 && NCH <= 4 && MERGE <= STATS, "chunk buffers");
 
   uint32_t split, g, G, pos, t0, n, lane, wave;
   const uint32_t *kc, *ks, *vc, *vs;  // codes and scales of the split's first row
@@ -68,36 +83,50 @@ struct Kv4Partial {
       (const __attribute__((address_space(1))) void *)(FROM),                          \
       (__attribute__((address_space(3))) void *)(TO), SIZE, 0, 0)
 
-  // Request i of the codes of rows r0.. (of K and V together: 64 NG pieces).  Rows past
-  // the split take its last row: they are masked, and what they hold is then no less
-  // finite than what the split holds (but for a new row's place, see run).
-  AMMON_DEV void codes(char *to, uint32_t r0, int i) const {
-    const uint32_t at = i * 64 + lane;
-    const bool v = at >= 32 * NG;
-    const uint32_t pc = piece(v ? at - 32 * NG : at), r = pc / NG;
-    const uint32_t *from = (v ? vc : kc) + (min(r0 + r, n - 1) * NG + (pc - r * NG)) * 4;
-    KV4_REQUEST(from, to + i * 1024, 16);
+  // Rows r0.. of one cache.  Rows past the split take its last row: they are masked, and
+  // what they hold is then no less finite than what the split holds (but for a new row's
+  // place, see run).  A wave's rows are one piece of memory, so whole ones need no
+  // lane's own row.
+  AMMON_DEV void stage_half(char *to, const uint32_t *codes, const uint32_t *scales,
+                            uint32_t r0) const {
+    constexpr uint32_t per = NG == 4 ? 1 : NG;  // scale requests' units per row
+    if (r0 + WROWS <= n) {
+      const char *c = (const char *)(codes + (size_t)r0 * (4 * NG));
+      const char *s = (const char *)(scales + (size_t)r0 * NG);
+      const uint32_t at = piece(lane) * 16;  // (the exchange is the same in every request)
+#pragma unroll
+      for (int i = 0; i < NG; ++i) KV4_REQUEST(c + i * 1024 + (size_t)at, to + i * 1024, 16);
+#pragma unroll
+      for (int i = 0; i < S::SREQ; ++i) {
+        if constexpr (NG == 4)
+          KV4_REQUEST(s + (size_t)(lane * 16), to + S::CODES, 16);
+        else
+          KV4_REQUEST(s + i * 256 + (size_t)(lane * 4), to + S::CODES + i * 256, 4);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint32_t pc = piece(i * 64 + lane), r = pc / NG;
+        const uint32_t *from = codes + (min(r0 + r, n - 1) * NG + (pc - r * NG)) * 4;
+        KV4_REQUEST(from, to + i * 1024, 16);
+      }
+#pragma unroll
+      for (int i = 0; i < S::SREQ; ++i) {
+        const uint32_t u = i * 64 + lane, r = u / per;
+        const uint32_t *from = scales + min(r0 + r, n - 1) * NG + (u - r * per);
+        if constexpr (NG == 4)
+          KV4_REQUEST(from, to + S::CODES, 16);
+        else
+          KV4_REQUEST(from, to + S::CODES + i * 256, 4);
+      }
+    }
   }
   // Chunk c of the split into ring buffer b.
   AMMON_DEV void stage(char *lds, uint32_t c, uint32_t b) const {
     char *to = lds + b * S::CHUNK + wave * S::WAVE;
     const uint32_t r0 = c * CROWS + wave * WROWS;
-#pragma unroll
-    for (int i = 0; i < NG - S::VREQ; ++i) codes(to, r0, i);
-#pragma unroll
-    for (int i = 0; i < S::SREQ; ++i) {
-      constexpr uint32_t per = NG == 4 ? 1 : NG;  // requests' units per row
-      const uint32_t at = i * 64 + lane;
-      const bool v = at >= 32 * per;
-      const uint32_t u = v ? at - 32 * per : at, r = u / per;
-      const uint32_t *from = (v ? vs : ks) + min(r0 + r, n - 1) * NG + (u - r * per);
-      if constexpr (NG == 4)
-        KV4_REQUEST(from, to + 2 * S::CODES, 16);
-      else
-        KV4_REQUEST(from, to + 2 * S::CODES + i * 256, 4);
-    }
-#pragma unroll
-    for (int i = NG - S::VREQ; i < NG; ++i) codes(to, r0, i);
+    stage_half(to, kc, ks, r0);
+    stage_half(to + S::HALF, vc, vs, r0);
   }
 
   // False for a dead split or a position out of range, which write nothing.
@@ -109,7 +138,7 @@ struct Kv4Partial {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // q beside the position: neither needs the other.  (Columns past the group take
     // head 0's; they are never used.)
-    const uint32_t h = lane & 15;
+    const uint32_t h = lane & 7;
     const float *q = p.q + (size_t)(g * G + (h < G ? h : 0)) * p.head;
 #pragma unroll
     for (int j = 0; j < NG; ++j) kv4_row(q, 4 * j + (lane >> 4), p.head, qraw[j]);
@@ -151,16 +180,25 @@ struct Kv4Partial {
     else wait_vmcnt<EXTRA>();
   }
 
+  AMMON_DEV static float other_half(float v) { return dpp_get<KV4_DPP_ROR8>(v); }
+  // fp16 numbers of v, but in the columns of BANKS (0x3: 0..7, 0xc: 8..15) the other
+  // half's of w.
+  template <int BANKS> AMMON_DEV static f16x8 halves(const f16x8 &v, const f16x8 &w) {
+    const u32x4 a = __builtin_bit_cast(u32x4, v), b = __builtin_bit_cast(u32x4, w);
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      r[e] = __builtin_amdgcn_update_dpp(a[e], b[e], KV4_DPP_ROR8, 0xf, BANKS, false);
+    return __builtin_bit_cast(f16x8, r);
+  }
+
   AMMON_DEV void run(const ammon_k_attention &p, char *lds) {
-    float *s_m = (float *)(lds + RING);                  // [4][8] wave maxima
-    float *s_l = s_m + AMMON_WAVES * KV4_MAX_GROUP;      // [4][8] wave sums
-    float *s_M = s_l + AMMON_WAVES * KV4_MAX_GROUP;      // [8] workgroup maxima
-    float *s_L = s_M + KV4_MAX_GROUP;                    // [8] workgroup sums
     const uint32_t h = lane & 15, grp = lane >> 4, head = p.head;
+    const bool second = h >= 8;  // this lane's columns: the second half
 
     const Kv4Bits bits;
     const float minus1 = kv4_minus1();
-    // q^T as the B operand, fp16 hi + lo of q 2^(14 - e), |q| < 2^e
+    // q^T as the B operand, fp16 hi or lo of q 2^(14 - e), |q| < 2^e
     float qmax = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
@@ -168,15 +206,15 @@ struct Kv4Partial {
       for (int e = 0; e < 8; ++e) qmax = fmaxf(qmax, fabsf(qraw[j][e]));
     qmax = pair32_max(pair16_max(qmax));
     const int qe = __builtin_amdgcn_frexp_expf(qmax);
-    f16x8 qhi[NG], qlo[NG];
+    f16x8 qb[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         f16x2 hi, lo;
         kv4_parts(ldexpf(qraw[j][e], 14 - qe), ldexpf(qraw[j][e + 1], 14 - qe), minus1, hi, lo);
-        qhi[j][e] = hi[0], qhi[j][e + 1] = hi[1];
-        qlo[j][e] = lo[0], qlo[j][e + 1] = lo[1];
+        qb[j][e] = second ? lo[0] : hi[0];
+        qb[j][e + 1] = second ? lo[1] : hi[1];
       }
     // log2(e) / sqrt(head), and q's scale back
     const float scale2 = ldexpf(1.4426950408889634f / sqrtf((float)head), qe - 14);
@@ -187,17 +225,33 @@ struct Kv4Partial {
     }
     const uint32_t fg = (lane & 15) >> 2, fp = lane & 3;  // its group and piece
 
-    f32x4 o[8];  // tile n: lane has word rows 4 grp + r of head h
+    // This lane's places in the wave's part of a buffer, in bytes: of score tile T the
+    // row 16 T + 4 (h % 4) + h / 4; of the values rows 4 r4 + grp and 16 more (and 32
+    // more for the second half's lanes where the products are of 64 positions).
+    const uint32_t krow = 4 * (h & 3) + (h >> 2);
+    const uint32_t kword = krow * (16 * NG) + (NG == 4 ? grp ^ (h & 3) : grp) * (4 * NG);
+    const uint32_t vrow = grp + (PAIRED && second ? 32 : 0);
+    const uint32_t i = NG >= 3 ? h % (4 * NG) : h % (4 * NG) % 8;  // (more than the words: not used)
+    const uint32_t vscale = S::HALF + S::CODES + (vrow * NG + i % NG) * 4;
+    uint32_t vword[NG == 4 ? 4 : 1];  // ... for each r4 at head 128, whose pieces are exchanged
+    if constexpr (NG == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r4 = 0; r4 < 4; ++r4)
+        vword[r4] = S::HALF + vrow * 64 + ((h >> 2) ^ r4) * 16 + (h & 3) * 4;
+    } else {
+      vword[0] = S::HALF + (vrow * (4 * NG) + i) * 4;
+    }
+
+    f32x4 o[8];  // tile n: lane has word rows 4 grp + r of its column
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // m: the reference maximum; l: this lane's positions
 
     const uint32_t nch = (n + CROWS - 1) / CROWS;
     uint32_t b = 0;  // chunk c's ring buffer
     for (uint32_t c = 0; c < nch; ++c) {
       char *buf = lds + b * S::CHUNK + wave * S::WAVE;
-      uint32_t *kw = (uint32_t *)buf, *vw = (uint32_t *)(buf + S::CODES);
-      uint32_t *kp = (uint32_t *)(buf + 2 * S::CODES), *vp = kp + S::SCALES / 4;
+      const uint32_t first = c * CROWS + wave * WROWS;  // the wave's first row
       // chunks requested after this one: the first NCH - 1, and then as the buffers
       // came free, up to the last
       const uint32_t later = min(c + NCH, max(nch, (uint32_t)NCH)) - 1 - c;
@@ -206,58 +260,69 @@ struct Kv4Partial {
           wait_chunks<0>(later);
           const uint32_t r = (n - 1) % WROWS, w = fp * NG + fg;
           const uint32_t at = NG == 4 ? (r * 4 + (fp ^ (r >> 2 & 3))) * 4 + fg : r * (4 * NG) + w;
+          uint32_t *to = (uint32_t *)(buf + (lane & 16 ? S::HALF : 0));
           if (lane < 32 && fg < NG) {
-            (lane & 16 ? vw : kw)[at] = word;
-            if (fp == 0) (lane & 16 ? vp : kp)[r * NG + fg] = sb;
+            to[at] = word;
+            if (fp == 0) to[S::CODES / 4 + r * NG + fg] = sb;
           }
           wave_lds_order();
         }
       }
       wait_chunks<S::VREQ>(later);
-      // scores: A row `h` is position 16 T + 4 (h % 4) + h / 4
-      f32x4 sc[2];
+      // scores: of 16 positions each; sc[r] is position 16 (r / 4) + 4 (r % 4) + grp of
+      // this lane's half, raw
+      float sc[8];
+      {
+        f32x4 t[4];
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        const uint32_t r = 16 * T + 4 * (h & 3) + (h >> 2);
-        uint32_t w[NG], ps[NG];
-        if constexpr (NG == 4) {
-          const u32x4 a = ((const u32x4 *)kw)[r * 4 + (grp ^ (h & 3))], b = ((const u32x4 *)kp)[r];
+        for (int T = 0; T < 4; ++T) {
+          const char *kw = buf + kword + T * (256 * NG);
+          const char *kp = buf + S::CODES + krow * (4 * NG) + T * (64 * NG);
+          uint32_t w[NG], ps[NG];
+          if constexpr (NG == 4) {
+            const u32x4 a = *(const u32x4 *)kw, b4 = *(const u32x4 *)kp;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = a[j], ps[j] = b[j];
-        } else {
+            for (int j = 0; j < 4; ++j) w[j] = a[j], ps[j] = b4[j];
+          } else {
 #pragma unroll
-          for (int j = 0; j < NG; ++j) w[j] = kw[r * (4 * NG) + grp * NG + j], ps[j] = kp[r * NG + j];
+            for (int j = 0; j < NG; ++j)
+              w[j] = ((const uint32_t *)kw)[j], ps[j] = ((const uint32_t *)kp)[j];
+          }
+          t[T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+            t[T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_numbers(w[j], ps[j], bits), qb[j], t[T], 0, 0, 0);
         }
-        f32x4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          const f16x8 a = kv4_numbers(w[j], ps[j], bits);
-          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qhi[j], hi, 0, 0, 0);
-          lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qlo[j], lo, 0, 0, 0);
+        for (int r = 0; r < 8; ++r) {
+          const float x = t[r >> 2][r & 3], y = t[2 + (r >> 2)][r & 3];
+          sc[r] = (second ? y : x) + other_half(second ? x : y);
         }
-        // lane: row 4 grp + r, position 16 T + 4 r + grp, of head h
-        const uint32_t first = c * CROWS + wave * WROWS + 16 * T + grp;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sc[T][i] = first + 4 * i < n ? (hi[i] + lo[i]) * scale2 : -INFINITY;
       }
-      float mc = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-      mc = pair32_max(pair16_max(mc));
+      if (first + WROWS > n) {
+        const uint32_t at = first + (second ? 32 : 0) + grp;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (at + 16 * (r >> 2) + 4 * (r & 3) >= n) sc[r] = -INFINITY;
+      }
+      float mc = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])),
+                       fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+      mc = fmaxf(mc, other_half(mc));
+      mc = pair32_max(pair16_max(mc)) * scale2;
       if (__any(mc > m + KV4_SLACK)) {
         const float mn = fmaxf(m, mc);
         const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= f;
+        for (int x = 0; x < 8; ++x) o[x] *= f;
         l *= f;
         m = mn;
       }
       // (a wave with no position yet has m = -inf, and weights 0)
-      const float mu = (m == -INFINITY ? 0.f : m) - KV4_BITS;
+      const float mu = KV4_BITS - (m == -INFINITY ? 0.f : m);
       f16x8 ph, pl;
       float pw[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pw[e] = __builtin_amdgcn_exp2f(sc[e / 4][e % 4] - mu);
+      for (int e = 0; e < 8; ++e) pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], scale2, mu));
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         f16x2 hi, lo;
@@ -266,58 +331,59 @@ struct Kv4Partial {
         pl[e] = lo[0], pl[e + 1] = lo[1];
       }
       l += ((pw[0] + pw[1]) + (pw[2] + pw[3])) + ((pw[4] + pw[5]) + (pw[6] + pw[7]));
-      // values: words of positions e = 4 T + r, row 16 T + 4 r + grp
+      // values: word i of positions e = 4 T + r, row 16 T + 4 r + grp
       wait_chunks<0>(later);
-      const uint32_t i = NG == 4 ? h : h % (4 * NG);  // (rows past the words are not used)
-      uint32_t vraw[8], sraw[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t r4 = e & 3, r = 16 * (e >> 2) + 4 * r4 + grp;
-        vraw[e] = NG == 4 ? vw[r * 16 + ((h >> 2) ^ r4) * 4 + (h & 3)] : vw[r * (4 * NG) + i];
-        sraw[e] = vp[r * NG + i % NG];
-      }
-      if constexpr (APPEND) {
-        // Rows past the split hold what the new row's place held before: nothing that a
-        // weight of 0 is sure to cancel.  As numbers they become 0.
-        const uint32_t first = c * CROWS + wave * WROWS;
-        if (first + WROWS > n) {
+      for (int half = 0; half < (PAIRED ? 1 : 2); ++half) {
+        uint32_t vraw[8], sraw[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (first + 16 * (e >> 2) + 4 * (e & 3) + grp >= n) sraw[e] = 0;
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t r = 32 * half + 16 * (e >> 2) + 4 * (e & 3);
+          vraw[e] = *(const uint32_t *)(buf + vword[NG == 4 ? e & 3 : 0] + r * (16 * NG));
+          sraw[e] = *(const uint32_t *)(buf + vscale + r * (4 * NG));
         }
-      }
-      uint32_t wl[4], wh[4];
-      f16x2 vs2[4], vb2[4];
+        if constexpr (APPEND) {
+          // Rows past the split hold what the new row's place held before: nothing that a
+          // weight of 0 is sure to cancel.  As numbers they become 0.
+          if (first + WROWS > n) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t w0 = vraw[2 * u], w1 = vraw[2 * u + 1], s0 = sraw[2 * u], s1 = sraw[2 * u + 1];
-        wl[u] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-        wh[u] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
-        vs2[u] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
-        vb2[u] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
-      }
-      auto tile = [&](const uint32_t (&x)[4], auto nib) {
-        f16x8 a;
+            for (int e = 0; e < 8; ++e)
+              if (first + vrow + 32 * half + 16 * (e >> 2) + 4 * (e & 3) >= n) sraw[e] = 0;
+          }
+        }
+        // hi in the columns whose positions these are, lo in the others
+        f16x8 pb = ph;
+        if constexpr (!PAIRED) pb = half ? halves<0x3>(ph, pl) : halves<0xc>(ph, pl);
+        uint32_t wl[4], wh[4];
+        f16x2 vs2[4], vb2[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const f16x2 v = __builtin_elementwise_fma(kv4_pair<decltype(nib)::value>(x[u], bits), vs2[u], vb2[u]);
-          a[2 * u] = v[0];
-          a[2 * u + 1] = v[1];
+          const uint32_t w0 = vraw[2 * u], w1 = vraw[2 * u + 1], s0 = sraw[2 * u], s1 = sraw[2 * u + 1];
+          wl[u] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+          wh[u] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+          vs2[u] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
+          vb2[u] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
         }
-        return a;
-      };
-      auto values = [&](int at, const f16x8 &a) {
-        o[at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[at], 0, 0, 0);
-        o[at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[at], 0, 0, 0);
-      };
-      values(0, tile(wl, Nib<0>{}));
-      values(1, tile(wl, Nib<1>{}));
-      values(2, tile(wl, Nib<2>{}));
-      values(3, tile(wl, Nib<3>{}));
-      values(4, tile(wh, Nib<0>{}));
-      values(5, tile(wh, Nib<1>{}));
-      values(6, tile(wh, Nib<2>{}));
-      values(7, tile(wh, Nib<3>{}));
+        auto values = [&](int at, const uint32_t (&x)[4], auto nib) {
+          f16x8 a;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const f16x2 v = __builtin_elementwise_fma(kv4_pair<decltype(nib)::value>(x[u], bits), vs2[u], vb2[u]);
+            a[2 * u] = v[0];
+            a[2 * u + 1] = v[1];
+          }
+          if constexpr (PAIRED) o[at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[at], 0, 0, 0);
+          o[at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb, o[at], 0, 0, 0);
+        };
+        values(0, wl, Nib<0>{});
+        values(1, wl, Nib<1>{});
+        values(2, wl, Nib<2>{});
+        values(3, wl, Nib<3>{});
+        values(4, wh, Nib<0>{});
+        values(5, wh, Nib<1>{});
+        values(6, wh, Nib<2>{});
+        values(7, wh, Nib<3>{});
+      }
       // refill the buffer once this wave's reads of it have returned
       if (c + NCH < nch) {
         wave_lds_order();
@@ -330,10 +396,12 @@ struct Kv4Partial {
     // every request has landed before the ring is reused
     wait_vmcnt<0>();
     l = pair32_sum(pair16_sum(l));
+    l += other_half(l);
     const float mr = m - KV4_BITS;  // the weights are relative to this
+    auto stats = [&](uint32_t w) { return (float *)(lds + STATS + w * S::WAVE); };  // maxima, sums
     if (lane < KV4_MAX_GROUP) {
-      s_m[wave * KV4_MAX_GROUP + lane] = mr;
-      s_l[wave * KV4_MAX_GROUP + lane] = l;
+      stats(wave)[lane] = mr;
+      stats(wave)[KV4_MAX_GROUP + lane] = l;
     }
     if constexpr (APPEND) {
       if (owner && lane < 32 && fg < NG) {
@@ -343,30 +411,33 @@ struct Kv4Partial {
       }
     }
     __syncthreads();
-    // this wave's tiles to the workgroup's maximum, rows [w][h][d]
-    if (h < G) {
-      float M = s_m[h];
+    // this lane's columns to the workgroup's maximum, rows [2 w + half][h][d]
+    const uint32_t hq = h & 7;
+    float *total_ml = stats(0) + 2 * KV4_MAX_GROUP;  // the workgroup's maxima, sums
+    if (hq < G) {
+      float M = stats(0)[hq];
 #pragma unroll
-      for (int w = 1; w < AMMON_WAVES; ++w) M = fmaxf(M, s_m[w * KV4_MAX_GROUP + h]);
+      for (int w = 1; w < AMMON_WAVES; ++w) M = fmaxf(M, stats(w)[hq]);
       // M is finite: a live split's first position is wave 0's
       const float f = __builtin_amdgcn_exp2f(mr - M);
-      float *row = (float *)lds + (wave * KV4_MAX_GROUP + h) * ATT_STAGED_OROW;
+      float *row = (float *)lds + ((2 * wave + second) * KV4_MAX_GROUP + hq) * OROW;
+      const bool block = !PAIRED || (grp >= 2) == second;  // its positions' words
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t w = 4 * grp + r;  // word (w / NG, w % NG)
-        if (NG == 4 || w < 4 * NG) {
+        const uint32_t w = PAIRED ? 4 * (grp & 1) + r : 4 * grp + r;  // word (w / NG, w % NG)
+        if (block && (NG == 4 || w < 4 * NG)) {
           float4 *to = (float4 *)(row + 32 * (w % NG) + 8 * (w / NG));
           to[0] = make_float4(o[0][r] * f, o[4][r] * f, o[1][r] * f, o[5][r] * f);
           to[1] = make_float4(o[2][r] * f, o[6][r] * f, o[3][r] * f, o[7][r] * f);
         }
       }
-      if (wave == 0 && grp == 0) {
+      if (wave == 0 && lane < KV4_MAX_GROUP) {
         float L = 0.f;
 #pragma unroll
         for (int w = 0; w < AMMON_WAVES; ++w)
-          L += s_l[w * KV4_MAX_GROUP + h] * __builtin_amdgcn_exp2f(s_m[w * KV4_MAX_GROUP + h] - M);
-        s_M[h] = M;
-        s_L[h] = L;
+          L += stats(w)[KV4_MAX_GROUP + hq] * __builtin_amdgcn_exp2f(stats(w)[hq] - M);
+        total_ml[hq] = M;
+        total_ml[KV4_MAX_GROUP + hq] = L;
       }
     }
     __syncthreads();
@@ -375,9 +446,9 @@ struct Kv4Partial {
       const uint32_t j = idx / head, d = idx - j * head;
       float total = 0.f;
 #pragma unroll
-      for (int w = 0; w < AMMON_WAVES; ++w)
-        total += ((const float *)lds)[(w * KV4_MAX_GROUP + j) * ATT_STAGED_OROW + d];
-      const float M = s_M[j], L = s_L[j];
+      for (uint32_t w = 0; w < MROWS; ++w)
+        total += ((const float *)lds)[(w * KV4_MAX_GROUP + j) * OROW + d];
+      const float M = total_ml[j], L = total_ml[KV4_MAX_GROUP + j];
       if (direct_out(p)) {
         st_out(p.out + (size_t)(g * G + j) * head + d, total / L);
         continue;
