@@ -880,7 +880,7 @@ AMMON_DEV void attention_combine_wave(const ammon_k_attention &p, uint32_t h) {
   const bool mine = 2 * lane < head, both = 2 * lane + 1 < head;  // (an odd head's last dim)
   float *out = p.out + (size_t)h * head + 2 * lane;
   const uint32_t pos = p.step->position + p.pos_add;
-  if (pos >= p.limit) {
+  if (pos >= p.limit || pos < p.pos_add) {  // (or past the last number)
     if (mine) {
       st_out(out, __uint_as_float(0x7fc00000u));
       if (both) st_out(out + 1, __uint_as_float(0x7fc00000u));

@@ -85,24 +85,24 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_load(ammon_k_kv
   }
 }
 
-// Pass 1 on a (splits, kv heads, tokens) grid.
-#define KV4_PARTIAL(NAME, NG, NCH, APPEND)                                            \
+// Pass 1 on a (splits, kv heads, sets of eight query rows) grid.
+#define KV4_PARTIAL(NAME, NG, MODE)                                                   \
   extern "C" __global__ __launch_bounds__(AMMON_WG, 2) void NAME(const ammon_k_step *step, \
                                                                 ammon_k_attention p_) { \
-    using Unit = Kv4Partial<NG, NCH, APPEND>;                                          \
+    using Unit = Kv4Partial<NG, MODE>;                                                 \
     __shared__ u32x4 lds[Unit::LDS_BYTES / 16];                                        \
-    ammon_k_attention p0 = p_;                                                         \
-    p0.step = step;                                                                    \
-    const ammon_k_attention p = attention_token(p0, blockIdx.z);                       \
+    ammon_k_attention p = p_;                                                          \
+    p.step = step;                                                                     \
     Unit unit;                                                                         \
-    if (unit.begin(p, blockIdx.x, blockIdx.y, (char *)lds))                            \
+    if (unit.begin(p, blockIdx.x, blockIdx.y, blockIdx.z, (char *)lds))                \
       unit.run(p, (char *)lds);                                                        \
     else                                                                               \
-      direct_out_nan(p, blockIdx.y);                                                   \
+      unit.out_of_range(p);                                                            \
   }
-#define KV4_PARTIAL_NG(NG)                                      \
-  KV4_PARTIAL(ammon_kv4_partial_n##NG, NG, 2, false)            \
-  KV4_PARTIAL(ammon_kv4_partial_append_n##NG, NG, 2, true)
+#define KV4_PARTIAL_NG(NG)                                          \
+  KV4_PARTIAL(ammon_kv4_partial_n##NG, NG, KV4_DECODE)              \
+  KV4_PARTIAL(ammon_kv4_partial_append_n##NG, NG, KV4_APPEND)       \
+  KV4_PARTIAL(ammon_kv4_partial_tokens_n##NG, NG, KV4_TOKENS)
 KV4_PARTIAL_NG(1)
 KV4_PARTIAL_NG(2)
 KV4_PARTIAL_NG(3)

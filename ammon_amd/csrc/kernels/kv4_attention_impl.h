@@ -1,8 +1,10 @@
 // kv4_attention_impl.h -- split-K decode attention over a KV4 cache (kv4_impl.h).
 //
 // Pass 1 of attention_impl.h's pair, any head up to 128 and up to 8 query heads per
-// kv head: one workgroup per (split, kv head), on matrix cores; the partials have
-// the other units' format, so pass 2 is theirs.  Chunks of 256 positions, 64 per
+// kv head: one workgroup per (split, kv head, eight query rows), on matrix cores; the
+// partials have the other units' format, so pass 2 is theirs.  The query rows of a kv
+// head are its query heads, token by token: a decode step has one set of rows, a short
+// prompt fills the sets with several tokens' heads.  Chunks of 256 positions, 64 per
 // wave; NCH chunks are requested ahead into a ring in LDS of which every wave reads
 // back only its own rows, so the chunk loop has no barrier.
 //
@@ -25,6 +27,10 @@
 //           product takes 64 positions: lanes 0..7 of A and columns 0..7 are the first
 //           32, the others the second, and the two blocks in which they meet are not
 //           used.
+//
+// Tokens of one set see different numbers of positions.  Scores past a token's own are
+// masked; a value that is not finite there, which a weight of 0 would not cancel, is
+// taken as 0 and noted, and the outputs that it does belong to become NaN at the end.
 //
 // What bounds it: HBM where the context is long, the two launches where it is short.
 // (Hi and lo in two products of one column half, and 32 positions per wave, took twice
@@ -52,9 +58,14 @@ template <int NG> struct Kv4Stage {
   static constexpr int REQ = 2 * VREQ;
 };
 
-template <int NG, int NCH, bool APPEND>
+// A decode step, a decode step that appends its rows, several tokens of a prompt.
+enum Kv4Mode { KV4_DECODE, KV4_APPEND, KV4_TOKENS };
+
+template <int NG, Kv4Mode MODE>
 struct Kv4Partial {
   using S = Kv4Stage<NG>;
+  static constexpr int NCH = 2;
+  static constexpr bool APPEND = MODE == KV4_APPEND, TOKENS = MODE == KV4_TOKENS;
   static constexpr uint32_t WROWS = S::ROWS, CROWS = AMMON_WAVES * WROWS;
   static constexpr bool PAIRED = NG <= 2;              // 64 positions a value product
   static constexpr uint32_t OROW = 32 * NG + 4;        // merge row: banks spread
@@ -64,9 +75,13 @@ struct Kv4Partial {
   // A wave's maxima and sums wait for the merge in its part of the last ring buffer,
   // past the merge's rows.
   static constexpr uint32_t STATS = S::CHUNK * (NCH - 1);
-  static_assert(NCH >= 2 && NCH <= 4 && MERGE <= STATS, "chunk buffers");
+  static_assert(MERGE <= STATS, "chunk buffers");
 
-  uint32_t split, g, G, pos, t0, n, lane, wave;
+  uint32_t split, g, G, lane, wave;
+  uint32_t pos, t0, n;        // the first token's position; the split's first, and how many
+                              // of them the last token sees
+  uint32_t mine, fewest;      // ... this lane's column's token, the first token
+  uint32_t row0, cols, rows;  // the set's first row, its rows, and all the rows
   const uint32_t *kc, *ks, *vc, *vs;  // codes and scales of the split's first row
   float qraw[NG][8];
   bool owner;      // APPEND: this wave has the new position
@@ -130,23 +145,36 @@ struct Kv4Partial {
   }
 
   // False for a dead split or a position out of range, which write nothing.
-  AMMON_DEV bool begin(const ammon_k_attention &p, uint32_t split_, uint32_t g_, char *lds) {
+  // Token `t` in range, and the split's first position seen by it.
+  AMMON_DEV bool alive(const ammon_k_attention &p, uint32_t t) const {
+    return pos + t < p.limit && t0 <= pos + t;
+  }
+  AMMON_DEV bool begin(const ammon_k_attention &p, uint32_t split_, uint32_t g_, uint32_t set,
+                       char *lds) {
     split = split_;
     g = g_;
     G = p.q_heads / p.kv_heads;
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // q beside the position: neither needs the other.  (Columns past the group take
-    // head 0's; they are never used.)
-    const uint32_t h = lane & 7;
-    const float *q = p.q + (size_t)(g * G + (h < G ? h : 0)) * p.head;
+    rows = TOKENS ? p.tokens * G : G;
+    row0 = TOKENS ? set * KV4_MAX_GROUP : 0;
+    cols = min(rows - row0, (uint32_t)KV4_MAX_GROUP);
+    // q beside the position: neither needs the other.  (Columns past the rows take the
+    // last one's; they are never used.)
+    const uint32_t row = row0 + min(lane & 7, cols - 1);
+    const uint32_t tok = TOKENS ? row / G : 0, first = TOKENS ? row0 / G : 0;
+    const uint32_t last = TOKENS ? (row0 + cols - 1) / G : 0;
+    const float *q = p.q + ((size_t)tok * p.q_heads + g * G + (row - tok * G)) * p.head;
 #pragma unroll
     for (int j = 0; j < NG; ++j) kv4_row(q, 4 * j + (lane >> 4), p.head, qraw[j]);
-    pos = p.step->position + p.pos_add;
-    if (pos >= p.limit) return false;
+    pos = min(p.step->position, p.limit);  // (no sum with it wraps around)
     t0 = split * p.split_len;
-    if (t0 > pos) return false;
-    n = min(p.split_len, pos + 1 - t0);
+    if (pos + first >= p.limit) return false;
+    const uint32_t end = min(pos + last, p.limit - 1);
+    if (t0 > end) return false;
+    n = min(p.split_len, end + 1 - t0);
+    mine = !TOKENS ? n : alive(p, tok) ? min(p.split_len, pos + tok + 1 - t0) : 0;
+    fewest = !TOKENS ? n : alive(p, first) ? min(p.split_len, pos + first + 1 - t0) : 0;
     kc = kv4_codes(p.k_cache, p.seq, NG, g, t0);
     vc = kv4_codes(p.v_cache, p.seq, NG, g, t0);
     ks = kv4_scales(p.k_cache, p.kv_heads, p.seq, NG, g, t0);
@@ -172,11 +200,10 @@ struct Kv4Partial {
     return true;
   }
 
-  // Wait until at most EXTRA requests and k whole chunks of this wave are outstanding.
+  // Wait until at most EXTRA requests and k whole chunks (0 or 1) of this wave are
+  // outstanding.
   template <int EXTRA> AMMON_DEV static void wait_chunks(uint32_t k) {
-    if (NCH > 3 && k >= 3) wait_vmcnt<EXTRA + 3 * S::REQ>();
-    else if (NCH > 2 && k == 2) wait_vmcnt<EXTRA + 2 * S::REQ>();
-    else if (NCH > 1 && k == 1) wait_vmcnt<EXTRA + S::REQ>();
+    if (k == 1) wait_vmcnt<EXTRA + S::REQ>();
     else wait_vmcnt<EXTRA>();
   }
 
@@ -246,12 +273,14 @@ struct Kv4Partial {
 #pragma unroll
     for (int x = 0; x < 8; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // m: the reference maximum; l: this lane's positions
+    uint32_t bad = ~0u;            // first noted position of this lane's group of 32 numbers
 
     const uint32_t nch = (n + CROWS - 1) / CROWS;
     uint32_t b = 0;  // chunk c's ring buffer
     for (uint32_t c = 0; c < nch; ++c) {
       char *buf = lds + b * S::CHUNK + wave * S::WAVE;
       const uint32_t first = c * CROWS + wave * WROWS;  // the wave's first row
+      if (first >= n) break;  // (uniform; this is the last chunk)
       // chunks requested after this one: the first NCH - 1, and then as the buffers
       // came free, up to the last
       const uint32_t later = min(c + NCH, max(nch, (uint32_t)NCH)) - 1 - c;
@@ -299,11 +328,11 @@ struct Kv4Partial {
           sc[r] = (second ? y : x) + other_half(second ? x : y);
         }
       }
-      if (first + WROWS > n) {
+      if (first + WROWS > fewest) {
         const uint32_t at = first + (second ? 32 : 0) + grp;
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (at + 16 * (r >> 2) + 4 * (r & 3) >= n) sc[r] = -INFINITY;
+          if (at + 16 * (r >> 2) + 4 * (r & 3) >= mine) sc[r] = -INFINITY;
       }
       float mc = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])),
                        fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
@@ -349,6 +378,16 @@ struct Kv4Partial {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               if (first + vrow + 32 * half + 16 * (e >> 2) + 4 * (e & 3) >= n) sraw[e] = 0;
+          }
+        }
+        if (TOKENS && fewest < n && first + WROWS > fewest) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t at = first + vrow + 32 * half + 16 * (e >> 2) + 4 * (e & 3), x = sraw[e];
+            if (at >= fewest && ((x & 0x7c00u) == 0x7c00u || (x >> 16 & 0x7c00u) == 0x7c00u)) {
+              bad = min(bad, min(at, n - 1));  // (rows past the split are copies of its last)
+              sraw[e] = 0;
+            }
           }
         }
         // hi in the columns whose positions these are, lo in the others
@@ -403,6 +442,17 @@ struct Kv4Partial {
       stats(wave)[lane] = mr;
       stats(wave)[KV4_MAX_GROUP + lane] = l;
     }
+    if constexpr (TOKENS) {
+      // (uniform) the positions noted of each group of numbers, as the wave's first
+      if (fewest < n) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          uint32_t x = i % NG == j ? bad : ~0u;
+          for (int s = 1; s < 64; s *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, s));
+          if (lane == 0) ((uint32_t *)stats(wave))[4 * KV4_MAX_GROUP + j] = x;
+        }
+      }
+    }
     if constexpr (APPEND) {
       if (owner && lane < 32 && fg < NG) {
         const void *cache = lane & 16 ? p.v_cache : p.k_cache;
@@ -414,11 +464,11 @@ struct Kv4Partial {
     // this lane's columns to the workgroup's maximum, rows [2 w + half][h][d]
     const uint32_t hq = h & 7;
     float *total_ml = stats(0) + 2 * KV4_MAX_GROUP;  // the workgroup's maxima, sums
-    if (hq < G) {
+    if (hq < cols) {
       float M = stats(0)[hq];
 #pragma unroll
       for (int w = 1; w < AMMON_WAVES; ++w) M = fmaxf(M, stats(w)[hq]);
-      // M is finite: a live split's first position is wave 0's
+      // M is finite where the column's token is alive: the first position is wave 0's
       const float f = __builtin_amdgcn_exp2f(mr - M);
       float *row = (float *)lds + ((2 * wave + second) * KV4_MAX_GROUP + hq) * OROW;
       const bool block = !PAIRED || (grp >= 2) == second;  // its positions' words
@@ -442,23 +492,51 @@ struct Kv4Partial {
     }
     __syncthreads();
     const uint32_t slot_w = head + 2;
-    for (uint32_t idx = threadIdx.x; idx < G * head; idx += AMMON_WG) {
+    for (uint32_t idx = threadIdx.x; idx < cols * head; idx += AMMON_WG) {
       const uint32_t j = idx / head, d = idx - j * head;
+      uint32_t tok = 0, hh = j;
       float total = 0.f;
 #pragma unroll
       for (uint32_t w = 0; w < MROWS; ++w)
         total += ((const float *)lds)[(w * KV4_MAX_GROUP + j) * OROW + d];
+      if constexpr (TOKENS) {
+        tok = (row0 + j) / G;
+        hh = row0 + j - tok * G;
+        if (!alive(p, tok)) {  // a merge writes the NaN of a position out of range
+          if (direct_out(p)) write_nan(p, tok, hh, d);
+          continue;
+        }
+        if (fewest < n) {
+          uint32_t x = ~0u;
+          for (uint32_t w = 0; w < AMMON_WAVES; ++w)
+            x = min(x, ((const uint32_t *)stats(w))[4 * KV4_MAX_GROUP + d / 32]);
+          if (x <= pos + tok - t0) total = __uint_as_float(0x7fc00000u);
+        }
+      }
       const float M = total_ml[j], L = total_ml[KV4_MAX_GROUP + j];
+      const size_t row = (size_t)tok * p.q_heads + g * G + hh;
       if (direct_out(p)) {
-        st_out(p.out + (size_t)(g * G + j) * head + d, total / L);
+        st_out(p.out + row * head + d, total / L);
         continue;
       }
-      float *to = p.partial + ((size_t)(g * G + j) * p.splits + split) * slot_w;
+      float *to = p.partial + (row * p.splits + split) * slot_w;
       st_out(to + d, total);
       if (d == 0) {
         st_out(to + head, M * 0.6931471805599453f);  // natural-log units
         st_out(to + head + 1, L);
       }
+    }
+  }
+
+  AMMON_DEV void write_nan(const ammon_k_attention &p, uint32_t tok, uint32_t hh, uint32_t d) const {
+    st_out(p.out + ((size_t)tok * p.q_heads + g * G + hh) * p.head + d, __uint_as_float(0x7fc00000u));
+  }
+  // A set that did not begin: with one split, all its tokens are out of range.
+  AMMON_DEV void out_of_range(const ammon_k_attention &p) const {
+    if (!direct_out(p)) return;
+    for (uint32_t idx = threadIdx.x; idx < cols * p.head; idx += AMMON_WG) {
+      const uint32_t j = idx / p.head, tok = (row0 + j) / G;
+      write_nan(p, tok, row0 + j - tok * G, idx - j * p.head);
     }
   }
 

@@ -302,7 +302,7 @@ struct Kv4PrefillTile {
     lane = threadIdx.x & 63;
     h = lane >> 5;
     head = p.head;
-    const uint32_t start = p.step->position;
+    const uint32_t start = min(p.step->position, p.limit);  // (no sum with it wraps around)
     const uint32_t G = p.q_heads / p.kv_heads, rows = p.tokens * G;
     const uint32_t w0 = tile * KV4_PF_ROWS + 32 * wave;  // the wave's first row
     live = w0 < rows;

@@ -67,7 +67,7 @@ struct Kernels {
   hipFunction_t kv4_store = nullptr;
   hipFunction_t kv4_rope_store = nullptr;
   hipFunction_t kv4_load = nullptr;
-  hipFunction_t kv4_partial[2][kKv4Groups] = {};
+  hipFunction_t kv4_partial[3][kKv4Groups] = {};  // [Kv4Mode]
   hipFunction_t kv4_prefill[kKv4Groups] = {};  // prefill tiles
 };
 

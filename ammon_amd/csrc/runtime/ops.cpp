@@ -261,16 +261,19 @@ int att_group_index(uint32_t g) {
   return -1;
 }
 
+enum Kv4Mode { kKv4Decode, kKv4Append, kKv4Tokens };
+
 // Pass-1 variant for a cache layout, or NULL when no chunk width fits (KV4: when the
 // caches are not aligned).
 // split_len 0: the kernel a split of 128 positions would take (occupancy
 // queries before the split is chosen).
 hipFunction_t attention_kernel(ammon_runtime *rt, ammon_dtype kv_dtype, uint32_t q_heads,
                                uint32_t kv_heads, uint32_t head, const void *k, const void *v,
-                               uint32_t split_len, bool append = false) {
+                               uint32_t split_len, Kv4Mode mode = kKv4Decode) {
   if (kv_dtype == AMMON_KV4)
-    return (((uintptr_t)k | (uintptr_t)v) & 15u) == 0 ? rt->k.kv4_partial[append][(head - 1) / 32]
-                                                      : nullptr;
+    return (((uintptr_t)k | (uintptr_t)v) & 15u) == 0
+               ? rt->k.kv4_partial[mode][(head - 1) / 32]
+               : nullptr;
   const int ci = att_chunk_index(kv_dtype, head, k, v);
   if (ci < 0) return nullptr;
   const int gi = att_group_index(q_heads / kv_heads);
@@ -366,9 +369,12 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
 //           after the first's,
 //   merge   a launch, and the partials written and read; rows of which one split sees
 //           anything write their result themselves.
-// Measured at 32 q / 8 kv heads of 128 (units, tiles, us): 64 tokens after 500: 15, 32; 64
-// after 4000: 78, 43 (16 kv heads, 40 tokens: 84, 43); 300 after 3000: 314, 50; 2048: 852,
-// 98 in one split, 101 in two; heads of 64: 64 after 500: 12, 22; 64 after 4000: 52, 36.
+// Units' time is a launch or two, and per workgroup (a set of eight rows, a split) a start
+// and the positions that it sees, at least its chunk of 256.
+// Measured at 32 q / 8 kv heads of 128 (units, tiles, us): 200 tokens 20.8, 18.7; 64 after
+// 500: 12.7, 32; 64 after 4000: 38, 51; 64 after 8000: 66, 53; 130 after 4000: 72, 48; heads
+// of 64: 64 after 4000: 25, 36; 64 after 8000: 39, 37.  Tiles of 300 tokens after 3000: 50;
+// of 2048: 98 in one split, 101 in two.
 PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
                              uint32_t head, uint32_t ctx, uint32_t scratch_splits, bool aligned) {
   PrefillPlan plan;
@@ -377,7 +383,10 @@ PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_head
   if (!aligned || rows >= (1ull << 31)) return plan;
   const double chunk_ns = 500 + 560 * ng;
   const double seen = ctx - tokens / 2.0;  // positions a token sees, on average
-  const double unit_ns = 6e3 + tokens * kv_heads * seen * (0.015 + 0.007 * ng);
+  const double unit_ns =
+      (scratch_splits > 1 ? 9e3 : 5e3) +
+      (double)cdiv(rows, 8) * kv_heads *
+          (6.0 * scratch_splits + std::max(seen, 256.0) * (0.004 + 0.0065 * ng));
   if (10e3 + chunk_ns >= unit_ns) return plan;  // (the shortest tiles: a small call asks no further)
   const double cus = std::max(rt->info.compute_units, 1);
   double best = unit_ns;
@@ -667,7 +676,7 @@ ammon_status attention_pass1(ammon_runtime *rt, ammon_stream stream, const float
   ammon_status st = attention_check(rt, "attention_partial", q_heads, kv_heads, head, seq, split_len);
   if (st != AMMON_OK) return st;
   hipFunction_t f = attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache,
-                                     split_len, k_new != nullptr);
+                                     split_len, k_new ? kKv4Append : kKv4Decode);
   AMMON_CHECK(f || kv_dtype != AMMON_KV4, "attention_partial: KV4 caches must be 16-byte aligned");
   AMMON_CHECK(f, "attention_partial: head %u needs an even width above 64", head);
   VALIDATE_ONLY();
@@ -919,7 +928,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
                   !overlaps(q, qbytes, partial, need),
               "attention_prefill: q, partial and out must not overlap");
   hipFunction_t f =
-      attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache, split_len);
+      attention_kernel(rt, kv_dtype, q_heads, kv_heads, head, k_cache, v_cache, split_len, kKv4Tokens);
   AMMON_CHECK(f || kv_dtype != AMMON_KV4, "attention_prefill: KV4 caches must be 16-byte aligned");
   AMMON_CHECK(f, "attention_prefill: head %u needs an even width above 64", head);
   VALIDATE_ONLY();
@@ -946,7 +955,10 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
   } else {
     // one split: the units write the merge's result themselves, as in decode
     p.single_out = splits == 1;
-    st = launch_att(rt, stream, f, splits, kv_heads, tokens, p, "attention_prefill");
+    // (KV4 units take eight query rows of a kv head, several tokens' where the group is smaller)
+    const uint32_t sets =
+        kv_dtype == AMMON_KV4 ? cdiv((uint64_t)tokens * (q_heads / kv_heads), 8) : tokens;
+    st = launch_att(rt, stream, f, splits, kv_heads, sets, p, "attention_prefill");
     if (st != AMMON_OK || splits == 1) return st;
   }
   return launch_att(rt, stream, rt->k.att_combine_waves, cdiv(q_heads, kWaves), 1, tokens, p,

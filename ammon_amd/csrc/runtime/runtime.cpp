@@ -181,10 +181,11 @@ static ammon_status load_kernels(ammon_runtime *rt) {
   R(7, "ammon_kv4_store", k.kv4_store);
   R(7, "ammon_kv4_rope_store", k.kv4_rope_store);
   R(7, "ammon_kv4_load", k.kv4_load);
-  for (int a = 0; a < 2; ++a)
+  const char *const mode[] = {"", "append_", "tokens_"};
+  for (int a = 0; a < 3; ++a)
     for (int n = 0; n < kKv4Groups; ++n) {
       char name[96];
-      snprintf(name, sizeof name, "ammon_kv4_partial_%sn%d", a ? "append_" : "", n + 1);
+      snprintf(name, sizeof name, "ammon_kv4_partial_%sn%d", mode[a], n + 1);
       R(7, name, k.kv4_partial[a][n]);
     }
   for (int n = 0; n < kKv4Groups; ++n) {

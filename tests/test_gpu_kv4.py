@@ -451,3 +451,58 @@ def test_prefill_in_a_graph(rt):
         np.testing.assert_array_equal(got, prefill(rt, q, c, start, 256, ctx=1500))
     call("ammon_graph_destroy", rt.handle, graph)
     call("ammon_stream_destroy", rt.handle, stream)
+
+
+# ---- a few tokens at a time: units of eight query rows of several tokens ------------------------
+SETS = [(6, 6, 48), (12, 4, 80), (8, 8, 128), (10, 2, 64), (32, 8, 128), (14, 2, 96), (16, 2, 33)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,head", SETS)
+@pytest.mark.parametrize("start,tokens", [(0, 2), (0, 17), (63, 3), (250, 13), (509, 9), (780, 19)])
+def test_prefill_few_tokens(rt, heads, kv_heads, head, start, tokens):
+    c = Cache(rt, kv_heads, 900, head, filled=start + tokens)
+    q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
+    for split in (256, 300, 1024):
+        assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+@pytest.mark.parametrize("heads,kv_heads,head", SETS)
+@pytest.mark.parametrize("start,at", [(0, 5), (60, 63), (60, 64), (250, 255), (250, 256), (250, 250)])
+def test_prefill_few_tokens_not_finite(rt, heads, kv_heads, head, start, at):
+    """A row that is not finite among the prompt's own: no token before it is touched."""
+    tokens = 12
+    for side in (0, 1):
+        c = Cache(rt, kv_heads, 700, head, filled=start + tokens)
+        for p, g, d in ((at, kv_heads - 1, head - 1), (start + tokens - 1, 0, 0)):
+            row = c.numbers(1, p)[side].astype(np.float32)
+            row[g, 0, d] = np.nan
+            kv4.pack(c.host[side], kv_heads, 700, head, p, row)
+        c.dev[side].upload(c.host[side])
+        q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+        want = kv4.attention(q, *c.numbers(start + tokens), start)
+        nan = np.isnan(want).any(-1)
+        assert nan[at - start:, -1].all() and nan[-1, 0] and not nan[:at - start].any()
+        for split in (128, 1024):
+            assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+@pytest.mark.parametrize("heads,kv_heads,head", [(6, 6, 48), (12, 4, 80)])
+@pytest.mark.parametrize("split", [64, 1024])
+def test_prefill_few_tokens_out_of_range(rt, heads, kv_heads, head, split):
+    """Tokens past ctx, and past the last position there is, give NaN; the others their rows."""
+    c = Cache(rt, kv_heads, 300, head, filled=300)
+    q = oracle.normal(10 * heads * head, 9).reshape(10, heads, head)
+    got = prefill(rt, q, c, 297, split, ctx=300)
+    assert off(got[:3], kv4.attention(q[:3], *c.numbers(300), 297)) <= TOL
+    assert np.isnan(got[3:]).all()
+    for start in (300, 2**32 - 4):
+        assert np.isnan(prefill(rt, q, c, start, split, ctx=300)).all()
+
+
+def test_prefill_past_the_last_position_there_is(rt):
+    c = Cache(rt, 4, 1000, 64, filled=1000)
+    q = oracle.normal(700 * 8 * 64, 9).reshape(700, 8, 64)
+    for start in (2**32 - 1, 2**32 - 256, 2**32 - 700):
+        for split in (1024, 100):
+            assert np.isnan(prefill(rt, q, c, start, split, ctx=900)).all()
