@@ -19,6 +19,7 @@ extern "C" {
 #define AMMON_K_F32 0
 #define AMMON_K_BF16 1
 #define AMMON_K_KV4 4 /* KV caches only: kernels/kv4_impl.h */
+#define AMMON_KV4_LOAD_ROWS 4 /* rows a lane of kv4_load takes */
 
 /* Device-resident control parcel: same layout as ammon_decode_step. */
 typedef struct {

@@ -563,7 +563,7 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
               first, count, seq);
   AMMON_CHECK((((uintptr_t)k_out | (uintptr_t)v_out) & 15u) == 0,
               "kv4_load: outputs must be 16-byte aligned");
-  AMMON_CHECK((uint64_t)count * kv_heads < (1ull << 34), "kv4_load: too many rows");
+  AMMON_CHECK((uint64_t)count * kv_heads < (1ull << 32) - 1024, "kv4_load: too many rows");
   const size_t rows = (size_t)count * kv_heads * head * dsize(out_dtype);
   const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
   for (const void *out : {k_out, v_out})
@@ -583,7 +583,8 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
   p.seq = seq;
   p.first = first;
   p.out_dtype = (uint32_t)out_dtype;
-  return launch(rt, stream, rt->k.kv4_load, cdiv((uint64_t)count * kv_heads, kWorkgroup / 16),
+  return launch(rt, stream, rt->k.kv4_load,
+                cdiv((uint64_t)count * kv_heads, kWorkgroup / 16 * AMMON_KV4_LOAD_ROWS),
                 v_out ? 2 : 1, 0, p, "kv4_load");
 }
 
