@@ -94,6 +94,7 @@ typedef struct {
                                rest, in reverse order (0: order as launched) */
   const float *k_new;       /* KV4 pass 1, append: the position's own key and value */
   const float *v_new;       /* rows [kv_heads, head], stored by the unit that has it */
+  uint32_t group;           /* KV4 pass 1: q_heads / kv_heads */
 } ammon_k_attention;
 
 /* KV4 rows stored and read back. */

@@ -15,9 +15,10 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_store(ammon_k_k
   if (pos >= p.seq) return;  // out of range: the cache stays as it is
   const float *src = blockIdx.y ? p.v : p.k;
   void *cache = blockIdx.y ? p.v_cache : p.k_cache;
-  float x[8];
-  kv4_row(src + (size_t)r * p.head, i, p.head, x);
-  kv4_put(cache, p.kv_heads, p.seq, p.head, g, (uint32_t)pos, i, x);
+  float x[1][8];
+  kv4_rows(src + (size_t)r * p.head, i, p.head, x);
+  kv4_row_ends(i, p.head, x);
+  kv4_put(cache, p.kv_heads, p.seq, p.head, g, (uint32_t)pos, i, x[0]);
 }
 
 // rope_store (rope.hip) into a KV4 cache: q rotated in place, a lane per pair, by the
@@ -42,8 +43,10 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_rope_store(ammo
   const uint32_t g = (blockIdx.x - qblocks) * (AMMON_WG / 16) + threadIdx.x / 16;
   if (g >= p.kv_heads) return;
   const uint32_t i = threadIdx.x & 15;
-  float x[8];
-  kv4_row(p.k + (size_t)g * p.head, i, p.head, x);
+  float row[1][8];
+  kv4_rows(p.k + (size_t)g * p.head, i, p.head, row);
+  kv4_row_ends(i, p.head, row);
+  float (&x)[8] = row[0];
 #pragma unroll
   for (uint32_t e = 0; e < 8; e += 2) {
     const uint32_t d = 8 * i + e;

@@ -84,8 +84,8 @@ struct Kv4Partial {
   uint32_t row0, cols, rows;  // the set's first row, its rows, and all the rows
   const uint32_t *kc, *ks, *vc, *vs;  // codes and scales of the split's first row
   float qraw[NG][8];
-  bool owner;      // APPEND: this wave has the new position
-  float fresh[8];  // ... lanes 0..15: the new key, 16..31: the new value
+  bool owner;         // APPEND: this wave has the new position
+  float fresh[1][8];  // ... lanes 0..15: the new key, 16..31: the new value
 
   // The 16-byte piece of the wave's rows that LDS slot `at` of its codes holds.  At head
   // 128 a row's pieces are exchanged by its place, so that the 8 lanes of a score
@@ -153,20 +153,21 @@ struct Kv4Partial {
                        char *lds) {
     split = split_;
     g = g_;
-    G = p.q_heads / p.kv_heads;
+    G = p.group;
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     rows = TOKENS ? p.tokens * G : G;
     row0 = TOKENS ? set * KV4_MAX_GROUP : 0;
     cols = min(rows - row0, (uint32_t)KV4_MAX_GROUP);
-    // q beside the position: neither needs the other.  (Columns past the rows take the
+    // q and the new rows beside the position: none needs another.  (Columns past the rows take the
     // last one's; they are never used.)
     const uint32_t row = row0 + min(lane & 7, cols - 1);
     const uint32_t tok = TOKENS ? row / G : 0, first = TOKENS ? row0 / G : 0;
     const uint32_t last = TOKENS ? (row0 + cols - 1) / G : 0;
     const float *q = p.q + ((size_t)tok * p.q_heads + g * G + (row - tok * G)) * p.head;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) kv4_row(q, 4 * j + (lane >> 4), p.head, qraw[j]);
+    kv4_rows(q, lane >> 4, p.head, qraw);
+    if constexpr (APPEND)
+      kv4_rows((lane & 16 ? p.v_new : p.k_new) + (size_t)g * p.head, lane & 15, p.head, fresh);
     pos = min(p.step->position, p.limit);  // (no sum with it wraps around)
     t0 = split * p.split_len;
     if (pos + first >= p.limit) return false;
@@ -179,23 +180,18 @@ struct Kv4Partial {
     vc = kv4_codes(p.v_cache, p.seq, NG, g, t0);
     ks = kv4_scales(p.k_cache, p.kv_heads, p.seq, NG, g, t0);
     vs = kv4_scales(p.v_cache, p.kv_heads, p.seq, NG, g, t0);
-    // q has come with the position, or nearly: waiting for it here keeps the compiler's
-    // wait for it, which would be for every request, out of the way of the requests
+    // they have come with the position, or nearly: waiting for them here keeps the
+    // compiler's wait, which would be for every request, out of the way of the requests
 #pragma unroll
-    for (int j = 0; j < NG; ++j)
+    for (int e = 0; e < 8; ++e) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(qraw[j][e]));
-    owner = false;
-    if constexpr (APPEND) {
-      // the split's last position is the new one
-      owner = pos < t0 + p.split_len && (n - 1) % CROWS / WROWS == wave;
-      if (owner) {
-        const float *x = (lane & 16 ? p.v_new : p.k_new) + (size_t)g * p.head;
-        kv4_row(x, lane & 15, p.head, fresh);
-      }
+      for (int j = 0; j < NG; ++j) asm volatile("" : "+v"(qraw[j][e]));
+      if constexpr (APPEND) asm volatile("" : "+v"(fresh[0][e]));
     }
-#pragma unroll
-    for (int b = 0; b < NCH; ++b) stage(lds, b, b);
+    // the split's last position is the new one
+    owner = APPEND && pos < t0 + p.split_len && (n - 1) % CROWS / WROWS == wave;
+    stage(lds, 0, 0);
+    if (n > CROWS) stage(lds, 1, 1);
     __builtin_amdgcn_sched_barrier(0);
     return true;
   }
@@ -226,6 +222,7 @@ struct Kv4Partial {
     const Kv4Bits bits;
     const float minus1 = kv4_minus1();
     // q^T as the B operand, fp16 hi or lo of q 2^(14 - e), |q| < 2^e
+    kv4_row_ends(grp, head, qraw);
     float qmax = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
@@ -248,7 +245,10 @@ struct Kv4Partial {
 
     uint32_t word = 0, sb = 0;
     if constexpr (APPEND) {
-      if (owner) kv4_quantise(fresh, lane & 15, head, word, sb);
+      if (owner) {
+        kv4_row_ends(lane & 15, head, fresh);
+        kv4_quantise(fresh[0], lane & 15, head, word, sb);
+      }
     }
     const uint32_t fg = (lane & 15) >> 2, fp = lane & 3;  // its group and piece
 
@@ -281,9 +281,7 @@ struct Kv4Partial {
       char *buf = lds + b * S::CHUNK + wave * S::WAVE;
       const uint32_t first = c * CROWS + wave * WROWS;  // the wave's first row
       if (first >= n) break;  // (uniform; this is the last chunk)
-      // chunks requested after this one: the first NCH - 1, and then as the buffers
-      // came free, up to the last
-      const uint32_t later = min(c + NCH, max(nch, (uint32_t)NCH)) - 1 - c;
+      const uint32_t later = min(c + NCH, nch) - 1 - c;  // chunks requested after this one
       if constexpr (APPEND) {
         if (owner && c == nch - 1) {  // the new row, into this wave's copy
           wait_chunks<0>(later);
@@ -491,52 +489,56 @@ struct Kv4Partial {
       }
     }
     __syncthreads();
-    const uint32_t slot_w = head + 2;
-    for (uint32_t idx = threadIdx.x; idx < cols * head; idx += AMMON_WG) {
-      const uint32_t j = idx / head, d = idx - j * head;
+    // a query row to a wave, two dimensions to a lane
+    const uint32_t d = 2 * lane;
+    for (uint32_t j = wave; j < cols; j += AMMON_WAVES) {
       uint32_t tok = 0, hh = j;
-      float total = 0.f;
-#pragma unroll
-      for (uint32_t w = 0; w < MROWS; ++w)
-        total += ((const float *)lds)[(w * KV4_MAX_GROUP + j) * OROW + d];
       if constexpr (TOKENS) {
         tok = (row0 + j) / G;
         hh = row0 + j - tok * G;
         if (!alive(p, tok)) {  // a merge writes the NaN of a position out of range
-          if (direct_out(p)) write_nan(p, tok, hh, d);
+          if (direct_out(p)) write_nan(p, tok, hh);
           continue;
         }
-        if (fewest < n) {
-          uint32_t x = ~0u;
-          for (uint32_t w = 0; w < AMMON_WAVES; ++w)
-            x = min(x, ((const uint32_t *)stats(w))[4 * KV4_MAX_GROUP + d / 32]);
-          if (x <= pos + tok - t0) total = __uint_as_float(0x7fc00000u);
+      }
+      float a = 0.f, b = 0.f;
+      if (d < head) {
+#pragma unroll
+        for (uint32_t w = 0; w < MROWS; ++w) {
+          const float2 x = *(const float2 *)((const float *)lds + (w * KV4_MAX_GROUP + j) * OROW + d);
+          a += x.x;
+          b += x.y;
         }
+      }
+      if (TOKENS && fewest < n) {
+        uint32_t x = ~0u;
+        for (uint32_t w = 0; w < AMMON_WAVES; ++w)
+          x = min(x, ((const uint32_t *)stats(w))[4 * KV4_MAX_GROUP + min(d / 32, NG - 1u)]);
+        if (x <= pos + tok - t0) a = b = __uint_as_float(0x7fc00000u);
       }
       const float M = total_ml[j], L = total_ml[KV4_MAX_GROUP + j];
       const size_t row = (size_t)tok * p.q_heads + g * G + hh;
-      if (direct_out(p)) {
-        st_out(p.out + row * head + d, total / L);
-        continue;
-      }
-      float *to = p.partial + (row * p.splits + split) * slot_w;
-      st_out(to + d, total);
-      if (d == 0) {
+      const bool direct = direct_out(p);
+      float *to = direct ? p.out + row * head : p.partial + (row * p.splits + split) * (head + 2);
+      if (d < head) st_out(to + d, direct ? a / L : a);
+      if (d + 1 < head) st_out(to + d + 1, direct ? b / L : b);
+      if (!direct && lane == 0) {
         st_out(to + head, M * 0.6931471805599453f);  // natural-log units
         st_out(to + head + 1, L);
       }
     }
   }
 
-  AMMON_DEV void write_nan(const ammon_k_attention &p, uint32_t tok, uint32_t hh, uint32_t d) const {
-    st_out(p.out + ((size_t)tok * p.q_heads + g * G + hh) * p.head + d, __uint_as_float(0x7fc00000u));
+  AMMON_DEV void write_nan(const ammon_k_attention &p, uint32_t tok, uint32_t hh) const {
+    float *to = p.out + ((size_t)tok * p.q_heads + g * G + hh) * p.head;
+    for (uint32_t d = lane; d < p.head; d += 64) st_out(to + d, __uint_as_float(0x7fc00000u));
   }
   // A set that did not begin: with one split, all its tokens are out of range.
   AMMON_DEV void out_of_range(const ammon_k_attention &p) const {
     if (!direct_out(p)) return;
-    for (uint32_t idx = threadIdx.x; idx < cols * p.head; idx += AMMON_WG) {
-      const uint32_t j = idx / p.head, tok = (row0 + j) / G;
-      write_nan(p, tok, row0 + j - tok * G, idx - j * p.head);
+    for (uint32_t j = wave; j < cols; j += AMMON_WAVES) {
+      const uint32_t tok = (row0 + j) / G;
+      write_nan(p, tok, row0 + j - tok * G);
     }
   }
 

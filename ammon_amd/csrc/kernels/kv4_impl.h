@@ -30,6 +30,7 @@
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // at any float
 
 #define KV4_LIMIT 16384.0f
 
@@ -113,19 +114,37 @@ AMMON_DEV void kv4_quantise(const float (&x)[8], uint32_t i, uint32_t head, uint
           : 0x7e007e00u;
 }
 
-// Numbers 8 i .. + 7 of an fp32 row, zeros past the head (no branch where head is a
-// multiple of 8: a lane past it reads the last ones).
-AMMON_DEV void kv4_row(const float *row, uint32_t i, uint32_t head, float (&x)[8]) {
+// Numbers 8 (i + 4 j) .. + 7 of an fp32 row, j < N, zeros past the head: every load is
+// requested before any is used, and a lane past the head reads the last numbers (a branch
+// or a select between the loads had them wait for each other: 1 us in a decode step).
+template <int N>
+AMMON_DEV void kv4_rows(const float *row, uint32_t i, uint32_t head, float (&x)[N][8]) {
   if (head % 8 == 0) {
-    const uint32_t at = min(8 * i, head - 8);
-    const float4 a = ld_in4(row + at), b = ld_in4(row + at + 4);
-    const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 8 * i < head ? y[e] : 0.f;
+    for (int j = 0; j < N; ++j) {
+      const uint32_t at = min(8 * (i + 4 * j), head - 8);
+      const f32x4_any a = *(const f32x4_any *)(row + at), b = *(const f32x4_any *)(row + at + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[j][e] = e < 4 ? a[e] : b[e - 4];
+    }
   } else {
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) x[e] = 8 * i + e < head ? ld_in(row + 8 * i + e) : 0.f;
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) x[j][e] = ld_in(row + min(8 * (i + 4 * j) + e, head - 1));
+    // (they are waited for here: left pending, they would be in the other path's waits too)
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(x[j][e]));
   }
+}
+// ... and the zeros, once they are to be used.
+template <int N> AMMON_DEV void kv4_row_ends(uint32_t i, uint32_t head, float (&x)[N][8]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) x[j][e] = 8 * (i + 4 * j) + e < head ? x[j][e] : 0.f;
 }
 
 // Where row (g, t) of a cache has its words and its scales | biases.

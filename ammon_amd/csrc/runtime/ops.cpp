@@ -684,7 +684,8 @@ ammon_status attention_pass1(ammon_runtime *rt, ammon_stream stream, const float
   const uint32_t splits = ammon_attention_splits(seq, split_len);
   ammon_k_attention p = {q, k_cache, v_cache, (const ammon_k_step *)step, partial, single_out,
                          q_heads, kv_heads, head, seq, split_len, splits, 0, seq,
-                         single_out ? 1u : 0u, nullptr, 0, 0, 0, 0, 0, 1, 0, k_new, v_new};
+                         single_out ? 1u : 0u, nullptr, 0, 0, 0, 0, 0, 1, 0, k_new, v_new,
+                         q_heads / kv_heads};
   return launch_att(rt, stream, f, splits, kv_heads, 1, p, "attention_partial");
 }
 
@@ -771,7 +772,7 @@ ammon_status ammon_attention_combine_warm(ammon_runtime *rt, ammon_stream stream
   ammon_k_attention p = {nullptr, nullptr, nullptr, (const ammon_k_step *)step, (float *)partial,
                          out, q_heads, 1, head, seq, split_len,
                          ammon_attention_splits(seq, split_len), 0, seq, 0, nullptr, 0, 0, 0, 0, 0, 1, 0,
-                         nullptr, nullptr};
+                         nullptr, nullptr, 0};
   const uint32_t grid = q_heads * cdiv(head, 8);
   if (next_w) {
     // The next GEMV (a RESIDUAL-mode ammon_gemv of next_rows x next_n) gives
@@ -939,7 +940,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
   const uint32_t splits = ammon_attention_splits(ctx, split_len);
   ammon_k_attention p = {q, k_cache, v_cache, (const ammon_k_step *)step, partial, out,
                          q_heads, kv_heads, head, seq, split_len, splits, 0, ctx, 0, nullptr, 0, 0, 0, 0, 0,
-                         tokens, 0, nullptr, nullptr};
+                         tokens, 0, nullptr, nullptr, q_heads / kv_heads};
   const uintptr_t bits = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache;
   const bool aligned = (bits & 15u) == 0 && ((uintptr_t)partial & 7u) == 0;
   const PrefillPlan plan =
