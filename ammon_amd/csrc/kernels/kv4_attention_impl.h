@@ -32,10 +32,18 @@
 // masked; a value that is not finite there, which a weight of 0 would not cancel, is
 // taken as 0 and noted, and the outputs that it does belong to become NaN at the end.
 //
-// What bounds it: HBM where the context is long, the two launches where it is short.
-// (Hi and lo in two products of one column half, and 32 positions per wave, took twice
-// the matrix instructions, and up to head 64 twice the vector ones: then these
-// bounded it.)
+// What bounds it.  Long contexts: HBM (8 kv heads of 64, 131072 positions: 84 MB in 23.8
+// us with the merge, some 9 us of which any two dependent launches take).  Short ones: a
+// wave's chain through its one chunk, in cycles 1800 for q and the position, 2900 until
+// the chunk is there, 1650 for scores and weights, 1650 for values, 2600 for the merge of
+// the waves and the partial; 525 vector and 32 matrix instructions a chunk, and a wave
+// has its SIMD for itself (8192 positions of 8 heads of 128: 8.2 us, merge 3.3).
+// Measured and not kept: hi and lo in products of their own and 32 positions per wave
+// (twice the matrix instructions, up to head 64 twice the vector ones: 34.0 us and 12.0
+// where the above are 23.8 and 10.0 with the merge); units of eight waves (the same up to
+// 32768 positions, 54 us against 41 at 131072 of head 128, where one fits on a CU in
+// place of two).  A third chunk in the ring would leave room for two units per CU up to
+// head 64, not four.
 #pragma once
 
 #include "attention_impl.h"
