@@ -25,6 +25,8 @@ size_t storage_bytes(const Shape &shape, DType dtype) {
   if (r < 3) throw Error(AMMON_E_VALIDATION, "a KV4 tensor is [.., kv_heads, seq, head], not " + shape.str());
   size_t bytes =
       ammon_kv_cache_bytes(AMMON_KV4, shape.dims[r - 3], shape.dims[r - 2], shape.dims[r - 1]);
+  if (r == 3) return bytes;
+  bytes = (bytes + 15) / 16 * 16;  // of a stack, every cache is aligned
   for (size_t i = 0; i + 3 < r; ++i) bytes *= shape.dims[i];
   return bytes;
 }
@@ -86,7 +88,8 @@ TensorView TensorView::narrow(size_t axis, uint32_t start, uint32_t len) const {
   }
   if (dtype_ == DType::KV4 && axis + 3 >= shape_.rank())
     throw Error(AMMON_E_VALIDATION, "narrow: a KV4 cache " + shape_.str() + " is not divisible");
-  const Shape inner = Shape{{shape_.dims.begin() + axis + 1, shape_.dims.end()}};
+  Shape inner = Shape{{shape_.dims.begin() + axis + 1, shape_.dims.end()}};
+  if (dtype_ == DType::KV4) inner.dims.insert(inner.dims.begin(), 1);  // (one of a stack)
   Shape s = shape_;
   s.dims[axis] = len;
   return TensorView((char *)ptr_ + (size_t)start * storage_bytes(inner, dtype_), s, dtype_);

@@ -692,7 +692,8 @@ ammon_status attention_pass1(ammon_runtime *rt, ammon_stream stream, const float
 // What an append asks beyond pass 1's own checks.
 ammon_status append_check(const char *what, const float *q, uint32_t q_heads, const float *k,
                           const float *v, const void *k_cache, const void *v_cache,
-                          ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t head, uint32_t seq) {
+                          ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t head, uint32_t seq,
+                          const float *partial, uint32_t split_len, const float *out) {
   AMMON_CHECK(kv_dtype == AMMON_KV4,
               "%s: only a KV4 cache is appended to (qkv_rope_store stores the rows of others)", what);
   AMMON_CHECK(k && v && k_cache && v_cache, "%s: NULL rows or cache", what);
@@ -704,6 +705,16 @@ ammon_status append_check(const char *what, const float *q, uint32_t q_heads, co
     AMMON_CHECK(!overlaps(k, row, cache, bytes) && !overlaps(v, row, cache, bytes) &&
                     !overlaps(q, qrow, cache, bytes),
                 "%s: q or the rows overlap a cache", what);
+  // some workgroups read their rows after others have written
+  const size_t scratch =
+      split_len ? ammon_attention_scratch_bytes(q_heads, head, seq, split_len) : 0;
+  for (const float *from : {k, v})
+    AMMON_CHECK(!overlaps(from, row, partial, scratch) && !(out && overlaps(from, row, out, qrow)),
+                "%s: the rows overlap the output or the scratch", what);
+  for (const void *cache : {k_cache, v_cache})
+    AMMON_CHECK(!overlaps(cache, bytes, partial, scratch) &&
+                    !(out && overlaps(cache, bytes, out, qrow)),
+                "%s: a cache overlaps the output or the scratch", what);
   return AMMON_OK;
 }
 }  // namespace
@@ -729,7 +740,7 @@ ammon_status ammon_attention_partial_append(ammon_runtime *rt, ammon_stream stre
                                             float *partial) {
   REQUIRE_RT();
   ammon_status st = append_check("attention_partial_append", q, q_heads, k, v, k_cache, v_cache,
-                                 kv_dtype, kv_heads, head, seq);
+                                 kv_dtype, kv_heads, head, seq, partial, split_len, nullptr);
   if (st != AMMON_OK) return st;
   return attention_pass1(rt, stream, q, q_heads, k_cache, v_cache, kv_dtype, kv_heads, head, seq,
                          step, split_len, partial, nullptr, k, v);
@@ -897,7 +908,7 @@ ammon_status ammon_attention_decode_append(ammon_runtime *rt, ammon_stream strea
                                            float *partial, size_t partial_bytes, float *out) {
   REQUIRE_RT();
   ammon_status st = append_check("attention_append", q, q_heads, k, v, k_cache, v_cache, kv_dtype,
-                                 kv_heads, head, seq);
+                                 kv_heads, head, seq, partial, split_len, out);
   if (st != AMMON_OK) return st;
   return attention_decode(rt, stream, q, q_heads, k, v, k_cache, v_cache, kv_dtype, kv_heads, head,
                           seq, step, split_len, partial, partial_bytes, out);

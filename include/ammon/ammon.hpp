@@ -83,7 +83,8 @@ struct Shape {
   bool operator==(const Shape &o) const { return dims == o.dims; }
 };
 
-// Bytes of a contiguous tensor.  KV4 tensors are stacked caches [.., kv_heads, seq, head].
+// Bytes of a contiguous tensor.  KV4 tensors are stacked caches [.., kv_heads, seq, head],
+// each at a multiple of 16 bytes.
 size_t storage_bytes(const Shape &shape, DType dtype);
 
 // Non-owning device view: pointer, shape, storage dtype.

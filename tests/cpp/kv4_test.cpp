@@ -24,7 +24,7 @@ template <typename F> bool throws(F &&f) {
 
 TEST(storage_bytes_of_kv4) {
   CHECK(ammon::storage_bytes(Shape::from_dims({3, 7, 128}), DType::KV4) == 3 * 7 * 80);
-  CHECK(ammon::storage_bytes(Shape::from_dims({2, 5, 3, 7, 33}), DType::KV4) == 10 * 3 * 7 * 40);
+  CHECK(ammon::storage_bytes(Shape::from_dims({2, 5, 3, 7, 33}), DType::KV4) == 10 * (3 * 7 * 40 + 8));
   CHECK(ammon::storage_bytes(Shape::from_dims({3, 7, 128}), DType::BF16) == 3 * 7 * 256);
   CHECK(throws([] { ammon::storage_bytes(Shape::from_dims({7, 128}), DType::KV4); }));
   CHECK(throws([] { ammon::dtype_size(DType::KV4); }));
@@ -40,6 +40,15 @@ TEST(views_of_kv4) {
   CHECK(throws([&] { v.narrow(2, 0, 4); }));
   CHECK(throws([&] { l.reshape({16, 2, 64}); }));
   CHECK(throws([&] { l.reshape({2, 8, 128}); }));
+}
+
+TEST(stacked_caches_are_aligned) {
+  // 3 x 7 rows of 40 bytes are no multiple of 16
+  const TensorView v((char *)4096, Shape::from_dims({2, 5, 3, 7, 33}), DType::KV4);
+  const TensorView a = v.narrow(0, 1, 1).narrow(1, 3, 1);
+  CHECK((char *)a.data() == (char *)4096 + 8 * 848);
+  CHECK(a.reshape({3, 7, 33}).nbytes() == 840);
+  CHECK(v.nbytes() == 10 * 848);
 }
 
 TEST(cache_records_and_reads_back) {

@@ -506,3 +506,63 @@ def test_prefill_past_the_last_position_there_is(rt):
     for start in (2**32 - 1, 2**32 - 256, 2**32 - 700):
         for split in (1024, 100):
             assert np.isnan(prefill(rt, q, c, start, split, ctx=900)).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,head", [(32, 8, 128), (8, 4, 64), (6, 2, 33)])
+def test_rows_at_any_float(rt, heads, kv_heads, head):
+    """q, the rows and the output a float past 16 bytes."""
+    seq, tokens = 300, 5
+    q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+    rows = [oracle.normal(tokens * kv_heads * head, s).reshape(tokens, kv_heads, head) for s in (1, 2)]
+    kept = [up(rt, np.concatenate([np.zeros(1, np.float32), a.ravel()])) for a in (q, *rows)]
+    dq, dk, dv = (b.offset(4) for b in kept)
+    step = rt.step(0, 0)
+    nbytes = int(lib.ammon_kv_cache_bytes(KV4, kv_heads, seq, head))
+    caches = [up(rt, np.zeros(nbytes, np.uint8)) for _ in "kv"]
+    call("ammon_kv4_store", rt.handle, None, dk, dv, tokens, kv_heads, head, *caches, seq, step)
+    k, v = (kv4.stored(r).transpose(1, 0, 2) for r in rows)
+    n = int(lib.ammon_attention_prefill_scratch_bytes(tokens, heads, head, tokens, 256))
+    part, out = rt.alloc(n + 4), rt.alloc(q.nbytes + 4)
+    call("ammon_attention_prefill", rt.handle, None, dq, tokens, heads, *caches, KV4, kv_heads, head,
+         seq, step, tokens, 256, part.offset(4), n, out.offset(4))
+    got = out.download(q.size + 1)[1:].reshape(q.shape)
+    assert off(got, kv4.attention(q, k, v, 0)) <= TOL
+    # the first token again at the next position, with its rows
+    n = int(lib.ammon_attention_scratch_bytes(heads, head, seq, 100))
+    part = rt.alloc(n + 4)
+    call("ammon_attention_decode_append", rt.handle, None, dq, heads, dk, dv, *caches, KV4, kv_heads,
+         head, seq, rt.step(0, tokens), 100, part.offset(4), n, out.offset(4))
+    got = out.download(heads * head + 1)[1:].reshape(1, heads, head)
+    k, v = (np.concatenate([x, x[:, :1]], 1) for x in (k, v))
+    assert off(got, kv4.attention(q[:1], k, v, tokens)) <= TOL
+
+
+def test_two_graphs_and_a_stream_share_a_cache(rt):
+    """Decode graphs of two streams with scratch of their own, replayed in turn and at once."""
+    heads, kv_heads, head, seq = 32, 8, 128, 2000
+    c = Cache(rt, kv_heads, seq, head, filled=seq)
+    n = int(lib.ammon_attention_scratch_bytes(heads, head, seq, 256))
+    runs = []
+    for seed in (1, 2):
+        stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+        call("ammon_stream_create", rt.handle, ctypes.byref(stream))
+        q = oracle.normal(heads * head, seed).reshape(1, heads, head)
+        dq, part, out, step = up(rt, q), rt.alloc(n), rt.alloc(q.nbytes), rt.step(0, 0)
+        rt.synchronize()
+        call("ammon_capture_begin", rt.handle, stream)
+        call("ammon_attention_decode", rt.handle, stream, dq, heads, *c.dev, KV4, kv_heads, head, seq,
+             step, 256, part, n, out)
+        call("ammon_capture_end", rt.handle, stream, ctypes.byref(graph))
+        runs.append((stream, graph, q, step, out, (dq, part)))
+    for at in ((0, 1999), (700, 3), (255, 256)):
+        for (stream, graph, q, step, out, _), pos in zip(runs, at):
+            rt.deposit(step, 0, pos, stream)
+        for _ in range(3):
+            for stream, graph, *_ in runs:
+                call("ammon_graph_launch", rt.handle, graph, stream)
+        for (stream, graph, q, step, out, _), pos in zip(runs, at):
+            got = out.download(q.shape, stream=stream)
+            assert off(got, kv4.attention(q, *c.numbers(pos + 1), pos)) <= TOL
+    for stream, graph, *_ in runs:
+        call("ammon_graph_destroy", rt.handle, graph)
+        call("ammon_stream_destroy", rt.handle, stream)

@@ -32,6 +32,8 @@ CONFIGS = {
     "mha48": Config(dim=288, n_layers=3, n_heads=6, n_kv_heads=6, hidden=768, vocab=500, max_seq=256),
     "gqa128_bf16": Config(dim=512, n_layers=2, n_heads=4, n_kv_heads=1, hidden=512, vocab=300,
                           max_seq=1500, w_dtype=BF16),
+    # a layer's cache is 255 rows of 20 bytes: no multiple of 16
+    "odd_cache": Config(dim=64, n_layers=3, n_heads=2, n_kv_heads=1, hidden=96, vocab=100, max_seq=255),
 }
 
 
@@ -280,7 +282,9 @@ def test_refusals(rt):
                       ("multiple", dict(heads=7)), ("exceeds 8", dict(heads=18, n=4 * n)),
                       ("exceeds", dict(head=130, n=4 * n)), ("scratch", dict(n=n - 4)), ("split length", dict(split=2048, n=4 * n)),
                       ("aligned", dict(kc=at(65540))), ("caches overlap", dict(vc=at(65552))),
-                      ("overlap a cache", dict(q=at(65536))), ("overlap a cache", dict(v=at(262144)))):
+                      ("overlap a cache", dict(q=at(65536))), ("overlap a cache", dict(v=at(262144))),
+                      ("overlap the output", dict(k=at(16384))), ("overlap the output", dict(v=at(524288))),
+                      ("cache overlaps the output", dict(kc=at(16384 - 4096)))):
         bad(match, "ammon_attention_decode_append", *append(**kw))
     bad("aligned", "ammon_attention_decode", q, 8, at(65540), vc, KV4, 2, 64, 100, step, 64, part, n, out)
     bad("aligned", "ammon_attention_prefill", q, 3, 8, at(65540), vc, KV4, 2, 64, 100, step, 50, 64, part,
