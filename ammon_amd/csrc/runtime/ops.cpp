@@ -846,7 +846,11 @@ uint32_t ammon_attention_default_split_for(ammon_runtime *rt, uint32_t q_heads,
     if (f) per_cu = std::min<uint32_t>(occupancy(rt, f, 0), 2);
     const uint32_t g = q_heads / kv_heads;
     if (kv_dtype == AMMON_BF16 && head == 128 && (g & (g - 1)) == 0) min_split = 64;
-    // KV4 units' chunk is 256 positions, and one unit per CU keeps enough of
+    // A KV4 cache of one split's length is one: its units need no merge (32 q /
+    // 8 kv heads of 128, 1024 positions, append: 11.1 us against 11.2 at split
+    // 256, and after 500 positions 8.0 against 11.2; heads of 64: 8.7, 9.7).
+    if (kv_dtype == AMMON_KV4 && seq > 0 && seq <= AMMON_ATTENTION_MAX_SPLIT) return seq;
+    // Their chunk is 256 positions, and one unit per CU keeps enough of
     // them requested: 64 q / 8 kv heads of 128 at 32768 positions take 18.0 us
     // at split 1024, one unit per CU, against 19.5 at 512; 8192 positions 10.7
     // at 256 against 13.0 at 128 and 11.9 at 512.

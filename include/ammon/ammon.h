@@ -186,7 +186,9 @@ uint32_t ammon_attention_default_split(ammon_runtime *rt, uint32_t kv_heads, uin
  * fit on a CU (two, or one for a kernel that fits only once), so a kernel
  * that runs one workgroup per CU gets one round of longer splits; and the
  * matrix-core kernels (bf16 cache, head 128, power-of-two group), which
- * score 64-position chunks, get splits of at least 64. */
+ * score 64-position chunks, get splits of at least 64.  A KV4 cache's units
+ * are one per CU and their splits at least their chunk of 256; a cache of at
+ * most 1024 positions gets one split. */
 uint32_t ammon_attention_default_split_for(ammon_runtime *rt, uint32_t q_heads,
                                            uint32_t kv_heads, uint32_t head,
                                            ammon_dtype kv_dtype, uint32_t seq);
@@ -248,8 +250,8 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
  * ceil(head / 32)].
  *
  * ammon_rope_store and ammon_cache_store write rows of such a cache, the
- * attention entries read it (16 query heads' width is always computed, so any
- * group up to 8 costs the same); ammon_rope, ammon_qkv_rope_store and its
+ * attention entries read it (8 query rows' width is always computed: a group of
+ * 8 costs a decode step what a group of 1 does); ammon_rope, ammon_qkv_rope_store and its
  * prefill form do not take it: ammon_qkv_rope and ammon_prefill_qkv_rope give
  * the rows, ammon_attention_decode_append and ammon_kv4_store take them. */
 
