@@ -449,13 +449,17 @@ struct Kv4Partial {
       stats(wave)[KV4_MAX_GROUP + lane] = l;
     }
     if constexpr (TOKENS) {
-      // (uniform) the positions noted of each group of numbers, as the wave's first
+      // the first position noted of each group of numbers, as a rule none
       if (fewest < n) {
+        uint32_t *noted = (uint32_t *)stats(wave) + 4 * KV4_MAX_GROUP;
+        if (lane < NG) noted[lane] = ~0u;
+        if (__any(bad != ~0u)) {
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          uint32_t x = i % NG == j ? bad : ~0u;
-          for (int s = 1; s < 64; s *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, s));
-          if (lane == 0) ((uint32_t *)stats(wave))[4 * KV4_MAX_GROUP + j] = x;
+          for (int j = 0; j < NG; ++j) {
+            uint32_t x = i % NG == j ? bad : ~0u;
+            for (int s = 1; s < 64; s *= 2) x = min(x, (uint32_t)__shfl_xor((int)x, s));
+            if (lane == 0) noted[j] = x;
+          }
         }
       }
     }
