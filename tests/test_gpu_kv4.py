@@ -566,3 +566,61 @@ def test_two_graphs_and_a_stream_share_a_cache(rt):
     for stream, graph, *_ in runs:
         call("ammon_graph_destroy", rt.handle, graph)
         call("ammon_stream_destroy", rt.handle, stream)
+
+
+# ---- borders of a wave's 64 positions, of a chunk's 256, of the ring's two chunks ----------------
+@pytest.mark.parametrize("pos", [63, 64, 191, 192, 255, 256, 511, 512, 767, 768, 1030])
+@pytest.mark.parametrize("heads,kv_heads,head", [(16, 2, 128), (6, 2, 96), (7, 7, 64), (2, 1, 20)])
+def test_decode_and_append_at_borders(rt, heads, kv_heads, head, pos):
+    a, b = (Cache(rt, kv_heads, 1100, head, filled=pos) for _ in "ab")
+    q = oracle.normal(heads * head, 9).reshape(heads, head)
+    k, v = rows_of(kv_heads, 1, head, 5), rows_of(kv_heads, 1, head, 50)
+    store(rt, b, k, v, pos)
+    b.pack(pos, k, v)
+    want = kv4.attention(q[None], *b.numbers(pos + 1), pos)[0]
+    for split in (1024, 768, 300, 256):
+        got = decode(rt, q, a, pos, split, new=(k, v))
+        np.testing.assert_array_equal(got, decode(rt, q, b, pos, split))
+        assert off(got, want) <= TOL, split
+    b.same()
+    a.pack(pos, k, v)
+    a.same()
+
+
+def test_caches_past_32_bits(rt):
+    """5 GB each: rows of the last heads at the last positions stored, read back, attended to."""
+    heads = kv_heads = 64
+    head, seq, tokens = 128, (1 << 20) - 3, 5
+    nbytes = int(lib.ammon_kv_cache_bytes(KV4, kv_heads, seq, head))
+    assert nbytes > 1 << 32
+    caches = [rt.alloc(nbytes) for _ in "kv"]
+    for c in caches:
+        rt.fill(c, F32, nbytes // 4, 0.0)  # zeros
+    k, v = rows_of(kv_heads, tokens, head, 5), rows_of(kv_heads, tokens, head, 50)
+    v += np.arange(head, dtype=np.float32) % 2 * 8192  # (so that they show beside a million zeros)
+    dk, dv = up(rt, k), up(rt, v)
+    call("ammon_kv4_store", rt.handle, None, dk, dv, tokens, kv_heads, head, *caches, seq,
+         rt.step(0, seq - tokens))
+    bufs = [rt.alloc(kv_heads * (tokens + 2) * head * 4) for _ in "kv"]
+    call("ammon_kv4_load", rt.handle, None, *caches, kv_heads, head, seq, seq - tokens - 2, tokens + 2,
+         *bufs, F32)
+    got = [b.download((kv_heads, tokens + 2, head)) for b in bufs]
+    want = [kv4.stored(x).transpose(1, 0, 2) for x in (k, v)]
+    for g, w in zip(got, want):
+        assert not g[:, :2].any()
+        np.testing.assert_array_equal(g[:, 2:], w)
+    # softmax of seq - tokens zeros and the stored rows' scores
+    q = oracle.normal(heads * head, 9).reshape(heads, head).astype(np.float64)
+    s = np.einsum("hd,htd->ht", q, want[0]) / np.sqrt(head)
+    e = np.exp(s)
+    out64 = np.einsum("ht,htd->hd", e, want[1]) / (seq - tokens + e.sum(1))[:, None]
+    n = int(lib.ammon_attention_scratch_bytes(heads, head, seq, 1024))
+    part, out = rt.alloc(n), rt.alloc(heads * head * 4)
+    call("ammon_attention_decode", rt.handle, None, up(rt, q.astype(np.float32)), heads, *caches, KV4,
+         kv_heads, head, seq, rt.step(0, seq - 1), 1024, part, n, out)
+    assert off(out.download((heads, head)), out64) <= TOL
+    # the same through the append of the last row, over what stands there
+    call("ammon_attention_decode_append", rt.handle, None, up(rt, q.astype(np.float32)), heads,
+         dk.offset(4 * (tokens - 1) * kv_heads * head), dv.offset(4 * (tokens - 1) * kv_heads * head),
+         *caches, KV4, kv_heads, head, seq, rt.step(0, seq - 1), 1024, part, n, out)
+    assert off(out.download((heads, head)), out64) <= TOL
