@@ -35,9 +35,11 @@
 // What bounds it.  Long contexts: HBM (8 kv heads of 64, 131072 positions: 84 MB in 23.8
 // us with the merge, some 9 us of which any two dependent launches take).  Short ones: a
 // wave's chain through its one chunk, in cycles 1800 for q and the position, 2900 until
-// the chunk is there, 1650 for scores and weights, 1650 for values, 2600 for the merge of
-// the waves and the partial; 525 vector and 32 matrix instructions a chunk, and a wave
-// has its SIMD for itself (8192 positions of 8 heads of 128: 8.2 us, merge 3.3).
+// the chunk is there, 1700 for scores and weights, 1650 for values, 1900 for the merge of
+// the waves and the partial (2600 with a barrier between maxima and rows); 525 vector and
+// 32 matrix instructions a chunk, and a wave has its SIMD for itself (8192 positions of 8
+// heads of 128, replayed in a graph: 9.5 us with the merge).  The wave that appends is
+// some 1200 cycles behind the others.
 // Measured and not kept: hi and lo in products of their own and 32 positions per wave
 // (twice the matrix instructions, up to head 64 twice the vector ones: 34.0 us and 12.0
 // where the above are 23.8 and 10.0 with the merge); units of eight waves (the same up to
@@ -77,13 +79,10 @@ struct Kv4Partial {
   static constexpr uint32_t WROWS = S::ROWS, CROWS = AMMON_WAVES * WROWS;
   static constexpr bool PAIRED = NG <= 2;              // 64 positions a value product
   static constexpr uint32_t OROW = 32 * NG + 4;        // merge row: banks spread
-  static constexpr uint32_t MROWS = 2 * AMMON_WAVES;   // merge rows per query head
-  static constexpr uint32_t MERGE = MROWS * KV4_MAX_GROUP * OROW * 4;
   static constexpr uint32_t LDS_BYTES = S::CHUNK * NCH;
-  // A wave's maxima and sums wait for the merge in its part of the last ring buffer,
-  // past the merge's rows.
-  static constexpr uint32_t STATS = S::CHUNK * (NCH - 1);
-  static_assert(MERGE <= STATS, "chunk buffers");
+  // For the merge a wave leaves its output rows [half of the columns][8] in its part of
+  // the first ring buffer, its maxima and sums in its part of the second.
+  static_assert(NCH == 2 && 2 * KV4_MAX_GROUP * OROW * 4 <= S::WAVE, "merge rows");
 
   uint32_t split, g, G, lane, wave;
   uint32_t pos, t0, n;        // the first token's position; the split's first, and how many
@@ -443,7 +442,8 @@ struct Kv4Partial {
     l = pair32_sum(pair16_sum(l));
     l += other_half(l);
     const float mr = m - KV4_BITS;  // the weights are relative to this
-    auto stats = [&](uint32_t w) { return (float *)(lds + STATS + w * S::WAVE); };  // maxima, sums
+    auto rows_of = [&](uint32_t w) { return (float *)(lds + w * S::WAVE); };
+    auto stats = [&](uint32_t w) { return (float *)(lds + S::CHUNK + w * S::WAVE); };  // maxima, sums
     if (lane < KV4_MAX_GROUP) {
       stats(wave)[lane] = mr;
       stats(wave)[KV4_MAX_GROUP + lane] = l;
@@ -463,6 +463,17 @@ struct Kv4Partial {
         }
       }
     }
+    const bool block = !PAIRED || (grp >= 2) == second;  // its positions' words
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t w = PAIRED ? 4 * (grp & 1) + r : 4 * grp + r;  // word (w / NG, w % NG)
+      if (block && (NG == 4 || w < 4 * NG)) {
+        float4 *to = (float4 *)(rows_of(wave) + h * OROW + 32 * (w % NG) + 8 * (w / NG));
+        to[0] = make_float4(o[0][r], o[4][r], o[1][r], o[5][r]);
+        to[1] = make_float4(o[2][r], o[6][r], o[3][r], o[7][r]);
+      }
+    }
+    __syncthreads();
     if constexpr (APPEND) {
       if (owner && lane < 32 && fg < NG) {
         const void *cache = lane & 16 ? p.v_cache : p.k_cache;
@@ -470,37 +481,6 @@ struct Kv4Partial {
         if (fp == 0) kv4_scales(cache, p.kv_heads, p.seq, NG, g, pos)[fg] = sb;
       }
     }
-    __syncthreads();
-    // this lane's columns to the workgroup's maximum, rows [2 w + half][h][d]
-    const uint32_t hq = h & 7;
-    float *total_ml = stats(0) + 2 * KV4_MAX_GROUP;  // the workgroup's maxima, sums
-    if (hq < cols) {
-      float M = stats(0)[hq];
-#pragma unroll
-      for (int w = 1; w < AMMON_WAVES; ++w) M = fmaxf(M, stats(w)[hq]);
-      // M is finite where the column's token is alive: the first position is wave 0's
-      const float f = __builtin_amdgcn_exp2f(mr - M);
-      float *row = (float *)lds + ((2 * wave + second) * KV4_MAX_GROUP + hq) * OROW;
-      const bool block = !PAIRED || (grp >= 2) == second;  // its positions' words
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t w = PAIRED ? 4 * (grp & 1) + r : 4 * grp + r;  // word (w / NG, w % NG)
-        if (block && (NG == 4 || w < 4 * NG)) {
-          float4 *to = (float4 *)(row + 32 * (w % NG) + 8 * (w / NG));
-          to[0] = make_float4(o[0][r] * f, o[4][r] * f, o[1][r] * f, o[5][r] * f);
-          to[1] = make_float4(o[2][r] * f, o[6][r] * f, o[3][r] * f, o[7][r] * f);
-        }
-      }
-      if (wave == 0 && lane < KV4_MAX_GROUP) {
-        float L = 0.f;
-#pragma unroll
-        for (int w = 0; w < AMMON_WAVES; ++w)
-          L += stats(w)[KV4_MAX_GROUP + hq] * __builtin_amdgcn_exp2f(stats(w)[hq] - M);
-        total_ml[hq] = M;
-        total_ml[KV4_MAX_GROUP + hq] = L;
-      }
-    }
-    __syncthreads();
     // a query row to a wave, two dimensions to a lane
     const uint32_t d = 2 * lane;
     for (uint32_t j = wave; j < cols; j += AMMON_WAVES) {
@@ -513,14 +493,20 @@ struct Kv4Partial {
           continue;
         }
       }
-      float a = 0.f, b = 0.f;
-      if (d < head) {
+      // the waves' rows to their largest maximum, which is finite: the token sees the first
+      // position, wave 0's
+      float M = stats(0)[j];
 #pragma unroll
-        for (uint32_t w = 0; w < MROWS; ++w) {
-          const float2 x = *(const float2 *)((const float *)lds + (w * KV4_MAX_GROUP + j) * OROW + d);
-          a += x.x;
-          b += x.y;
-        }
+      for (int w = 1; w < AMMON_WAVES; ++w) M = fmaxf(M, stats(w)[j]);
+      float a = 0.f, b = 0.f, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < AMMON_WAVES; ++w) {
+        const float f = __builtin_amdgcn_exp2f(stats(w)[j] - M);
+        L += stats(w)[KV4_MAX_GROUP + j] * f;
+        const float *row = rows_of(w) + j * OROW + (d < head ? d : 0);
+        const float2 x = *(const float2 *)row, y = *(const float2 *)(row + KV4_MAX_GROUP * OROW);
+        a += (x.x + y.x) * f;
+        b += (x.y + y.y) * f;
       }
       if (TOKENS && fewest < n) {
         uint32_t x = ~0u;
@@ -528,7 +514,6 @@ struct Kv4Partial {
           x = min(x, ((const uint32_t *)stats(w))[4 * KV4_MAX_GROUP + min(d / 32, NG - 1u)]);
         if (x <= pos + tok - t0) a = b = __uint_as_float(0x7fc00000u);
       }
-      const float M = total_ml[j], L = total_ml[KV4_MAX_GROUP + j];
       const size_t row = (size_t)tok * p.q_heads + g * G + hh;
       const bool direct = direct_out(p);
       float *to = direct ? p.out + row * head : p.partial + (row * p.splits + split) * (head + 2);
