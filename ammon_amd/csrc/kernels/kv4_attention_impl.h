@@ -247,8 +247,8 @@ struct Kv4Partial {
         qb[j][e] = second ? lo[0] : hi[0];
         qb[j][e + 1] = second ? lo[1] : hi[1];
       }
-    // log2(e) / sqrt(head), and q's scale back
-    const float scale2 = ldexpf(1.4426950408889634f / sqrtf((float)head), qe - 14);
+    // log2(e) / sqrt(head), and q's scale back (not 0: a masked score is -inf times this)
+    const float scale2 = fmaxf(ldexpf(1.4426950408889634f / sqrtf((float)head), qe - 14), 0x1p-126f);
 
     uint32_t word = 0, sb = 0;
     if constexpr (APPEND) {
