@@ -280,6 +280,7 @@ struct Kv4Partial {
 #pragma unroll
     for (int x = 0; x < 8; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // m: the reference maximum; l: this lane's positions
+    bool far = false;              // uniform: an m past KV4_FAR
     uint32_t bad = ~0u;            // first noted position of this lane's group of 32 numbers
 
     const uint32_t nch = (n + CROWS - 1) / CROWS;
@@ -343,20 +344,28 @@ struct Kv4Partial {
                        fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
       mc = fmaxf(mc, other_half(mc));
       mc = pair32_max(pair16_max(mc)) * scale2;
-      if (__any(mc > m + KV4_SLACK)) {
+      if (__any(mc - m > KV4_SLACK)) {
         const float mn = fmaxf(m, mc);
         const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
         for (int x = 0; x < 8; ++x) o[x] *= f;
         l *= f;
         m = mn;
+        far = __any(fabsf(m == -INFINITY ? 0.f : m) > KV4_FAR);
       }
       // (a wave with no position yet has m = -inf, and weights 0)
-      const float mu = KV4_BITS - (m == -INFINITY ? 0.f : m);
+      const float mz = m == -INFINITY ? 0.f : m;
+      float mu = KV4_BITS - mz, by = scale2;
+      if (far) {  // (scores become distances)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e] = kv4_distance(sc[e], scale2, mz);
+        mu = KV4_BITS;
+        by = 1.f;
+      }
       f16x8 ph, pl;
       float pw[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], scale2, mu));
+      for (int e = 0; e < 8; ++e) pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], by, mu));
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         f16x2 hi, lo;

@@ -328,6 +328,7 @@ struct Kv4PrefillTile {
 #pragma unroll
     for (int db = 0; db < NG; ++db) o[db] = zero16();
     float m = -INFINITY, l = 0.f;  // l: this lane's positions only, summed at the end
+    bool far = false;              // uniform: a row's m past KV4_FAR
     uint32_t nan = 0;              // value groups of which the row sees one
     const uint32_t lim = min(qpos, t1 - 1);  // last position of this lane's row
     f32x16 s[2];
@@ -349,7 +350,7 @@ struct Kv4PrefillTile {
       load(c + 2);
       __builtin_amdgcn_sched_barrier(0);
       if (c < mine) {
-        softmax(lds, c, lim, minus1, s, ph, pl, o, m, l, nan);
+        softmax(lds, c, lim, minus1, s, ph, pl, o, m, l, far, nan);
 #pragma unroll
         for (int kk = 0; kk < 1; ++kk) read_v(lds, c, 0, kk, a);
       }
@@ -369,7 +370,7 @@ struct Kv4PrefillTile {
   // Scores s of chunk c to the parts of its weights.
   AMMON_DEV void softmax(const char *lds, uint32_t c, uint32_t lim, float minus1, f32x16 (&s)[2],
                          f16x8 (&ph)[4], f16x8 (&pl)[4], f32x16 (&o)[NG], float &m, float &l,
-                         uint32_t &nan) const {
+                         bool &far, uint32_t &nan) const {
     const uint32_t first = t0 + c * CH;
     const uint32_t *notes = (const uint32_t *)(lds + NOTES) + (c & 1) * CH + lane;
     const uint32_t kn = notes[0], vn = notes[2 * CH];
@@ -402,21 +403,31 @@ struct Kv4PrefillTile {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mc = fmaxf(mc, s[b][i]);
     mc = pair32_max(mc) * scale2;
-    if (__any(mc > m + PF_SLACK)) {
+    if (__any(mc - m > PF_SLACK)) {
       const float mn = fmaxf(m, mc);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
       for (int db = 0; db < NG; ++db) o[db] *= f;
       l *= f;
       m = mn;
+      far = __any(fabsf(m == -INFINITY ? 0.f : m) > KV4_FAR);
     }
     // (a row with no position yet keeps (m, l, o) = (-inf, 0, 0))
-    const float mu = (m == -INFINITY ? 0.f : m) - KV4_PF_BITS;
+    const float mz = m == -INFINITY ? 0.f : m;
+    float mu = mz - KV4_PF_BITS, by = scale2;
+    if (far) {  // (scores become distances)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = kv4_distance(s[b][i], scale2, mz);
+      mu = -KV4_PF_BITS;
+      by = 1.f;
+    }
     float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], scale2, -mu));
+      for (int i = 0; i < 16; ++i) s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], by, -mu));
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll

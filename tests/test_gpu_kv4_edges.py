@@ -6,7 +6,7 @@ import pytest
 
 import oracle
 from oracle import kv4
-from test_gpu_kv4 import TOL, Cache, decode, off, prefill, rows_of
+from test_gpu_kv4 import TOL, Cache, decode, off, prefill, rows_of, up
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +38,60 @@ def test_tiny_q_with_masked_positions(rt, heads, kv_heads, head, scale):
 def test_tiny_q_of_a_prompt(rt, start, tokens, scale):
     c = Cache(rt, 2, 2600, 128, filled=start + tokens)
     q = (oracle.normal(tokens * 1024, 9).reshape(tokens, 8, 128) * np.float32(scale)).astype(np.float32)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
+    for split in (64, 1024):
+        assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+# ---- scores too large for fp32 to hold their distance to a maximum exactly ------------------------
+def huge(rt, heads, kv_heads, head, seq, tokens, start, size):
+    """A cache of rows near the format's limit, and q: of each row of scores the largest is so far
+    above the rest that its weight is 1 (the others' distances are above 100, while a score's error is
+    at most 2^-21 of |q| |k| / sqrt(head), a tenth of them or less)."""
+    c = Cache(rt, kv_heads, seq, head)
+    rows = [rows_of(kv_heads, start + tokens, head, s) for s in (1, 11)]
+    rows[0] *= np.float32(4000)
+    c.pack(0, *rows)
+    c.dev = [up(rt, h) for h in c.host]
+    q = (oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head) * np.float32(size)).astype(np.float32)
+    k, _ = c.numbers(start + tokens)
+    for t in range(tokens):
+        for h in range(heads):
+            x = k[h // (heads // kv_heads), :start + t + 1]
+            qh = q[t, h].astype(np.float64)
+            s = np.sort(x @ qh) / np.sqrt(head)
+            err = 2.0**-21 * np.linalg.norm(qh) * np.max(np.linalg.norm(x, axis=1)) / np.sqrt(head)
+            if len(s) > 1 and s[-1] - s[-2] < max(100, 10 * err):
+                q[t, h] = 0  # (rows of no clear winner are left out)
+    assert (q != 0).any(-1).mean() > 0.7
+    return c, q
+
+
+SIZES = [30.0, 3e3, 1e4, 1e6, 1e9, 1e20]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("heads,kv_heads,head", [(8, 2, 128), (6, 2, 96), (4, 4, 48), (8, 1, 20)])
+def test_scores_of_any_size(rt, heads, kv_heads, head, size):
+    for pos in (63, 200, 299):
+        c, q = huge(rt, heads, kv_heads, head, 300, 1, pos, size)
+        want = kv4.attention(q, *c.numbers(pos + 1), pos)[0]
+        for split in (300, 128, 16):
+            assert off(decode(rt, q[0], c, pos, split), want) <= TOL, (pos, split)
+        rows = [x[:, pos].astype(np.float32)[None] for x in c.numbers(pos + 1)]
+        b = Cache(rt, kv_heads, 300, head)
+        for h, x in zip(b.host, c.host):
+            h[:] = x
+        b.pack(pos, *rows)  # (stored numbers stored again)
+        b.dev = [up(rt, h) for h in b.host]
+        want = kv4.attention(q, *b.numbers(pos + 1), pos)[0]
+        assert off(decode(rt, q[0], b, pos, 128, new=rows), want) <= TOL, pos
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("start,tokens", [(0, 6), (40, 9), (250, 13), (2000, 300)])  # units, and tiles
+def test_scores_of_any_size_of_a_prompt(rt, start, tokens, size):
+    c, q = huge(rt, 8, 2, 128, 2600, tokens, start, size)
     want = kv4.attention(q, *c.numbers(start + tokens), start)
     for split in (64, 1024):
         assert off(prefill(rt, q, c, start, split), want) <= TOL
