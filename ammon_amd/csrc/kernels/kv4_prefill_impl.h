@@ -34,7 +34,8 @@
 // bf16 cache 103), 300 after 3000 50 (67), 2048 tokens 98 (95: its tiles are balanced
 // better): 350 TFLOP/s of products once each.
 //
-// Numbers that are not finite.  A stored group is finite or NaN (all of it).  NaN times
+// Numbers that are not finite.  A stored group is finite or NaN (all of it); one with a
+// scale or a bias that is not finite, however it came there, is taken as NaN.  NaN times
 // the weight 0 of a masked position would reach the rows before it, so NaN groups are
 // expanded as zeros and noted per position: a key's (any group) makes the scores of the
 // rows that see the position NaN, a value's makes the group's outputs of those rows NaN.
@@ -114,11 +115,12 @@ struct Kv4PrefillTile {
     f16x2 any = __builtin_bit_cast(f16x2, cp[0]);
 #pragma unroll
     for (int j = 1; j < NG; ++j) any += __builtin_bit_cast(f16x2, cp[j]);
-    // (the sum of the scales is finite unless one is not)
-    if (__any(any[0] - any[0] != (_Float16)0)) {
+    // (a sum of scales or of biases that is not finite: one is not, or they are large)
+    any *= (_Float16)0;
+    if (__any(any[0] + any[1] != (_Float16)0)) {
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const bool bad = (cp[j] & 0x7c00u) == 0x7c00u;
+        const bool bad = (cp[j] & 0x7c00u) == 0x7c00u || (cp[j] & 0x7c000000u) == 0x7c000000u;
         found |= bad ? 1u << j : 0u;
         cp[j] = bad ? 0u : cp[j];
       }

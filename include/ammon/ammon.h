@@ -247,7 +247,8 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
  * codes as 32-bit words [kv_heads, seq, 4, ceil(head / 32)], word (p, j) with
  * numbers 32 j + 8 p .. + 7, number + e in bits 4 n .. 4 n + 3, n = e / 2 for
  * even e and 4 + e / 2 for odd e; then words s | b << 16 [kv_heads, seq,
- * ceil(head / 32)].
+ * ceil(head / 32)].  A group of which s or b is NaN is NaN.  Words written by
+ * other means are such groups, or stand for finite numbers.
  *
  * ammon_rope_store and ammon_cache_store write rows of such a cache, the
  * attention entries read it (8 query rows' width is always computed: a group of

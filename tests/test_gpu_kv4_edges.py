@@ -95,3 +95,26 @@ def test_scores_of_any_size_of_a_prompt(rt, start, tokens, size):
     want = kv4.attention(q, *c.numbers(start + tokens), start)
     for split in (64, 1024):
         assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+# ---- groups with one word of scale and bias that is not finite ------------------------------------
+@pytest.mark.parametrize("word", [0x7e000000, 0x00007e00, 0xfe00fe00])  # bias, scale, both (NaN)
+@pytest.mark.parametrize("start,tokens", [(250, 13), (700, 400)])  # units, tiles
+def test_half_of_a_group_not_finite(rt, start, tokens, word):
+    """A later token's NaN does not reach an earlier one, whichever of the two it is in."""
+    heads, kv_heads, head = 8, 4, 128
+    last = start + tokens - 1
+    for side in (0, 1):
+        c = Cache(rt, kv_heads, 1200, head, filled=start + tokens)
+        sb = kv4.views(c.host[side], kv_heads, 1200, head)[1]
+        keep = 0xffff if word == 0x7e000000 else 0xffff0000 if word == 0x7e00 else 0
+        for g, at, j in ((0, last, 1), (1, start + tokens // 2, 3), (2, start, 0)):
+            sb[g, at, j] = (int(sb[g, at, j]) & keep) | word
+        c.dev[side].upload(c.host[side])
+        q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+        want = kv4.attention(q, *c.numbers(start + tokens), start)
+        nan = np.isnan(want).any(-1)
+        assert nan[-1, :6].all() and not nan[:-1, :2].any() and not nan[:tokens // 2, 2:4].any()
+        assert nan[:, 4:6].all() and not nan[:, 6:].any()
+        for split in (64, 1024):
+            assert off(prefill(rt, q, c, start, split), want) <= TOL
