@@ -374,7 +374,8 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
 // Measured at 32 q / 8 kv heads of 128 (units, tiles, us): 200 tokens 20.8, 18.7; 64 after
 // 500: 12.7, 32; 64 after 4000: 38, 51; 64 after 8000: 66, 53; 130 after 4000: 72, 48; heads
 // of 64: 64 after 4000: 25, 36; 64 after 8000: 39, 37.  Tiles of 300 tokens after 3000: 50;
-// of 2048: 98 in one split, 101 in two.
+// of 2048: 98 in one split, 101 in two.  After 140000: 16 tokens 304, 248; 64: 974, 360; 512:
+// 7600, 2190.
 PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
                              uint32_t head, uint32_t ctx, uint32_t scratch_splits, bool aligned) {
   PrefillPlan plan;
@@ -390,9 +391,11 @@ PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_head
   if (10e3 + chunk_ns >= unit_ns) return plan;  // (the shortest tiles: a small call asks no further)
   const double cus = std::max(rt->info.compute_units, 1);
   double best = unit_ns;
-  for (uint32_t n = 1; n <= std::min<uint32_t>(scratch_splits, 64); ++n) {
+  // at most 64 splits, or past 64 of the longest twice as many as those need
+  const uint32_t fewest = cdiv(ctx, kPrefillMaxSplit);
+  const uint32_t most = std::min(scratch_splits, fewest > 64 ? 2 * fewest : 64);
+  for (uint32_t n = fewest; n <= most; ++n) {
     const uint32_t len = cdiv(cdiv(ctx, n), 64) * 64;
-    if (len > kPrefillMaxSplit) continue;
     if (n > 1 && len < 256) break;
     const uint32_t splits = cdiv(ctx, len);
     const double units = (double)tiles * kv_heads * splits;

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import oracle
+from ammon_amd._abi import F32, KV4, call, lib
 from oracle import kv4
 from test_gpu_kv4 import TOL, Cache, decode, off, prefill, rows_of, up
 
@@ -118,3 +119,33 @@ def test_half_of_a_group_not_finite(rt, start, tokens, word):
         assert nan[:, 4:6].all() and not nan[:, 6:].any()
         for split in (64, 1024):
             assert off(prefill(rt, q, c, start, split), want) <= TOL
+
+
+# ---- which kernel a prompt gets -------------------------------------------------------------------
+def prefill_scratch(rt, q, c, start, split, shift=0):
+    """The result, and how much of the scratch was written: units write a part of every row for every
+    `split` positions, tiles of ranges as long as they choose."""
+    tokens, heads = q.shape[:2]
+    ctx = start + tokens
+    n = int(lib.ammon_attention_prefill_scratch_bytes(tokens, heads, c.head, ctx, split))
+    part, out = rt.alloc(n + 4), rt.alloc(q.nbytes + 4)
+    for buf, count in ((part, n // 4 + 1), (out, q.size + 1)):
+        rt.fill(buf, F32, count, 7.0)
+    dq = up(rt, np.concatenate([np.zeros(1, np.float32), q.ravel()]) if shift else q)
+    call("ammon_attention_prefill", rt.handle, None, dq.offset(4 * shift), tokens, heads, *c.dev, KV4,
+         c.kv_heads, c.head, c.seq, rt.step(0, start), ctx, split, part.offset(4 * shift), n,
+         out.offset(4 * shift))
+    got, used = out.download(q.size + 1), part.download(n // 4 + 1)
+    assert got[0 if shift else -1] == 7.0 and used[0 if shift else -1] == 7.0
+    return got[shift:shift + q.size].reshape(q.shape), np.mean(used != 7.0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head,start,tokens", [(2, 1, 64, 131072, 200), (4, 1, 128, 131000, 73),
+                                                              (2, 2, 40, 130950, 300), (1, 1, 32, 290001, 333)])
+def test_tiles_past_131072_positions(rt, heads, kv_heads, head, start, tokens):
+    c = Cache(rt, kv_heads, start + tokens + 3, head, filled=start + tokens)
+    q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
+    got, used = prefill_scratch(rt, q, c, start, 256)
+    assert off(got, want) <= TOL
+    assert used < 0.6  # units write nearly all of it
