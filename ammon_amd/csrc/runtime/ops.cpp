@@ -362,7 +362,7 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
 }
 
 // The same for a KV4 cache (kv4_prefill_impl.h): tiles of 256 rows, one workgroup per
-// CU.  The number of splits is the one with the least estimated time, of
+// CU, of q and out at any float.  The number of splits is the one with the least estimated time, of
 //   chunks  the longest workgroup's, or what each CU gets of all of them (with causal
 //           masking a tile sees half of its prompt: splits even that out),
 //   ends    a workgroup's first and last steps; workgroups of a second round have theirs
@@ -377,11 +377,11 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
 // of 2048: 98 in one split, 101 in two.  After 140000: 16 tokens 304, 248; 64: 974, 360; 512:
 // 7600, 2190.
 PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
-                             uint32_t head, uint32_t ctx, uint32_t scratch_splits, bool aligned) {
+                             uint32_t head, uint32_t ctx, uint32_t scratch_splits) {
   PrefillPlan plan;
   const uint32_t g = q_heads / kv_heads, ng = cdiv(head, 32);
   const uint64_t rows = (uint64_t)tokens * g, tiles = cdiv(rows, 256);
-  if (!aligned || rows >= (1ull << 31)) return plan;
+  if (rows >= (1ull << 31)) return plan;
   const double chunk_ns = 500 + 560 * ng;
   const double seen = ctx - tokens / 2.0;  // positions a token sees, on average
   const double unit_ns =
@@ -963,7 +963,7 @@ ammon_status ammon_attention_prefill(ammon_runtime *rt, ammon_stream stream, con
   const bool aligned = (bits & 15u) == 0 && ((uintptr_t)partial & 7u) == 0;
   const PrefillPlan plan =
       kv_dtype == AMMON_KV4
-          ? kv4_prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, aligned)
+          ? kv4_prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits)
           : prefill_plan(rt, tokens, q_heads, kv_heads, head, ctx, splits, kv_dtype, aligned);
   if (plan.f) {
     p.split_len = plan.split_len;

@@ -149,3 +149,17 @@ def test_tiles_past_131072_positions(rt, heads, kv_heads, head, start, tokens):
     got, used = prefill_scratch(rt, q, c, start, 256)
     assert off(got, want) <= TOL
     assert used < 0.6  # units write nearly all of it
+
+
+@pytest.mark.parametrize("heads,kv_heads,head", [(32, 8, 128), (18, 6, 96), (8, 8, 64), (6, 6, 33)])
+@pytest.mark.parametrize("start,tokens", [(0, 700), (1500, 500)])
+def test_tiles_of_rows_at_any_float(rt, heads, kv_heads, head, start, tokens):
+    """q, the scratch and the output a float past 16 bytes: the same kernel, the same numbers."""
+    c = Cache(rt, kv_heads, 2100, head, filled=start + tokens)
+    q = oracle.normal(tokens * heads * head, 9).reshape(tokens, heads, head)
+    want = kv4.attention(q, *c.numbers(start + tokens), start)
+    got, used = prefill_scratch(rt, q, c, start, 64)
+    shifted, used_shifted = prefill_scratch(rt, q, c, start, 64, shift=1)
+    assert off(got, want) <= TOL
+    np.testing.assert_array_equal(got, shifted)
+    assert abs(used - used_shifted) < 1e-6 and used < 0.6
