@@ -399,7 +399,7 @@ PrefillPlan kv4_prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_head
     if (n > 1 && len < 256) break;
     const uint32_t splits = cdiv(ctx, len);
     const double units = (double)tiles * kv_heads * splits;
-    if (units >= (1u << 30)) break;
+    if (units + 8 >= (1ull << 32) / (2 * kWorkgroup)) break;  // (a launch's work items)
     const double longest = cdiv(std::min(len, ctx), 64);
     const double all = (double)tiles * kv_heads * (seen / 64 + 0.5 * splits) / cus;
     // (a second round of workgroups starts where the first's end, from its beginning)
@@ -496,6 +496,10 @@ ammon_status ammon_rmsnorm(ammon_runtime *rt, ammon_stream stream, const float *
 }  // extern "C"
 
 namespace {
+// A launch has fewer than 2^32 work items in a dimension; a row takes 16 of them (in a
+// load, AMMON_KV4_LOAD_ROWS rows do).
+constexpr uint64_t kKv4StoreRows = ((1ull << 32) / kWorkgroup - 1) * (kWorkgroup / 16);
+
 // What every call on KV4 caches asks of them (v NULL: of one).
 ammon_status kv4_check(const char *what, uint32_t kv_heads, uint32_t head, uint32_t seq, const void *k,
                        const void *v) {
@@ -517,7 +521,7 @@ ammon_status kv4_store(ammon_runtime *rt, ammon_stream stream, const float *k, c
                        const char *what) {
   ammon_status st = kv4_check(what, kv_heads, head, seq, k_cache, v_cache);
   if (st != AMMON_OK) return st;
-  AMMON_CHECK((uint64_t)tokens * kv_heads < (1ull << 31), "%s: too many rows", what);
+  AMMON_CHECK((uint64_t)tokens * kv_heads <= kKv4StoreRows, "%s: too many rows", what);
   const size_t rows = (size_t)tokens * kv_heads * head * 4;
   const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
   for (const float *src : {k, v})
@@ -566,7 +570,8 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
               first, count, seq);
   AMMON_CHECK((((uintptr_t)k_out | (uintptr_t)v_out) & 15u) == 0,
               "kv4_load: outputs must be 16-byte aligned");
-  AMMON_CHECK((uint64_t)count * kv_heads < (1ull << 32) - 1024, "kv4_load: too many rows");
+  AMMON_CHECK((uint64_t)count * kv_heads <= kKv4StoreRows * AMMON_KV4_LOAD_ROWS,
+              "kv4_load: too many rows");
   const size_t rows = (size_t)count * kv_heads * head * dsize(out_dtype);
   const size_t bytes = ammon_kv_cache_bytes(AMMON_KV4, kv_heads, seq, head);
   for (const void *out : {k_out, v_out})

@@ -257,14 +257,15 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
  * the rows, ammon_attention_decode_append and ammon_kv4_store take them. */
 
 /* Rows k, v [tokens, kv_heads, head] into the caches at positions
- * step->position + t; a position at or past seq is left out. */
+ * step->position + t; a position at or past seq is left out.  At most 2^28 - 16
+ * rows (tokens * kv_heads) a call. */
 ammon_status ammon_kv4_store(ammon_runtime *rt, ammon_stream stream, const float *k,
                              const float *v, uint32_t tokens, uint32_t kv_heads, uint32_t head,
                              void *k_cache, void *v_cache, uint32_t seq,
                              const ammon_decode_step *step);
 /* The numbers of positions [first, first + count), first + count <= seq, as
  * [kv_heads, count, head] fp32 or bf16 (16-byte aligned).  v_cache and v_out
- * may both be NULL. */
+ * may both be NULL.  At most 2^30 - 64 rows (count * kv_heads) a call. */
 ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *k_cache,
                             const void *v_cache, uint32_t kv_heads, uint32_t head, uint32_t seq,
                             uint32_t first, uint32_t count, void *k_out, void *v_out,

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 import oracle
-from ammon_amd._abi import F32, KV4, call, lib
+from ammon_amd import _abi
+from ammon_amd._abi import F32, KV4, AmmonError, call, lib
 from oracle import kv4
 from test_gpu_kv4 import TOL, Cache, decode, off, prefill, rows_of, up
 
@@ -163,3 +164,23 @@ def test_tiles_of_rows_at_any_float(rt, heads, kv_heads, head, start, tokens):
     assert off(got, want) <= TOL
     np.testing.assert_array_equal(got, shifted)
     assert abs(used - used_shifted) < 1e-6 and used < 0.6
+
+
+# ---- more rows than a launch takes (nothing is launched) --------------------------------------------
+@pytest.mark.parametrize("rows,kv_heads,fits", [((1 << 28) - 16, 1, True), ((1 << 28) - 15, 1, False),
+                                               ((1 << 25) - 2, 8, True), ((1 << 25) - 1, 8, False),
+                                               (0xffffffff, 1, False)])
+def test_rows_of_one_launch(rt, rows, kv_heads, fits):
+    """16 lanes a row (of a load four rows), fewer than 2^32 lanes."""
+    V, step = _abi.STREAM_VALIDATE, rt.step(0, 0)
+    at = [1 << n for n in (50, 51, 52, 53)]  # (nothing is read or written)
+    store = ("ammon_kv4_store", rt.handle, V, at[0], at[1], rows, kv_heads, 1, at[2], at[3], 100, step)
+    load = ("ammon_kv4_load", rt.handle, V, at[2], at[3], kv_heads, 1, 0xffffffff, 0, min(4 * rows, 0xffffffff),
+            at[0], at[1], F32)
+    for c in (store, load):
+        if fits:
+            call(*c)
+            continue
+        with pytest.raises(AmmonError, match="too many rows") as e:
+            call(*c)
+        assert e.value.status == _abi.E_VALIDATION
