@@ -5,8 +5,9 @@
 #include "kv4_prefill_impl.h"
 
 // Rows [tokens, kv_heads, head] (fp32) into the cache at position step->position + t:
-// 16 lanes a row, 16 rows a workgroup, blockIdx.y 0 the keys, 1 the values.  Bytes
-// bound it: 4 head read and 20 NG written per row.
+// 16 lanes a row, 16 rows a workgroup, blockIdx.y 0 the keys, 1 the values.  One row in
+// flight per 16 lanes bounds it: 2048 rows of 8 heads of 128 (19 MB, 4 head bytes read and
+// 20 NG written per row) take 7.6 us traced, the load of as many bytes 5.1.
 extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_kv4_store(ammon_k_kv4 p) {
   const uint32_t r = blockIdx.x * (AMMON_WG / 16) + threadIdx.x / 16, i = threadIdx.x & 15;
   if (r >= p.tokens * p.kv_heads) return;  // (a row's 16 lanes go together)

@@ -13,7 +13,7 @@
 //     c = clamp(rint((x - b) (1 / s) - 16), 0, 15), 0 where s = 0
 // (|b| <= 16384 + 32 x 16384 / 15 is a finite fp16).  A group with a number that is
 // not finite has s = b = NaN and so reads back as NaN.  What is lost: half a step of
-// (max - min) / 15 per number, and 2^-11 of its size in fp16.
+// (max - min) / 15 per number, and 2^-11 each of the bias's and the number's size.
 //
 // Memory of one cache, NG = ceil(head / 32): the codes as 32-bit words [kv_heads,
 // seq, 4, NG] -- word (p, j) has numbers 32 j + 8 p .. + 7 of the row, number + e in

@@ -28,11 +28,15 @@
 //
 // So K c and V c each need two buffers (c's parity).
 //
-// What bounds it: a turn is 2700 cycles, of which the matrix unit is busy 2050 and the
-// issue of vector instructions (386 of both waves, and some 12 cycles for every matrix
-// instruction) 2300.  Measured, 32 q / 8 kv heads of 128: 301 tokens after 7001 81 us (a
-// bf16 cache 103), 300 after 3000 50 (67), 2048 tokens 98 (95: its tiles are balanced
-// better): 350 TFLOP/s of products once each.
+// What bounds it: alone, a turn is 2700 cycles, of which the matrix unit is busy 2050 and
+// the issue of vector instructions (386 of both waves, and some 12 cycles for every matrix
+// instruction) 2300.  With every CU at it a turn takes 3600 cycles, starts and ends
+// included (301 tokens after 7001): the matrix unit is busy 58% of them, vector issue 54%.
+// At head 128 the kernel has all 256 registers and spills 14 (60 bytes of scratch a lane),
+// some of which come back in the chunk loop.  Measured, 32 q / 8 kv heads of 128: 301
+// tokens after 7001 81 us (a bf16 cache 103), 300 after 3000 50 (67), 2048 tokens 97 (95:
+// its tiles are balanced better; here a CU is busy 52% of the time): 354 TFLOP/s of
+// products once each.
 //
 // Numbers that are not finite.  A stored group is finite or NaN (all of it); one with a
 // scale or a bias that is not finite, however it came there, is taken as NaN.  NaN times

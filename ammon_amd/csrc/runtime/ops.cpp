@@ -362,7 +362,8 @@ PrefillPlan prefill_plan(ammon_runtime *rt, uint32_t tokens, uint32_t q_heads, u
 }
 
 // The same for a KV4 cache (kv4_prefill_impl.h): tiles of 256 rows, one workgroup per
-// CU, of q and out at any float.  The number of splits is the one with the least estimated time, of
+// CU, of q and out at any float.  The number of splits is the one with the least
+// estimated time, of
 //   chunks  the longest workgroup's, or what each CU gets of all of them (with causal
 //           masking a tile sees half of its prompt: splits even that out),
 //   ends    a workgroup's first and last steps; workgroups of a second round have theirs

@@ -241,7 +241,10 @@ ammon_status ammon_cache_store(ammon_runtime *rt, ammon_stream stream, const flo
  *   s = fp16((max x - min x) / 15),  b = fp16(min x - 16 s)
  *   c = clamp(rint((x - b) (1 / s) - 16), 0, 15), 0 where s = 0
  * A group with a number that is not finite reads back as NaN.  A stored number
- * is off by at most about half a step s, i.e. 1/30 of its group's range.
+ * within the limits is off by at most about half a step s, i.e. 1/30 of its
+ * group's range, and by the fp16 rounding of the bias and of the number itself
+ * (2^-11 of their size each, more than a step in a group of large numbers that
+ * differ little).
  *
  * Memory of one cache (20 ceil(head / 32) bytes a row, 16-byte aligned): the
  * codes as 32-bit words [kv_heads, seq, 4, ceil(head / 32)], word (p, j) with
