@@ -7,7 +7,7 @@ binding over that library for tests and benchmarks; importing it fails if
 the library has not been built.
 """
 from . import _abi
-from ._abi import (ATTENTION_MAX_HEAD, ATTENTION_SPLIT_REF, BF16, DEFAULT_ROPE_THETA, F32, KV4,
+from ._abi import (ATTENTION_MAX_HEAD, ATTENTION_SPLIT_REF, BF16, DEFAULT_ROPE_THETA, F32, KV4, Q8, Q24, W4,
                    AmmonError, DecodeStep)
 from .runtime import (DeviceBuffer, Runtime, Timer, argmax_scratch_bytes, attention_scratch_bytes,
                       attention_splits, kv_permute, kv_unpermute, rope_table_host, storage_dtype)
@@ -19,7 +19,7 @@ from .tokenizer import BpeTokenizer
 LIB_PATH = _abi.LIB_PATH
 
 __all__ = [
-    "ATTENTION_MAX_HEAD", "ATTENTION_SPLIT_REF", "BF16", "DEFAULT_ROPE_THETA", "F32", "KV4",
+    "ATTENTION_MAX_HEAD", "ATTENTION_SPLIT_REF", "BF16", "DEFAULT_ROPE_THETA", "F32", "KV4", "Q8", "Q24", "W4",
     "AmmonError", "DecodeStep", "DeviceBuffer", "Runtime", "Timer", "argmax_scratch_bytes",
     "attention_scratch_bytes", "attention_splits", "kv_permute", "kv_unpermute",
     "rope_table_host", "storage_dtype", "LIB_PATH", "LlamaModel", "model", "BpeTokenizer",

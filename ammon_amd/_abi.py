@@ -16,6 +16,8 @@ LIB_PATH = os.path.join(_HERE, "libammon_amd.so")
 OK, E_VALIDATION, E_HIP, E_OOM, E_NO_DEVICE = 0, 1, 2, 3, 4
 F32, BF16 = 0, 1
 KV4 = 4  # KV caches only
+W4 = 5  # weight matrices only
+Q8, Q24 = 6, 7  # rows of 8-bit digits: one a number, three a number
 COPY_H2D, COPY_D2H, COPY_D2D = 1, 2, 3
 STREAM_VALIDATE = ctypes.c_void_p(1)
 
@@ -91,6 +93,13 @@ SIGNATURES = {
     "ammon_cache_store": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT, _U32, _P]),
     "ammon_kv4_store": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _U32, _P]),
     "ammon_kv4_load": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _DT]),
+    "ammon_w4_bytes": (_SZ, [_U32, _U32]),
+    "ammon_w4_store": (_ST, [_P, _P, _P, _DT, _U32, _U32, _P]),
+    "ammon_w4_load": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT]),
+    "ammon_q8_bytes": (_SZ, [_DT, _U32, _U32]),
+    "ammon_q8_store": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT]),
+    "ammon_rmsnorm_q8": (_ST, [_P, _P, _P, _P, _P, _P, _DT, _F, _U32, _U32, _P, _DT]),
+    "ammon_q8_load": (_ST, [_P, _P, _P, _DT, _U32, _U32, _P]),
     "ammon_attention_partial": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _U32, _P,
                                       _U32, _P]),
     "ammon_attention_combine": (_ST, [_P, _P, _P, _U32, _U32, _U32, _P, _U32, _P]),
@@ -130,6 +139,12 @@ SIGNATURES = {
     "ammon_prefill_qkv_rope": (_ST, [_P, _P, _P, _U32, _P, _P, _P, _DT, _U32, _U32, _U32, _U32, _P,
                                      _P, _P, _U32, _P, _P, _P, _SZ]),
     "ammon_prefill_gate_up_swiglu": (_ST, [_P, _P, _P, _U32, _P, _P, _DT, _U32, _U32, _P]),
+    "ammon_prefill_gemm_w4": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT, _U32, _P, _P, _P, _SZ]),
+    "ammon_prefill_gate_up_swiglu_w4": (_ST, [_P, _P, _P, _DT, _U32, _P, _P, _U32, _U32, _P]),
+    "ammon_prefill_qkv_rope_w4": (_ST, [_P, _P, _P, _DT, _U32, _P, _P, _P, _U32, _U32, _U32, _U32,
+                                        _P, _P, _P, _U32, _P, _P, _P, _SZ]),
+    "ammon_prefill_qkv_rope_store_w4": (_ST, [_P, _P, _P, _DT, _U32, _P, _P, _P, _U32, _U32, _U32,
+                                              _U32, _P, _P, _P, _DT, _U32, _P, _P, _P, _SZ]),
     "ammon_attention_prefill_scratch_bytes": (_SZ, [_U32, _U32, _U32, _U32, _U32]),
     "ammon_attention_prefill": (_ST, [_P, _P, _P, _U32, _U32, _P, _P, _DT, _U32, _U32, _U32, _P,
                                       _U32, _U32, _P, _SZ, _P]),

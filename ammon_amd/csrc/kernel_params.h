@@ -19,6 +19,9 @@ extern "C" {
 #define AMMON_K_F32 0
 #define AMMON_K_BF16 1
 #define AMMON_K_KV4 4 /* KV caches only: kernels/kv4_impl.h */
+#define AMMON_K_W4 5  /* weights only: kernels/w4_impl.h */
+#define AMMON_K_Q8 6  /* rows of one 8-bit digit a number, and of three */
+#define AMMON_K_Q24 7
 #define AMMON_KV4_LOAD_ROWS 4 /* rows a lane of kv4_load takes */
 
 /* Device-resident control parcel: same layout as ammon_decode_step. */
@@ -110,6 +113,27 @@ typedef struct {
   uint32_t out_dtype, q_numel;
 } ammon_k_kv4;
 
+/* 4-bit weights stored and read back. */
+typedef struct {
+  const void *w;            /* store: [d, n] fp32 or bf16 */
+  void *w4;                 /* panels: kernels/w4_impl.h */
+  void *out;                /* load: [d, n] fp32 or bf16 */
+  uint32_t d, n, dtype;
+  uint32_t vec;             /* store: w's rows in 16-byte (bf16: 8-byte) pieces */
+} ammon_k_w4;
+
+/* Rows of digits made and read back. */
+typedef struct {
+  const float *x;           /* [tokens, n] */
+  const float *residual;    /* [tokens, n] or NULL */
+  float *sum;               /* x + residual, with one; load: the numbers [tokens, n] */
+  const void *w;            /* [n] RMSNorm weight or NULL (no norm) */
+  void *rows;               /* panels: kernels/w4_impl.h */
+  uint32_t tokens, n, w_dtype;
+  uint32_t w_vec, vec;      /* w; x, residual and sum: in 16-byte (bf16: 8-byte) pieces */
+  float eps;
+} ammon_k_q8;
+
 typedef struct {
   float *hb;                /* [n] in/out (swiglu) or out (add) */
   const float *a;           /* add: first operand */
@@ -155,7 +179,7 @@ typedef struct {
  * 16-row wave tile never straddles q/k/v (q_dim, kv_dim multiples of 16). */
 typedef struct {
   const void *w0, *w1, *w2; /* row-major [*, n] matrices */
-  const float *x;           /* [tokens, n] */
+  const float *x;           /* [tokens, n]; W4: rows of digits */
   const float *residual;    /* RESIDUAL: [tokens, d] (may equal y) */
   float *y;                 /* [tokens, d]; QKV: q [tokens, q_dim] */
   void *k_cache, *v_cache;  /* QKV: layer views [kv_heads, seq, head] */

@@ -81,6 +81,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef f32x4 f32x4a4 __attribute__((aligned(4)));  // a 16-byte access at a float's alignment
 
 // Buffer resource (V#) over [base, base + bytes): raw buffer loads at byte
 // offsets >= bytes return zero and touch no memory, which replaces

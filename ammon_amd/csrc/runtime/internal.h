@@ -23,6 +23,8 @@ constexpr int kAttGroups = 4;  // GMAX = 1, 2, 4, 8
 constexpr int kGemvModes = 4;
 // KV4 variants: ceil(head / 32).
 constexpr int kKv4Groups = 4;
+// W4 GEMM tiles: w4_prefill.hip's suffixes.
+constexpr int kW4Tiles = 2;
 // Bytes of a KV4 row per group of 32 numbers: 16 of codes, 4 of scale and bias.
 constexpr size_t kKv4RowBytes = 20;
 
@@ -69,6 +71,13 @@ struct Kernels {
   hipFunction_t kv4_load = nullptr;
   hipFunction_t kv4_partial[3][kKv4Groups] = {};  // [Kv4Mode]
   hipFunction_t kv4_prefill[kKv4Groups] = {};  // prefill tiles
+  // 4-bit weights and rows of digits: [Q8, Q24]
+  hipFunction_t w4_store = nullptr;
+  hipFunction_t w4_load = nullptr;
+  hipFunction_t q8_rows[2] = {};
+  hipFunction_t q8_load[2] = {};
+  hipFunction_t w4_gemv[kGemvModes + 1] = {};               // [mode], PLAIN_ARGMAX last
+  hipFunction_t w4_gemm[2][kW4Tiles][kGemvModes] = {};
 };
 
 // LDS per compute unit on gfx950 (bytes); bounds resident GEMV workgroups.

@@ -29,6 +29,9 @@ AMMON_BLOB(gemv)
 AMMON_BLOB(misc)
 AMMON_BLOB(prefill)
 AMMON_BLOB(kv4)
+AMMON_BLOB(w4)
+AMMON_BLOB(w4_gemv)
+AMMON_BLOB(w4_prefill)
 
 namespace ammon_rt {
 
@@ -81,7 +84,9 @@ static ammon_status load_kernels(ammon_runtime *rt) {
   } blobs[] = {{"embed", ammon_co_embed}, {"norm", ammon_co_norm},
                {"rope", ammon_co_rope},   {"attention", ammon_co_attention},
                {"gemv", ammon_co_gemv},   {"misc", ammon_co_misc},
-               {"prefill", ammon_co_prefill}, {"kv4", ammon_co_kv4}};
+               {"prefill", ammon_co_prefill}, {"kv4", ammon_co_kv4},
+               {"w4", ammon_co_w4},       {"w4_gemv", ammon_co_w4_gemv},
+               {"w4_prefill", ammon_co_w4_prefill}};
   constexpr int kModules = (int)(sizeof(blobs) / sizeof(blobs[0]));
   hipModule_t mods[kModules];
   for (int i = 0; i < kModules; ++i) {
@@ -193,6 +198,28 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_kv4_prefill_n%d", n + 1);
     R(7, name, k.kv4_prefill[n]);
   }
+  R(8, "ammon_w4_store", k.w4_store);
+  R(8, "ammon_w4_load", k.w4_load);
+  for (int q = 0; q < 2; ++q) {
+    char name[96];
+    snprintf(name, sizeof name, "ammon_q8_rows_%d", q ? 3 : 1);
+    R(8, name, k.q8_rows[q]);
+    snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
+    R(8, name, k.q8_load[q]);
+  }
+  for (int m = 0; m <= kGemvModes; ++m) {
+    char name[96];
+    snprintf(name, sizeof name, "ammon_w4_gemv_%s", m < kGemvModes ? modes[m] : "plain_argmax");
+    R(9, name, k.w4_gemv[m]);
+  }
+  const char *w4_tiles[kW4Tiles] = {"t16", "t64"};
+  for (int q = 0; q < 2; ++q)
+    for (int t = 0; t < kW4Tiles; ++t)
+      for (int m = 0; m < kGemvModes; ++m) {
+        char name[96];
+        snprintf(name, sizeof name, "ammon_w4_gemm_%s_q%d_%s", modes[m], q ? 3 : 1, w4_tiles[t]);
+        R(10, name, k.w4_gemm[q][t][m]);
+      }
 #undef R
   return AMMON_OK;
 }
@@ -519,6 +546,7 @@ size_t ammon_kv_cache_bytes(ammon_dtype kv_dtype, uint32_t kv_heads, uint32_t se
     case AMMON_F32: return rows * head * 4;
     case AMMON_BF16: return rows * head * 2;
     case AMMON_KV4: return rows * kKv4RowBytes * (((size_t)head + 31) / 32);
+    default: break;  // no cache's
   }
   return 0;
 }

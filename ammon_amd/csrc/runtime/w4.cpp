@@ -1,0 +1,429 @@
+// w4.cpp -- C-ABI entry points of the 4-bit weights (AMMON_W4) and the rows of 8-bit digits
+// (AMMON_Q8, AMMON_Q24): validate, pick the variant, launch.  No counterpart in the reference.
+#include <hip/hip_runtime_api.h>
+
+#include "ops_common.h"
+
+using namespace ammon_rt;
+
+namespace {
+
+// A launch has fewer than 2^32 work items in a dimension.
+constexpr uint64_t kMaxWorkgroups = (1ull << 32) / kWorkgroup - 1;
+
+bool valid_digits(ammon_dtype d) { return d == AMMON_Q8 || d == AMMON_Q24; }
+
+// 16-byte (bf16: 8-byte) pieces of rows of n.
+bool pieces(const void *base, ammon_dtype dt, uint32_t n) {
+  return n % 4 == 0 && ((uintptr_t)base & (dt == AMMON_BF16 ? 7u : 15u)) == 0;
+}
+
+ammon_status shape_check(const char *what, uint32_t rows, uint32_t n) {
+  AMMON_CHECK(rows > 0 && n > 0, "%s: empty shape (%u rows of %u)", what, rows, n);
+  AMMON_CHECK(cdiv(rows, 16) <= kMaxWorkgroups, "%s: %u rows are too many", what, rows);
+  AMMON_CHECK(n < (1u << 28), "%s: rows of %u numbers are too long", what, n);
+  return AMMON_OK;
+}
+
+ammon_status aligned(const char *what, const void *p, const char *name) {
+  AMMON_CHECK(((uintptr_t)p & 15u) == 0, "%s: %s must be 16-byte aligned", what, name);
+  return AMMON_OK;
+}
+
+#define TRY(expr)                         \
+  do {                                    \
+    const ammon_status st_ = (expr);      \
+    if (st_ != AMMON_OK) return st_;      \
+  } while (0)
+
+// Panels of 16 rows: queries, keys and values begin one each.
+ammon_status qkv_check(const char *what, uint64_t q_dim, uint64_t kv_dim) {
+  AMMON_CHECK(q_dim % 16 == 0 && kv_dim % 16 == 0,
+              "%s: W4 queries, keys and values must be a multiple of 16 rows each", what);
+  return AMMON_OK;
+}
+
+// ---- prompt products -------------------------------------------------------------------------
+struct W4GemmArgs {
+  int mode;
+  const void *w0, *w1, *w2;
+  uint32_t d, n, rows, tokens;
+  const void *x;
+  ammon_dtype x_dtype;
+  const float *residual;
+  float *y;
+  size_t y_bytes;
+  void *k_cache, *v_cache;
+  size_t kv_bytes;
+  const ammon_decode_step *step;
+  const float *table;
+  uint32_t kv_dim, head, seq;
+  ammon_dtype kv_dtype;
+  bool kv_rows;
+  void *ws;
+  size_t ws_bytes;
+};
+
+ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a, const char *what) {
+  AMMON_CHECK(a.w0 && a.x && a.y, "%s: NULL weight, x or y", what);
+  AMMON_CHECK(valid_digits(a.x_dtype), "%s: x is rows of digits (AMMON_Q8 or AMMON_Q24), not dtype %d",
+              what, (int)a.x_dtype);
+  TRY(shape_check(what, a.rows, a.n));
+  AMMON_CHECK(a.d > 0 && a.rows < (1u << 31), "%s: empty or too large (d=%u)", what, a.d);
+  TRY(shape_check(what, a.tokens, a.n));
+  const void *const ws[] = {a.w0, a.w1, a.w2};
+  const uint32_t wd[] = {a.d, a.mode == AMMON_GEMV_QKV ? a.kv_dim : a.d, a.kv_dim};
+  for (int i = 0; i < 3; ++i)
+    if (ws[i]) {
+      TRY(aligned(what, ws[i], "weights"));
+      AMMON_CHECK(!overlaps(ws[i], ammon_w4_bytes(wd[i], a.n), a.y, a.y_bytes), "%s: y overlaps weights", what);
+    }
+  TRY(aligned(what, a.x, "x"));
+  const size_t xbytes = ammon_q8_bytes(a.x_dtype, a.tokens, a.n);
+  AMMON_CHECK(!overlaps(a.x, xbytes, a.y, a.y_bytes), "%s: y overlaps x", what);
+  AMMON_CHECK(!a.residual || a.residual == a.y || !overlaps(a.residual, a.y_bytes, a.y, a.y_bytes),
+              "%s: residual partially overlaps y", what);
+  for (const void *to : {a.k_cache, a.v_cache})
+    AMMON_CHECK(!to || (!overlaps(to, a.kv_bytes, a.x, xbytes) && !overlaps(to, a.kv_bytes, a.y, a.y_bytes)),
+                "%s: k or v overlaps x or q", what);
+  if (a.ws) {
+    TRY(aligned(what, a.ws, "workspace"));
+    AMMON_CHECK(!overlaps(a.ws, a.ws_bytes, a.x, xbytes) && !overlaps(a.ws, a.ws_bytes, a.y, a.y_bytes) &&
+                    !(a.residual && overlaps(a.ws, a.ws_bytes, a.residual, a.y_bytes)) &&
+                    !(a.k_cache && overlaps(a.ws, a.ws_bytes, a.k_cache, a.kv_bytes)) &&
+                    !(a.v_cache && overlaps(a.ws, a.ws_bytes, a.v_cache, a.kv_bytes)),
+                "%s: workspace overlaps x, y, residual, k or v", what);
+  }
+  ammon_k_gemm p = {};
+  p.w0 = a.w0;
+  p.w1 = a.w1;
+  p.w2 = a.w2;
+  p.x = (const float *)a.x;
+  p.residual = a.residual;
+  p.y = a.y;
+  p.k_cache = a.k_cache;
+  p.v_cache = a.v_cache;
+  p.step = (const ammon_k_step *)a.step;
+  p.table = a.table;
+  p.d = a.d;
+  p.n = a.n;
+  p.rows = a.rows;
+  p.tokens = a.tokens;
+  p.kv_dim = a.kv_dim;
+  p.head = a.head;
+  p.seq = a.seq;
+  p.kv_dtype = (uint32_t)a.kv_dtype;
+  p.kv_rows = a.kv_rows;
+  const int tile = a.tokens > 16;
+  const uint32_t ct = tile ? 4 : 1, gated = a.mode == AMMON_GEMV_SWIGLU ? 2 : 1;
+  const uint32_t per = (tile ? 16 : 2) / gated;  // panels of results per workgroup
+  const uint64_t panels = cdiv(gated == 2 ? a.d : a.rows, 16);
+  const uint64_t grid = (uint64_t)cdiv(cdiv(panels, per), 8) * 8 * cdiv(a.tokens, 16 * ct);
+  AMMON_CHECK(grid <= kMaxWorkgroups, "%s: grid too large", what);
+  VALIDATE_ONLY();
+  return launch(rt, stream, rt->k.w4_gemm[a.x_dtype == AMMON_Q24][tile][a.mode], (uint32_t)grid, 1, 0, p,
+                what);
+}
+
+ammon_status w4_qkv(ammon_runtime *rt, ammon_stream stream, const void *x, ammon_dtype x_dtype,
+                    uint32_t tokens, const void *wq, const void *wk, const void *wv, uint32_t dim,
+                    uint32_t q_heads, uint32_t kv_heads, uint32_t head, float *q, void *k, void *v,
+                    ammon_dtype kv_dtype, bool rows, uint32_t seq, const ammon_decode_step *step,
+                    const float *table, void *workspace, size_t workspace_bytes, const char *what) {
+  AMMON_CHECK(wq && wk && wv, "%s: NULL wq, wk or wv", what);
+  AMMON_CHECK(k && v && step && table, "%s: NULL %s, step or table", what, rows ? "row buffer" : "cache");
+  AMMON_CHECK(kv_dtype != AMMON_KV4, "%s: a KV4 cache takes rows (prefill_qkv_rope_w4, then kv4_store)", what);
+  AMMON_CHECK(valid_dtype(kv_dtype), "%s: unknown kv dtype %d", what, (int)kv_dtype);
+  AMMON_CHECK(q_heads > 0 && kv_heads > 0 && seq > 0, "%s: empty shape", what);
+  AMMON_CHECK(head >= 2 && head % 2 == 0, "%s: head size %u must be even", what, head);
+  const uint64_t q_dim = (uint64_t)q_heads * head, kv_dim = (uint64_t)kv_heads * head;
+  TRY(qkv_check(what, q_dim, kv_dim));
+  AMMON_CHECK(kv_dim <= q_dim, "%s: kv width must be no wider than q", what);
+  AMMON_CHECK(q_dim + 2 * kv_dim < (1ull << 31), "%s: too many rows", what);
+  const size_t kv_bytes = (size_t)kv_dim * (rows ? tokens : seq) * dsize(kv_dtype);
+  AMMON_CHECK(!overlaps(k, kv_bytes, v, kv_bytes), "%s: key and value %s overlap", what,
+              rows ? "rows" : "caches");
+  AMMON_CHECK((((uintptr_t)k | (uintptr_t)v) & (kv_dtype == AMMON_BF16 ? 3u : 7u)) == 0,
+              "%s: k and v must be aligned to pairs of numbers", what);
+  W4GemmArgs a = {};
+  a.mode = AMMON_GEMV_QKV;
+  a.w0 = wq;
+  a.w1 = wk;
+  a.w2 = wv;
+  a.d = (uint32_t)q_dim;
+  a.n = dim;
+  a.rows = (uint32_t)(q_dim + 2 * kv_dim);
+  a.tokens = tokens;
+  a.x = x;
+  a.x_dtype = x_dtype;
+  a.y = q;
+  a.y_bytes = (size_t)tokens * q_dim * 4;
+  a.k_cache = k;
+  a.v_cache = v;
+  a.kv_bytes = kv_bytes;
+  a.step = step;
+  a.table = table;
+  a.kv_dim = (uint32_t)kv_dim;
+  a.head = head;
+  a.seq = seq;
+  a.kv_dtype = kv_dtype;
+  a.kv_rows = rows;
+  a.ws = workspace;
+  a.ws_bytes = workspace ? workspace_bytes : 0;
+  return w4_gemm(rt, stream, a, what);
+}
+
+// Rows x (+ residual, normalised with w) into digits.
+ammon_status q8_rows(ammon_runtime *rt, ammon_stream stream, const float *x, const float *residual,
+                     float *sum, const void *w, ammon_dtype w_dtype, float eps, uint32_t tokens, uint32_t n,
+                     void *out, ammon_dtype dtype, const char *what) {
+  AMMON_CHECK(x && out, "%s: NULL x or rows", what);
+  AMMON_CHECK(valid_digits(dtype), "%s: rows are AMMON_Q8 or AMMON_Q24, not dtype %d", what, (int)dtype);
+  TRY(shape_check(what, tokens, n));
+  AMMON_CHECK(tokens <= kMaxWorkgroups, "%s: %u tokens are too many", what, tokens);
+  TRY(aligned(what, out, "rows"));
+  const size_t bytes = (size_t)tokens * n * 4, to = ammon_q8_bytes(dtype, tokens, n);
+  AMMON_CHECK(!overlaps(x, bytes, out, to) && !(residual && overlaps(residual, bytes, out, to)) &&
+                  !(sum && overlaps(sum, bytes, out, to)),
+              "%s: rows overlap x, residual or sum", what);
+  if (residual)
+    for (const float *from : {x, residual})
+      AMMON_CHECK(sum == from || !overlaps(sum, bytes, from, bytes), "%s: sum partially overlaps x or residual",
+                  what);
+  if (w) {
+    const size_t wbytes = n * dsize(w_dtype);
+    AMMON_CHECK(!overlaps(w, wbytes, out, to) && !(sum && overlaps(w, wbytes, sum, bytes)),
+                "%s: weight overlaps rows or sum", what);
+  }
+  VALIDATE_ONLY();
+  ammon_k_q8 p = {};
+  p.x = x;
+  p.residual = residual;
+  p.sum = sum;
+  p.w = w;
+  p.rows = out;
+  p.tokens = tokens;
+  p.n = n;
+  p.w_dtype = (uint32_t)w_dtype;
+  p.w_vec = w && pieces(w, w_dtype, n);
+  p.vec = pieces(x, AMMON_F32, n) && (!residual || (pieces(residual, AMMON_F32, n) && pieces(sum, AMMON_F32, n)));
+  p.eps = eps;
+  return launch(rt, stream, rt->k.q8_rows[dtype == AMMON_Q24], tokens, 1, 0, p, what);
+}
+
+}  // namespace
+
+namespace ammon_rt {
+
+ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, const char *what,
+                     uint32_t *grid_out) {
+  AMMON_CHECK(a.w0 && a.x && a.y, "%s: NULL weight, x or y", what);
+  TRY(shape_check(what, a.rows, a.n));
+  AMMON_CHECK(a.d > 0, "%s: empty matrix (d=%u)", what, a.d);
+  AMMON_CHECK(a.mode != AMMON_GEMV_PLAIN || !a.step, "%s: takes no W4 weights", what);
+  AMMON_CHECK(!a.norm_w || valid_dtype(a.norm_dtype), "%s: unknown norm dtype", what);
+  AMMON_CHECK(!a.norm_w || (std::isfinite(a.eps) && a.eps >= 0.f), "%s: eps must be finite and >= 0", what);
+  for (const void *w : {a.w0, a.w1, a.w2})
+    if (w) TRY(aligned(what, w, "W4 weights"));
+  const size_t ybytes = (size_t)a.d * 4;
+  AMMON_CHECK(!overlaps(a.x, (size_t)a.n * 4, a.y, ybytes), "%s: y overlaps x", what);
+  AMMON_CHECK(!a.residual || !overlaps(a.x, (size_t)a.n * 4, a.residual, ybytes), "%s: residual overlaps x", what);
+  if (a.mode == AMMON_GEMV_QKV) TRY(qkv_check(what, a.d, a.kv_dim));
+  // x's digits and scales
+  const size_t lds = (size_t)cdiv(a.n, 128) * (3 * 128 + 16);
+  AMMON_CHECK(lds + 1024 <= (size_t)rt->info.max_shared_per_block,
+              "%s: reduction length n=%u needs %zu bytes of LDS; the device allows %d", what, a.n, lds + 1024,
+              rt->info.max_shared_per_block);
+  ammon_k_gemv p = {};
+  p.w0 = a.w0;
+  p.w1 = a.w1;
+  p.w2 = a.w2;
+  p.x = a.x;
+  p.norm_w = a.norm_w;
+  p.residual = a.residual;
+  p.y = a.y;
+  p.k_cache = a.k_cache;
+  p.v_cache = a.v_cache;
+  p.step = (const ammon_k_step *)a.step;
+  p.table = a.table;
+  p.d = a.d;
+  p.n = a.n;
+  p.rows = a.rows;
+  p.row_blocks = cdiv(a.rows, 16);
+  p.norm_dtype = (uint32_t)a.norm_dtype;
+  p.eps = a.eps;
+  p.kv_dim = a.kv_dim;
+  p.head = a.head;
+  p.seq = a.seq;
+  p.kv_dtype = (uint32_t)a.kv_dtype;
+  p.kv_rows = a.kv_rows;
+  p.cand_v = a.cand_v;
+  p.cand_i = a.cand_i;
+  hipFunction_t f = rt->k.w4_gemv[a.mode];
+  VALIDATE_ONLY();
+  const uint32_t cus = (uint32_t)std::max(rt->info.compute_units, 1);
+  DeviceGuard guard(rt->device);
+  uint32_t grid = std::min(p.row_blocks, cus * std::min(occupancy(rt, f, lds), 2u));
+  if (a.mode == AMMON_GEMV_PLAIN_ARGMAX) grid = std::min(grid, a.cand_cap);
+  if (grid_out) *grid_out = grid;
+  void *args[] = {&p, &grid};
+  const hipError_t e = hipModuleLaunchKernel(f, grid, 1, 1, kWorkgroup, 1, 1, (uint32_t)lds,
+                                             stream ? (hipStream_t)stream : rt->stream, args, nullptr);
+  if (e != hipSuccess) return hip_error(e, what);
+  return AMMON_OK;
+}
+
+}  // namespace ammon_rt
+
+extern "C" {
+
+size_t ammon_w4_bytes(uint32_t d, uint32_t n) { return (size_t)cdiv(d, 16) * cdiv(n, 128) * 1056; }
+
+ammon_status ammon_w4_store(ammon_runtime *rt, ammon_stream stream, const void *w, ammon_dtype w_dtype,
+                            uint32_t d, uint32_t n, void *out) {
+  REQUIRE_RT();
+  AMMON_CHECK(w && out, "w4_store: NULL matrix or output");
+  AMMON_CHECK(valid_dtype(w_dtype), "w4_store: unknown dtype %d", (int)w_dtype);
+  TRY(shape_check("w4_store", d, n));
+  TRY(aligned("w4_store", out, "W4 weights"));
+  AMMON_CHECK(!overlaps(w, (size_t)d * n * dsize(w_dtype), out, ammon_w4_bytes(d, n)),
+              "w4_store: the output overlaps the matrix");
+  VALIDATE_ONLY();
+  ammon_k_w4 p = {};
+  p.w = w;
+  p.w4 = out;
+  p.d = d;
+  p.n = n;
+  p.dtype = (uint32_t)w_dtype;
+  p.vec = pieces(w, w_dtype, n);
+  return launch(rt, stream, rt->k.w4_store, cdiv(d, 16), std::min(cdiv(n, 128), 65535u), 0, p, "w4_store");
+}
+
+ammon_status ammon_w4_load(ammon_runtime *rt, ammon_stream stream, const void *w4, uint32_t d, uint32_t n,
+                           void *out, ammon_dtype out_dtype) {
+  REQUIRE_RT();
+  AMMON_CHECK(w4 && out, "w4_load: NULL weights or output");
+  AMMON_CHECK(valid_dtype(out_dtype), "w4_load: unknown output dtype %d", (int)out_dtype);
+  TRY(shape_check("w4_load", d, n));
+  TRY(aligned("w4_load", w4, "W4 weights"));
+  AMMON_CHECK(!overlaps(out, (size_t)d * n * dsize(out_dtype), w4, ammon_w4_bytes(d, n)),
+              "w4_load: the output overlaps the weights");
+  VALIDATE_ONLY();
+  ammon_k_w4 p = {};
+  p.w4 = (void *)w4;
+  p.out = out;
+  p.d = d;
+  p.n = n;
+  p.dtype = (uint32_t)out_dtype;
+  return launch(rt, stream, rt->k.w4_load, cdiv(d, 16), std::min(cdiv(n, 128), 65535u), 0, p, "w4_load");
+}
+
+size_t ammon_q8_bytes(ammon_dtype dtype, uint32_t tokens, uint32_t n) {
+  if (!valid_digits(dtype)) return 0;
+  return (size_t)cdiv(tokens, 16) * cdiv(n, 128) * (2048 * (dtype == AMMON_Q8 ? 1 : 3) + 64);
+}
+
+ammon_status ammon_q8_store(ammon_runtime *rt, ammon_stream stream, const float *x, uint32_t tokens, uint32_t n,
+                            void *out, ammon_dtype dtype) {
+  REQUIRE_RT();
+  return q8_rows(rt, stream, x, nullptr, nullptr, nullptr, AMMON_F32, 0.f, tokens, n, out, dtype, "q8_store");
+}
+
+ammon_status ammon_rmsnorm_q8(ammon_runtime *rt, ammon_stream stream, const float *x, const float *residual,
+                              float *sum, const void *weight, ammon_dtype weight_dtype, float eps,
+                              uint32_t tokens, uint32_t n, void *out, ammon_dtype dtype) {
+  REQUIRE_RT();
+  AMMON_CHECK(weight != nullptr, "rmsnorm_q8: parameter `weight` is NULL");
+  AMMON_CHECK(valid_dtype(weight_dtype), "rmsnorm_q8: unknown weight dtype %d", (int)weight_dtype);
+  AMMON_CHECK(std::isfinite(eps) && eps >= 0.f, "rmsnorm_q8: eps must be finite and >= 0");
+  AMMON_CHECK(!residual == !sum, "rmsnorm_q8: residual and sum go together");
+  return q8_rows(rt, stream, x, residual, sum, weight, weight_dtype, eps, tokens, n, out, dtype, "rmsnorm_q8");
+}
+
+ammon_status ammon_q8_load(ammon_runtime *rt, ammon_stream stream, const void *rows, ammon_dtype dtype,
+                           uint32_t tokens, uint32_t n, float *out) {
+  REQUIRE_RT();
+  AMMON_CHECK(rows && out, "q8_load: NULL rows or output");
+  AMMON_CHECK(valid_digits(dtype), "q8_load: rows are AMMON_Q8 or AMMON_Q24, not dtype %d", (int)dtype);
+  TRY(shape_check("q8_load", tokens, n));
+  TRY(aligned("q8_load", rows, "rows"));
+  AMMON_CHECK(!overlaps(out, (size_t)tokens * n * 4, rows, ammon_q8_bytes(dtype, tokens, n)),
+              "q8_load: the output overlaps the rows");
+  VALIDATE_ONLY();
+  ammon_k_q8 p = {};
+  p.rows = (void *)rows;
+  p.sum = out;
+  p.tokens = tokens;
+  p.n = n;
+  p.vec = pieces(out, AMMON_F32, n);
+  const uint64_t eights = (uint64_t)tokens * cdiv(n, 8);
+  return launch(rt, stream, rt->k.q8_load[dtype == AMMON_Q24],
+                (uint32_t)std::min<uint64_t>((eights + kWorkgroup - 1) / kWorkgroup, 1u << 20), 1, 0, p, "q8_load");
+}
+
+ammon_status ammon_prefill_gemm_w4(ammon_runtime *rt, ammon_stream stream, const void *w, uint32_t d, uint32_t n,
+                                   const void *x, ammon_dtype x_dtype, uint32_t tokens, float *y,
+                                   const float *residual, void *workspace, size_t workspace_bytes) {
+  REQUIRE_RT();
+  W4GemmArgs a = {};
+  a.mode = residual ? AMMON_GEMV_RESIDUAL : AMMON_GEMV_PLAIN;
+  a.w0 = w;
+  a.d = d;
+  a.n = n;
+  a.rows = d;
+  a.tokens = tokens;
+  a.x = x;
+  a.x_dtype = x_dtype;
+  a.residual = residual;
+  a.y = y;
+  a.y_bytes = (size_t)tokens * d * 4;
+  a.ws = workspace;
+  a.ws_bytes = workspace ? workspace_bytes : 0;
+  return w4_gemm(rt, stream, a, "prefill_gemm_w4");
+}
+
+ammon_status ammon_prefill_gate_up_swiglu_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                             ammon_dtype x_dtype, uint32_t tokens, const void *w1,
+                                             const void *w3, uint32_t dim, uint32_t hidden, float *hb) {
+  REQUIRE_RT();
+  AMMON_CHECK(w1 && w3, "prefill_gate_up_swiglu_w4: NULL w1 or w3");
+  AMMON_CHECK((uint64_t)hidden * 2 < (1ull << 31), "prefill_gate_up_swiglu_w4: too many rows");
+  W4GemmArgs a = {};
+  a.mode = AMMON_GEMV_SWIGLU;
+  a.w0 = w1;
+  a.w1 = w3;
+  a.d = hidden;
+  a.n = dim;
+  a.rows = 2 * hidden;
+  a.tokens = tokens;
+  a.x = x;
+  a.x_dtype = x_dtype;
+  a.y = hb;
+  a.y_bytes = (size_t)tokens * hidden * 4;
+  return w4_gemm(rt, stream, a, "prefill_gate_up_swiglu_w4");
+}
+
+ammon_status ammon_prefill_qkv_rope_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                       ammon_dtype x_dtype, uint32_t tokens, const void *wq, const void *wk,
+                                       const void *wv, uint32_t dim, uint32_t q_heads, uint32_t kv_heads,
+                                       uint32_t head, float *q, float *k, float *v, uint32_t seq,
+                                       const ammon_decode_step *step, const float *table, void *workspace,
+                                       size_t workspace_bytes) {
+  REQUIRE_RT();
+  return w4_qkv(rt, stream, x, x_dtype, tokens, wq, wk, wv, dim, q_heads, kv_heads, head, q, k, v, AMMON_F32,
+                true, seq, step, table, workspace, workspace_bytes, "prefill_qkv_rope_w4");
+}
+
+ammon_status ammon_prefill_qkv_rope_store_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                             ammon_dtype x_dtype, uint32_t tokens, const void *wq,
+                                             const void *wk, const void *wv, uint32_t dim, uint32_t q_heads,
+                                             uint32_t kv_heads, uint32_t head, float *q, void *k_cache,
+                                             void *v_cache, ammon_dtype kv_dtype, uint32_t seq,
+                                             const ammon_decode_step *step, const float *table,
+                                             void *workspace, size_t workspace_bytes) {
+  REQUIRE_RT();
+  return w4_qkv(rt, stream, x, x_dtype, tokens, wq, wk, wv, dim, q_heads, kv_heads, head, q, k_cache, v_cache,
+                kv_dtype, false, seq, step, table, workspace, workspace_bytes, "prefill_qkv_rope_store_w4");
+}
+
+}  // extern "C"

@@ -17,8 +17,10 @@
  *   - Every call returns an ammon_status.  On failure nothing is launched and
  *     ammon_last_error() returns a message on the calling thread.
  *   - Storage dtypes: AMMON_F32, or AMMON_BF16 (bit patterns, round to nearest
- *     even when written); KV caches also AMMON_KV4 (4 bits a number, below).
- *     Activations are always fp32.
+ *     even when written); KV caches also AMMON_KV4 and weight matrices
+ *     AMMON_W4 (4 bits a number, below).  Activations are fp32; those that
+ *     prompt products of W4 weights take are rows of digits (AMMON_Q8,
+ *     AMMON_Q24, below).
  *   - KV caches are head-major per layer: [kv_heads, seq, head].  The
  *     reference is position-major [seq, kv_heads, head]
  *     (reference src/modules.rs:37-71); ammon_kv_unpermute converts.
@@ -49,9 +51,17 @@ typedef enum ammon_status {
   AMMON_E_NO_DEVICE = 4   /* no usable gfx950 device */
 } ammon_status;
 
-/* AMMON_KV4 is a storage type of KV caches alone (2 and 3 are left to the C++
+/* AMMON_KV4 is a storage type of KV caches alone, AMMON_W4 of weight matrices, AMMON_Q8 and
+ * AMMON_Q24 of the rows that W4 matrices are multiplied with (2 and 3 are left to the C++
  * layer's index types). */
-typedef enum ammon_dtype { AMMON_F32 = 0, AMMON_BF16 = 1, AMMON_KV4 = 4 } ammon_dtype;
+typedef enum ammon_dtype {
+  AMMON_F32 = 0,
+  AMMON_BF16 = 1,
+  AMMON_KV4 = 4,
+  AMMON_W4 = 5,
+  AMMON_Q8 = 6,
+  AMMON_Q24 = 7
+} ammon_dtype;
 
 typedef enum ammon_copy_kind {
   AMMON_COPY_H2D = 1,
@@ -273,6 +283,70 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
                             const void *v_cache, uint32_t kv_heads, uint32_t head, uint32_t seq,
                             uint32_t first, uint32_t count, void *k_out, void *v_out,
                             ammon_dtype out_dtype);
+
+/* ---- 4-bit weights (AMMON_W4) ------------------------------------------------
+ * No counterpart in the reference.  A matrix [d, n] holds its numbers in groups
+ * of 128 of a row, the last one shorter where n is no multiple of 128.  A group
+ * has a scale s (bf16) and a code c in -8..7 per number, which stands for s c.
+ * Storing numbers w (each step rounds to fp32):
+ *   s = bf16(max |w| / 7), 0 where that is below 2^-126
+ *   c = clamp(rint(w (1 / s)), -7, 7), 0 where s = 0
+ * so that a number is off by at most about half a step s, 1/14 of its group's
+ * largest.  A group with a number that is not finite reads back as NaN.
+ *
+ * Memory (ammon_w4_bytes, 16-byte aligned): panels of 16 rows, G = ceil(n / 128)
+ * groups; rows past d and numbers past n are zeros.  A panel has its codes
+ * [G, 4 pieces, 16 rows, 16 bytes], byte b of piece j with number 32 j + b of
+ * the group in its low half and 32 j + 16 + b in its high half (two's
+ * complement), then its scales [4, G, 4], row 4 i + r of the panel at [i, g, r].
+ *
+ * As w_dtype (w1, w3; wq, wk, wv alike) it is taken by ammon_gemv,
+ * ammon_gemv_rmsnorm, ammon_gate_up_swiglu, ammon_qkv_rope(_store) and
+ * ammon_greedy_lm_head: x's numbers enter as 24-bit whole numbers with a scale
+ * per 128 of them (AMMON_Q24 below), their products with the codes of a group
+ * are summed exactly, and the groups in fp32.  An x with a number that is not
+ * finite (after the norm) gives NaN.  Queries, keys and values have to be a
+ * multiple of 16 rows each; n is at most 52096.  ammon_prefill_*_w4 below take
+ * it for several tokens. */
+size_t ammon_w4_bytes(uint32_t d, uint32_t n);
+/* w [d, n] fp32 or bf16 into out. */
+ammon_status ammon_w4_store(ammon_runtime *rt, ammon_stream stream, const void *w,
+                            ammon_dtype w_dtype, uint32_t d, uint32_t n, void *out);
+/* The numbers as [d, n] fp32 or bf16. */
+ammon_status ammon_w4_load(ammon_runtime *rt, ammon_stream stream, const void *w4, uint32_t d,
+                           uint32_t n, void *out, ammon_dtype out_dtype);
+
+/* ---- rows of 8-bit digits (AMMON_Q8, AMMON_Q24) -------------------------------
+ * No counterpart in the reference.  Rows x [tokens, n] in blocks of 128 numbers,
+ * the last one shorter: a scale s (fp32) and a whole number q per number, which
+ * stands for s q (each step rounds to fp32):
+ *   Q8   s = max |x| / 127, 0 where that is below 2^-120
+ *        q = clamp(rint(x (1 / s)), -127, 127), 0 where s = 0
+ *   Q24  s the least power of two >= 2^-120 with max |x| < 127 2^16 s
+ *        q = rint(x / s)
+ * A block with a number that is not finite reads back as NaN.  Q24 is off by at
+ * most 2^-22.9 of its block's largest number (or 2^-121), about the last bit of
+ * an fp32 that large.  q is one digit, or three, d0 + 256 d1 + 65536 d2, in -128..127.
+ *
+ * Memory (ammon_q8_bytes, 16-byte aligned): panels of 16 tokens, B =
+ * ceil(n / 128) blocks: digits [B, digits, 2 halves, 4 pieces, 16 tokens, 16
+ * bytes], byte b of half h and piece j for number 32 j + 16 h + b of the block,
+ * then scales [B, 16].  Tokens past the last one are left as they were. */
+size_t ammon_q8_bytes(ammon_dtype dtype, uint32_t tokens, uint32_t n); /* 0: another dtype */
+/* x [tokens, n] into out. */
+ammon_status ammon_q8_store(ammon_runtime *rt, ammon_stream stream, const float *x,
+                            uint32_t tokens, uint32_t n, void *out, ammon_dtype dtype);
+/* The residual's addition, RMSNorm and the digits in one launch: h = x +
+ * residual to sum (which may be x or residual; both NULL: h = x), then the
+ * digits of v = weight (r h), r = 1 / sqrt(mean(h^2) + eps).  The mean and r are
+ * 64-bit numbers, r rounded to fp32 once; h and each product round to fp32. */
+ammon_status ammon_rmsnorm_q8(ammon_runtime *rt, ammon_stream stream, const float *x,
+                              const float *residual, float *sum, const void *weight,
+                              ammon_dtype weight_dtype, float eps, uint32_t tokens, uint32_t n,
+                              void *out, ammon_dtype dtype);
+/* The numbers as fp32 [tokens, n]. */
+ammon_status ammon_q8_load(ammon_runtime *rt, ammon_stream stream, const void *rows,
+                           ammon_dtype dtype, uint32_t tokens, uint32_t n, float *out);
 
 /* attention_partial (reference src/kernels.rs:228-345): split-K pass over
  * the head-major cache, one workgroup per (split, kv head) serving all
@@ -503,6 +577,34 @@ ammon_status ammon_prefill_gate_up_swiglu(ammon_runtime *rt, ammon_stream stream
                                           uint32_t tokens, const void *w1, const void *w3,
                                           ammon_dtype w_dtype, uint32_t dim, uint32_t hidden,
                                           float *hb);
+/* The same three over W4 weights, x as rows of digits (x_dtype AMMON_Q8 or
+ * AMMON_Q24): products and sums of a group of 128 are exact whole numbers, and
+ * the groups are summed in fp32.  An x row with a NaN block gives NaN.  The
+ * workspace (may be NULL) is ammon_prefill_gemm_ws's; queries, keys and values
+ * are a multiple of 16 rows each. */
+ammon_status ammon_prefill_gemm_w4(ammon_runtime *rt, ammon_stream stream, const void *w,
+                                   uint32_t d, uint32_t n, const void *x, ammon_dtype x_dtype,
+                                   uint32_t tokens, float *y, const float *residual,
+                                   void *workspace, size_t workspace_bytes);
+ammon_status ammon_prefill_gate_up_swiglu_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                             ammon_dtype x_dtype, uint32_t tokens, const void *w1,
+                                             const void *w3, uint32_t dim, uint32_t hidden,
+                                             float *hb);
+ammon_status ammon_prefill_qkv_rope_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                       ammon_dtype x_dtype, uint32_t tokens, const void *wq,
+                                       const void *wk, const void *wv, uint32_t dim,
+                                       uint32_t q_heads, uint32_t kv_heads, uint32_t head, float *q,
+                                       float *k, float *v, uint32_t seq,
+                                       const ammon_decode_step *step, const float *table,
+                                       void *workspace, size_t workspace_bytes);
+ammon_status ammon_prefill_qkv_rope_store_w4(ammon_runtime *rt, ammon_stream stream, const void *x,
+                                             ammon_dtype x_dtype, uint32_t tokens, const void *wq,
+                                             const void *wk, const void *wv, uint32_t dim,
+                                             uint32_t q_heads, uint32_t kv_heads, uint32_t head,
+                                             float *q, void *k_cache, void *v_cache,
+                                             ammon_dtype kv_dtype, uint32_t seq,
+                                             const ammon_decode_step *step, const float *table,
+                                             void *workspace, size_t workspace_bytes);
 /* ammon_attention_decode for each of `tokens` query rows q [tokens, q_heads,
  * head] at positions step->position + t, which must be below ctx <= seq
  * (the scratch and the grid cover ctx positions); out [tokens, q_heads,

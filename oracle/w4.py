@@ -1,0 +1,155 @@
+"""4-bit weights (AMMON_W4) and rows of 8-bit digits (AMMON_Q8, AMMON_Q24) restated in numpy --
+TEST INFRASTRUCTURE.
+
+Every step of the definitions in include/ammon/ammon.h is computed in float64 and rounded where
+the definition rounds; nothing is shared with the kernels.  Products are float64 over the stored
+numbers.  Matrices and rows are the byte arrays that the kernels read.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+GROUP = 128
+
+
+def groups(n: int) -> int:
+    return -(-n // GROUP)
+
+
+def w4_bytes(d: int, n: int) -> int:
+    return -(-d // 16) * groups(n) * 1056
+
+
+def q8_bytes(digits: int, tokens: int, n: int) -> int:
+    return -(-tokens // 16) * groups(n) * (2048 * digits + 64)
+
+
+def f32(x):
+    with np.errstate(over="ignore"):
+        return np.asarray(x, np.float64).astype(np.float32).astype(np.float64)
+
+
+def bf16(x):
+    """fp32 numbers (float64) rounded to nearest even bf16."""
+    u = np.ascontiguousarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    u = ((u + 0x7fff + ((u >> 16) & 1)) & 0xffff0000).astype(np.uint32)
+    return np.where(np.isnan(x), np.nan, u.view(np.float32).astype(np.float64))
+
+
+def blocks(x):
+    """Rows [r, n] as [r, groups, 128], zeros past the end (float64)."""
+    x = np.asarray(x, np.float64)
+    out = np.zeros((x.shape[0], groups(x.shape[1]) * GROUP))
+    out[:, :x.shape[1]] = x
+    return out.reshape(x.shape[0], -1, GROUP)
+
+
+def _ends(b):
+    bad = ~np.isfinite(b).all(-1)
+    return bad, np.abs(np.where(np.isfinite(b), b, 0)).max(-1), np.where(bad[..., None], 0, b)
+
+
+def w4_quantise(w):
+    """Codes [d, groups, 128] and scales [d, groups] of a matrix."""
+    bad, top, b = _ends(blocks(w))
+    s = bf16(f32(top / 7))
+    s = np.where(s < 2.0**-126, 0, s)
+    inv = np.where(s > 0, f32(1 / np.where(s > 0, s, 1)), 0)
+    c = np.clip(np.rint(f32(b * inv[..., None])), -7, 7)
+    return c.astype(np.int8), np.where(bad, np.nan, s)
+
+
+def w4_numbers(codes, s, n):
+    return (codes * s[..., None]).reshape(codes.shape[0], -1)[:, :n]
+
+
+def w4_pack(codes, s):
+    """The bytes of codes [d, groups, 128] and scales [d, groups]."""
+    d, g = s.shape
+    dp = -(-d // 16) * 16
+    c = np.zeros((dp, g, GROUP), np.int8)
+    c[:d] = codes
+    sc = np.zeros((dp, g), np.float32)
+    sc[:d] = s
+    out = np.zeros((dp // 16, g * 1056), np.uint8)
+    for p in range(dp // 16):
+        for r in range(16):
+            for j in range(4):
+                piece = c[16 * p + r, :, 32 * j:32 * j + 32].astype(np.uint8) & 15
+                byte = piece[:, :16] | piece[:, 16:] << 4
+                for k in range(g):
+                    at = 1024 * k + 256 * j + 16 * r
+                    out[p, at:at + 16] = byte[k]
+            for k in range(g):
+                at = 1024 * g + 2 * (((r // 4) * g + k) * 4 + r % 4)
+                u = np.float32(sc[16 * p + r, k]).view(np.uint32) >> 16
+                out[p, at:at + 2] = [u & 255, u >> 8]
+    return out.reshape(-1)
+
+
+def q_quantise(x, digits):
+    """Whole numbers [tokens, blocks, 128] and scales [tokens, blocks] of rows."""
+    bad, top, b = _ends(blocks(x))
+    if digits == 1:
+        s = f32(top / 127)
+        s = np.where(s < 2.0**-120, 0, s)
+        inv = np.where(s > 0, f32(1 / np.where(s > 0, s, 1)), 0)
+        q = np.clip(np.rint(f32(b * inv[..., None])), -127, 127)
+    else:
+        s = np.full(top.shape, 2.0**-120)
+        while (top >= 127 * 65536 * s).any():
+            s = np.where(top >= 127 * 65536 * s, 2 * s, s)
+        q = np.rint(b / s[..., None])
+    return q.astype(np.int32), np.where(bad, np.nan, s)
+
+
+def q_numbers(q, s, n):
+    return f32(q * s[..., None]).reshape(q.shape[0], -1)[:, :n]
+
+
+def q_pack(q, s, digits, into=None):
+    """The bytes of rows; what a panel's tokens past the last one hold is kept from `into`."""
+    t, b = s.shape
+    tp = -(-t // 16) * 16
+    size = b * (2048 * digits + 64)
+    out = (np.zeros(tp // 16 * size, np.uint8) if into is None else into.copy()).reshape(tp // 16, size)
+    scales = np.ascontiguousarray(s, np.float32)
+    for i in range(t):
+        rest = q[i].astype(np.int64)  # [blocks, 128]
+        for d in range(digits):
+            low = (rest + 128) % 256 - 128
+            rest = (rest - low) // 256
+            for h in range(2):
+                for j in range(4):
+                    piece = low[:, 32 * j + 16 * h:32 * j + 16 * h + 16].astype(np.int8).view(np.uint8)
+                    for k in range(b):
+                        at = ((k * digits + d) * 2 + h) * 1024 + 256 * j + 16 * (i % 16)
+                        out[i // 16, at:at + 16] = piece[k]
+        assert not rest.any()
+        for k in range(b):
+            at = b * 2048 * digits + 4 * (16 * k + i % 16)
+            out[i // 16, at:at + 4] = np.frombuffer(scales[i, k].tobytes(), np.uint8)
+    return out.reshape(-1)
+
+
+def normed(x, w, eps):
+    """RMSNorm as ammon_rmsnorm_q8 defines it: the mean and its root in 64 bits, the rest in 32."""
+    x = np.asarray(x, np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        r = f32(1 / np.sqrt((x * x).mean(-1, keepdims=True) + np.float64(np.float32(eps))))
+        return f32(np.asarray(w, np.float64) * f32(r * x))
+
+
+def product_bar(x, w, exact_x):
+    """How far fp32 results of rows x [t, n] (float64) times w [d, n] may be from float64's [t, d].
+    With x as Q24 in the call (exact_x False), a number of x is off by half a step, 2^-22.98 of its
+    block's largest.  A group's sum is exact, its conversion from whole numbers (of 24 bits and
+    more) and its addition round by 2^-24 of the sums so far, at most sum |w| |x|, and so do three
+    additions of digits, three of waves, seven of ranges and the residual's."""
+    a, b = np.abs(x), np.abs(w)
+    size = a @ b.T
+    bar = (2 * groups(x.shape[1]) + 16) * 2.0**-24 * size
+    if not exact_x:
+        top = blocks(a).max(-1)  # [t, groups]
+        bar += 2.0**-22.98 * top @ blocks(b).sum(-1).T
+    return bar
