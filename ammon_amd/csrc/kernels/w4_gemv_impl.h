@@ -35,26 +35,23 @@ template <int MODE> struct W4Gemv {
 
   AMMON_DEV Unit unit(uint32_t u) const {
     const uint32_t j = lane >> 4;
-    const void *base;
+    const void *const w0 = p.w0, *const w1 = p.w1, *const w2 = p.w2, *base = w0;
     uint32_t panel = u, row = lane & 15, quad = j;
-    size_t bytes = (size_t)groups * W4_PANEL_BYTES;
+    const size_t bytes = (size_t)groups * W4_PANEL_BYTES;
     if (MODE == AMMON_GEMV_SWIGLU) {
       // rows 0..7 gate, 8..15 up; results' quads 0, 1 gate, 2, 3 up
       const uint32_t half = (u & 1) * 8;
       panel = u >> 1;
-      const uint8_t *codes = (const uint8_t *)(row < 8 ? p.w0 : p.w1) + panel * bytes;
-      const uint8_t *sc = (const uint8_t *)(quad < 2 ? p.w0 : p.w1) + panel * bytes;
+      const uint8_t *codes = (const uint8_t *)(row < 8 ? w0 : w1) + panel * bytes;
+      const uint8_t *sc = (const uint8_t *)(quad < 2 ? w0 : w1) + panel * bytes;
       row = half + (row & 7);
       quad = half / 4 + (quad & 1);
       return Unit{codes + j * 256 + row * 16, sc + (size_t)groups * 1024 + (size_t)quad * groups * 8};
     }
-    base = p.w0;
     if (MODE == AMMON_GEMV_QKV) {
       const uint32_t q = p.d / 16, kv = p.kv_dim / 16;
-      if (u >= q + kv)
-        base = p.w2, panel = u - q - kv;
-      else if (u >= q)
-        base = p.w1, panel = u - q;
+      base = u >= q + kv ? w2 : u >= q ? w1 : w0;
+      panel -= u >= q + kv ? q + kv : u >= q ? q : 0;
     }
     const uint8_t *at = (const uint8_t *)base + panel * bytes;
     return Unit{at + j * 256 + row * 16, at + (size_t)groups * 1024 + (size_t)quad * groups * 8};

@@ -21,7 +21,7 @@ bool pieces(const void *base, ammon_dtype dt, uint32_t n) {
 ammon_status shape_check(const char *what, uint32_t rows, uint32_t n) {
   AMMON_CHECK(rows > 0 && n > 0, "%s: empty shape (%u rows of %u)", what, rows, n);
   AMMON_CHECK(cdiv(rows, 16) <= kMaxWorkgroups, "%s: %u rows are too many", what, rows);
-  AMMON_CHECK(n < (1u << 28), "%s: rows of %u numbers are too long", what, n);
+  AMMON_CHECK(n < (1u << 22), "%s: rows of %u numbers are too long", what, n);
   return AMMON_OK;
 }
 
