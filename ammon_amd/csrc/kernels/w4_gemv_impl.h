@@ -1,28 +1,34 @@
 // w4_gemv_impl.h -- products of one token's row with 4-bit weights (w4_impl.h): the modes of
 // gemv_impl.h (plain, residual, SwiGLU, QKV, argmax candidates) over AMMON_W4 matrices.
 //
-// y_r = sum_k W[r, k] x_k.  x (RMS-normalised where a weight is given) becomes Q24 digits in LDS,
-// once per workgroup; a wave multiplies 16 rows x 128 numbers, 1 KiB of codes, by two
-// v_mfma_i32_16x16x64_i8: the codes are operand A as they lie in memory but for an AND and a
-// shift, and the three digits are columns 0..2 of operand B (the other columns repeat the third
-// and are scaled by 0).  A group's sums are exact; they are scaled by s_w s_x 256^digit, exact
-// too, and added up over the groups in fp32 with one rounding each.
+// y_r = sum_k W[r, k] x_k.  x (RMS-normalised where a weight is given) becomes whole numbers in
+// LDS, once per workgroup: as Q24's, but of four digits (2^-31 of a block's largest number: exact
+// next to the fp32 sums), since a matrix instruction has 16 columns and takes them for nothing.  A
+// wave multiplies 16 rows x 128 numbers, 1 KiB of codes, by two v_mfma_i32_16x16x64_i8: the codes
+// are operand A as they lie in memory but for an AND and a shift, and the digits are columns 0..3
+// of operand B (the other columns repeat them and are not used).  A group's sums are exact; they
+// are scaled by s_w s_x 256^digit, exact too, and added up over the groups in fp32 with one
+// rounding each.
 //
-// A workgroup of 4 waves takes units of 16 virtual rows (a panel; SwiGLU: 8 gate and the same 8
-// up rows) and splits the groups over its waves; each wave has the codes of U groups in two
-// register buffers, the next ones requested before the current are multiplied.
+// A workgroup has US sets of 8 waves.  A set takes a unit of 16 virtual rows (a panel; SwiGLU: 8
+// gate and the same 8 up rows) at a time; its waves take the chunks of U groups in turn, and their
+// sums meet in LDS.  Each wave has two chunks in registers: one is multiplied while the other is
+// on its way, and is then requested anew.
 #pragma once
 
 #include "argmax_impl.h"
 #include "w4_impl.h"
 
-template <int MODE> struct W4Gemv {
-  static constexpr uint32_t U = 8;  // groups a register buffer holds
+template <int MODE, uint32_t US> struct W4Gemv {
+  static constexpr uint32_t U = AMMON_W4_CHUNK;         // groups a register buffer holds
+  static constexpr uint32_t KS = AMMON_W4_SET;          // waves of a set
+  static constexpr uint32_t THREADS = 64 * KS * US;
+  static constexpr int D = 4;
 
   ammon_k_gemv p;
-  uint32_t lane, wave, groups, per;  // per: groups of a wave
-  uint8_t *digits;                   // LDS: [groups][2 halves][3 digits][64 bytes]
-  float *scales;                     // LDS: [groups][4], s_x 256^digit / 16 (the codes are 16 c); 0
+  uint32_t lane, wave, set, groups, chunks;  // chunks: a wave's of a unit
+  uint8_t *digits;                   // LDS: [groups][2 halves][4 digits][64 bytes]
+  float *scales;                     // LDS: [groups][4], s_x 256^digit / 16 (the codes are 16 c)
   // operands' addresses in the current unit
   struct Unit {
     const uint8_t *codes;
@@ -57,96 +63,152 @@ template <int MODE> struct W4Gemv {
     return Unit{at + j * 256 + row * 16, at + (size_t)groups * 1024 + (size_t)quad * groups * 8};
   }
 
-  // Groups first .. + U - 1 of this wave's; past its last one, that one again (not multiplied).
-  AMMON_DEV void load(const Unit &u, uint32_t first, uint32_t last, Buffer &b) const {
+  // The groups of this wave's chunk c of a unit; past the last group, that one (x is zeros there).
+  AMMON_DEV void load(const Unit &u, uint32_t c, Buffer &b) const {
+    const uint32_t first = (c * KS + wave) * U;
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
-      const uint32_t g = min(first + i, last);
+      const uint32_t g = min(first + i, groups - 1);
       b.codes[i] = __builtin_nontemporal_load((const u32x4 *)(u.codes + (size_t)g * 1024));
       b.scales[i] = __builtin_nontemporal_load((const u32x2 *)(u.scales + (size_t)g * 8));
     }
   }
 
-  AMMON_DEV void multiply(uint32_t first, uint32_t end, const Buffer &b, f32x4 &acc) const {
-    const uint32_t col = min(lane & 15, 3u), digit = min(col, 2u), j = lane >> 4;
+  AMMON_DEV void multiply(uint32_t c, const Buffer &b, f32x4 &acc) const {
+    const uint32_t first = (c * KS + wave) * U, col = lane & 3, j = lane >> 4;
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
-      const uint32_t g = first + i;
-      if (g >= end) break;
-      const uint8_t *d = digits + ((size_t)g * 6 + digit) * 64 + j * 16;
-      const i32x4 b0 = *(const i32x4 *)d, b1 = *(const i32x4 *)(d + 192);
-      i32x4 c = i32x4{0, 0, 0, 0};
-      c = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half0(b.codes[i]), b0, c, 0, 0, 0);
-      c = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half1(b.codes[i]), b1, c, 0, 0, 0);
-      const float sx = scales[4 * g + col];
+      const uint8_t *d = digits + (first + i) * (2 * D * 64) + col * 64 + j * 16;
+      const i32x4 b0 = *(const i32x4 *)d, b1 = *(const i32x4 *)(d + D * 64);
+      i32x4 t = i32x4{0, 0, 0, 0};
+      t = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half0(b.codes[i]), b0, t, 0, 0, 0);
+      t = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half1(b.codes[i]), b1, t, 0, 0, 0);
+      const float sx = scales[4 * (first + i) + col];
       const u32x2 s = b.scales[i];
       const float sw[4] = {bf16_lo(s[0]), bf16_hi(s[0]), bf16_lo(s[1]), bf16_hi(s[1])};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] = fmaf((float)c[r], sx * sw[r], acc[r]);
+      for (int r = 0; r < 4; ++r) acc[r] = fmaf((float)t[r], sx * sw[r], acc[r]);
     }
   }
 
-  // x as digits in LDS, normalised first where there is a weight.  red: AMMON_WAVES floats.
-  AMMON_DEV void stage(float *red) {
-    constexpr int R = 4;  // eights of x that a thread keeps in registers
-    const uint32_t tid = threadIdx.x, eights = groups * 16, n = p.n;
-    const bool vec = (n & 3u) == 0 && ((uintptr_t)p.x & 15u) == 0;
-    const bool wvec = (n & 3u) == 0 && ((uintptr_t)p.norm_w & (p.norm_dtype == AMMON_K_BF16 ? 7u : 15u)) == 0;
-    float v[R][8];
+  // x as digits in LDS, normalised first where there is a weight; zeros up to whole rounds of
+  // chunks.  Eights of x: R of a thread's are requested by begin() and kept in registers, the
+  // others read again by each pass of stage().
+  static constexpr int R = 2;
+  struct Staged {
+    u32x4 x[R][2], w[R][2];
+  };
+  AMMON_DEV static u32x4 four(const __amdgpu_buffer_rsrc_t &r, uint32_t at, bool vec) {
+    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+    return u32x4{__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0), __builtin_amdgcn_raw_buffer_load_b32(r, at + 4, 0, 0),
+                 __builtin_amdgcn_raw_buffer_load_b32(r, at + 8, 0, 0),
+                 __builtin_amdgcn_raw_buffer_load_b32(r, at + 12, 0, 0)};
+  }
+  // (past the end buffers read as zero)
+  AMMON_DEV void load_x(uint32_t c, u32x4 (&v)[2]) const {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.x, p.n * 4);
+    const bool vec = (p.n & 3u) == 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (tid + r * AMMON_WG < eights) w4_load8(p.x, tid + r * AMMON_WG, n, vec, v[r]);
+    for (int h = 0; h < 2; ++h) v[h] = four(r, 32 * c + 16 * h, vec);
+  }
+  AMMON_DEV void load_w(uint32_t c, u32x4 (&v)[2]) const {  // bf16: v[0], raw
+    if (p.norm_dtype == AMMON_K_F32) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(p.norm_w, p.n * 4);
+      const bool vec = (p.n & 3u) == 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[h] = four(r, 32 * c + 16 * h, vec);
+    } else {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(p.norm_w, p.n * 2);
+      if ((p.n & 7u) == 0 && ((uintptr_t)p.norm_w & 3u) == 0) {
+        v[0] = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * c, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[0][e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e, 0, 0) |
+                    (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e + 2, 0, 0) << 16;
+      }
+      v[1] = u32x4{0, 0, 0, 0};
+    }
+  }
+  AMMON_DEV void begin(Staged &s) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      load_x(threadIdx.x + r * THREADS, s.x[r]);
+      if (p.norm_w) load_w(threadIdx.x + r * THREADS, s.w[r]);
+    }
+  }
+  AMMON_DEV static void square(const u32x4 (&v)[2], float &ss) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = __uint_as_float(v[h][e]);
+        ss = fmaf(f, f, ss);
+      }
+  }
+  AMMON_DEV void put(uint32_t c, const u32x4 (&x)[2], const u32x4 (&w)[2], float scale) const {
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = __uint_as_float(x[e / 4][e % 4]);
+    if (p.norm_w) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = p.norm_dtype == AMMON_K_F32 ? __uint_as_float(w[e / 4][e % 4])
+                        : e % 2                     ? bf16_hi(w[0][e / 2])
+                                                    : bf16_lo(w[0][e / 2]);
+        h[e] = f * (scale * h[e]);
+      }
+    }
+    uint2 d[D];
+    const float s = q8_digits<D>(h, d);
+    const uint32_t g = c / 16, i = c & 15;
+    uint8_t *at = digits + g * (2 * D * 64) + ((i >> 1) & 1) * (D * 64) + (i >> 2) * 16 + (i & 1) * 8;
+#pragma unroll
+    for (int k = 0; k < D; ++k) *(uint2 *)(at + 64 * k) = d[k];
+    if (i == 0) *(float4 *)(scales + 4 * g) = make_float4(s * 0.0625f, s * 16.f, s * 4096.f, s * 1048576.f);
+  }
+  AMMON_DEV void stage(const Staged &st, float *red) const {
+    const uint32_t tid = threadIdx.x, eights = chunks * KS * U * 16;
     float scale = 1.f;
     if (p.norm_w) {
       float ss = 0.f;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (tid + r * AMMON_WG < eights)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(v[r][e], v[r][e], ss);
-      for (uint32_t c = tid + R * AMMON_WG; c < eights; c += AMMON_WG) {
-        float h[8];
-        w4_load8(p.x, c, n, vec, h);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
+      for (int r = 0; r < R; ++r) square(st.x[r], ss);
+      for (uint32_t c = tid + R * THREADS; c < eights; c += THREADS) {
+        u32x4 v[2];
+        load_x(c, v);
+        square(v, ss);
       }
-      ss = block_sum(ss, red);
-      scale = 1.0f / sqrtf(ss / (float)n + p.eps);
+      ss = wave_sum(ss);
+      if (lane == 0) red[threadIdx.x >> 6] = ss;
+      __syncthreads();
+      ss = red[0];
+#pragma unroll
+      for (uint32_t w = 1; w < KS * US; ++w) ss += red[w];
+      scale = 1.0f / sqrtf(ss / (float)p.n + p.eps);
     }
-    auto put = [&](uint32_t c, float (&h)[8]) {
-      if (p.norm_w) {
-        float w[8];
-        w4_load8(p.norm_w, p.norm_dtype, c, n, wvec, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = w[e] * (scale * h[e]);
-      }
-      uint2 d[3];
-      const float s = q8_digits<3>(h, d);
-      const uint32_t g = c / 16, i = c & 15;
-      uint8_t *at = digits + ((size_t)g * 6 + ((i >> 1) & 1) * 3) * 64 + (i >> 2) * 16 + (i & 1) * 8;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) *(uint2 *)(at + 64 * k) = d[k];
-      if (i == 0) *(float4 *)(scales + 4 * g) = make_float4(s * 0.0625f, s * 16.f, s * 4096.f, 0.f);
-    };
+    // (a block's 16 lanes go together: eights and the stride are multiples of 16)
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (tid + r * AMMON_WG < eights) put(tid + r * AMMON_WG, v[r]);
-    for (uint32_t c = tid + R * AMMON_WG; c < eights; c += AMMON_WG) {
-      float h[8];
-      w4_load8(p.x, c, n, vec, h);
-      put(c, h);
+      if (tid + r * THREADS < eights) put(tid + r * THREADS, st.x[r], st.w[r], scale);
+    for (uint32_t c = tid + R * THREADS; c < eights; c += THREADS) {
+      u32x4 v[2], w[2];
+      load_x(c, v);
+      if (p.norm_w) load_w(c, w);
+      put(c, v, w, scale);
     }
   }
 
-  // Rows' sums of unit u, red [waves][16]: added in wave order, then the mode's epilogue.
+  // Rows' sums of unit u, red [waves][16]: added in wave order, then the mode's epilogue, by one
+  // wave.
   AMMON_DEV float row_sum(const float *red, uint32_t r) const {
     float v = red[r];
 #pragma unroll
-    for (int w = 1; w < AMMON_WAVES; ++w) v += red[16 * w + r];
+    for (uint32_t w = 1; w < KS; ++w) v += red[16 * w + r];
     return v;
   }
   AMMON_DEV void finish(uint32_t u, const float *red, uint32_t pos, float &cand_v, uint32_t &cand_i) const {
-    const uint32_t e = threadIdx.x;
+    const uint32_t e = lane;
     if (MODE == AMMON_GEMV_SWIGLU) {
       if (e >= 8 || 8 * u + e >= p.d) return;
       const float gate = row_sum(red, e), up = row_sum(red, 8 + e);
@@ -197,66 +259,82 @@ template <int MODE> struct W4Gemv {
   }
 
   AMMON_DEV void run(const ammon_k_gemv &params, uint32_t nwg, uint8_t *lds) {
-    __shared__ float red[2][AMMON_WAVES][16];
+    __shared__ float red[2][US][KS][16];
     p = params;
     lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wave = w % KS, set = w / KS;
     groups = w4_groups(p.n);
-    per = (groups + AMMON_WAVES - 1) / AMMON_WAVES;
+    chunks = (groups + KS * U - 1) / (KS * U);
     scales = (float *)lds;
-    digits = lds + (size_t)groups * 16;
-    const uint32_t gbeg = min(wave * per, groups), gend = min(gbeg + per, groups);
-    const uint32_t last = groups - 1;  // (a wave without groups requests the last one)
-    const uint32_t chunks = (per + U - 1) / U, units = p.row_blocks;
+    digits = lds + (size_t)chunks * KS * U * 16;
     uint32_t pos = 0;
     if (MODE == AMMON_GEMV_QKV) pos = p.step->position;
 
-    // steps (unit, chunk) of this workgroup, two buffers ahead
-    const uint32_t total = blockIdx.x < units ? ((units - 1 - blockIdx.x) / nwg + 1) * chunks : 0;
-    Buffer bufs[2];
-    uint32_t lu = blockIdx.x, lc = 0;  // the next request's
-    Unit at = unit(min(lu, units - 1));
+    // The sets of a workgroup take units blockIdx.x, + nwg, .. in pairs of US; steps are (unit,
+    // chunk), and a set without a unit in the last one multiplies the last unit again, unheard.
+    const uint32_t units = p.row_blocks, rounds = (units + nwg * US - 1) / (nwg * US);
+    const uint32_t total = rounds * chunks;
+    auto unit_of = [&](uint32_t round) { return (round * nwg + blockIdx.x) * US + set; };
+    uint32_t lr = 0, lc = 0;  // the next request's round and chunk
+    Unit at = unit(min(unit_of(0), units - 1));
     auto request = [&](Buffer &b) {
-      if (lu >= units) return;
-      load(at, gbeg + lc * U, gend ? min(gend - 1, last) : last, b);
+      load(at, lc, b);
       if (++lc == chunks) {
         lc = 0;
-        lu += nwg;
-        at = unit(min(lu, units - 1));
+        at = unit(min(unit_of(++lr), units - 1));
       }
     };
-    request(bufs[0]);
-    stage(&red[0][0][0]);
+    Staged st;
+    begin(st);
+    Buffer b0, b1;
+    request(b0);
+    if (total > 1) request(b1);
+    stage(st, &red[0][0][0][0]);
     __syncthreads();
     float cand_v = 0.f;
     uint32_t cand_i = ARGMAX_NONE;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    uint32_t u = blockIdx.x, c = 0, flip = 0;
-    auto step = [&](Buffer &now, Buffer &next) {
-      request(next);
-      multiply(gbeg + c * U, gend, now, acc);
+    uint32_t round = 0, c = 0;
+    auto step = [&](const Buffer &now) {
+      multiply(c, now, acc);
       if (++c < chunks) return;
-      // columns 0..2 of a row, then the waves
-      float(&r)[AMMON_WAVES][16] = red[flip];
+      // the four columns of a row, then the set's waves
+      float(&r)[KS][16] = red[round & 1][set];
       f32x4 sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = group_sum16(acc[i], 4);
       if ((lane & 15) == 0) *(f32x4 *)&r[wave][4 * (lane >> 4)] = sum;
       __syncthreads();
-      finish(u, &r[0][0], pos, cand_v, cand_i);
+      const uint32_t u = unit_of(round);
+      if (wave == round % KS && u < units) finish(u, &r[0][0], pos, cand_v, cand_i);
       acc = f32x4{0.f, 0.f, 0.f, 0.f};
       c = 0;
-      u += nwg;
-      flip ^= 1;
+      ++round;
     };
-    for (uint32_t i = 0; i < total; i += 2) {
-      step(bufs[0], bufs[1]);
-      if (i + 1 < total) step(bufs[1], bufs[0]);
+    uint32_t i = 0;
+    for (; i + 3 < total; i += 2) {
+      step(b0);
+      request(b0);
+      step(b1);
+      request(b1);
     }
+    step(b0);
+    if (i + 2 < total) request(b0);
+    if (i + 1 < total) step(b1);
+    if (i + 2 < total) step(b0);
     if (MODE == AMMON_GEMV_PLAIN_ARGMAX) {
+      // the workgroup's candidate
       __syncthreads();
-      block_cand_reduce(cand_v, cand_i, &red[0][0][0], (uint32_t *)&red[1][0][0]);
+      float *sv = &red[0][0][0][0];
+      uint32_t *si = (uint32_t *)&red[1][0][0][0];
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1)
+        cand_merge(cand_v, cand_i, __shfl_xor(cand_v, off, 64), __shfl_xor(cand_i, off, 64));
+      if (lane == 0) sv[w] = cand_v, si[w] = cand_i;
+      __syncthreads();
       if (threadIdx.x == 0) {
+        for (uint32_t k = 1; k < KS * US; ++k) cand_merge(cand_v, cand_i, sv[k], si[k]);
         st_out(p.cand_v + blockIdx.x, cand_v);
         st_out(p.cand_i + blockIdx.x, cand_i);
       }

@@ -84,7 +84,7 @@ template <int DIGITS> AMMON_DEV float q8_digits(const float (&x)[8], uint2 (&dig
     inv = s > 0.f ? 1.0f / s : 0.f;
   } else {
     // the exponent, one more where the fraction is at least 127 / 64
-    const int k = max((int)((top + 0x20000u) >> 23) - 127 - 22, -120);
+    const int k = max((int)((top + 0x20000u) >> 23) - 127 - (8 * DIGITS - 2), -120);
     s = __uint_as_float((uint32_t)(k + 127) << 23);
     inv = __uint_as_float((uint32_t)(127 - k) << 23);
   }

@@ -207,11 +207,12 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
     R(8, name, k.q8_load[q]);
   }
-  for (int m = 0; m <= kGemvModes; ++m) {
-    char name[96];
-    snprintf(name, sizeof name, "ammon_w4_gemv_%s", m < kGemvModes ? modes[m] : "plain_argmax");
-    R(9, name, k.w4_gemv[m]);
-  }
+  for (int u = 0; u < 2; ++u)
+    for (int m = 0; m <= kGemvModes; ++m) {
+      char name[96];
+      snprintf(name, sizeof name, "ammon_w4_gemv_%s_s%d", m < kGemvModes ? modes[m] : "plain_argmax", u + 1);
+      R(9, name, k.w4_gemv[u][m]);
+    }
   const char *w4_tiles[kW4Tiles] = {"t16", "t64"};
   for (int q = 0; q < 2; ++q)
     for (int t = 0; t < kW4Tiles; ++t)
