@@ -22,9 +22,7 @@ extern "C" {
 #define AMMON_K_W4 5  /* weights only: kernels/w4_impl.h */
 #define AMMON_K_Q8 6  /* rows of one 8-bit digit a number, and of three */
 #define AMMON_K_Q24 7
-/* W4 GEMV: waves of a set, which share a unit's rows; groups of 128 a wave takes at once */
-#define AMMON_W4_SET 8
-#define AMMON_W4_CHUNK 4
+#define AMMON_W4_CHUNK 4 /* W4 GEMV: groups of 128 that a wave takes at once */
 #define AMMON_KV4_LOAD_ROWS 4 /* rows a lane of kv4_load takes */
 
 /* Device-resident control parcel: same layout as ammon_decode_step. */

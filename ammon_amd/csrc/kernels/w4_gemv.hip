@@ -2,18 +2,20 @@
 // with the workgroups of the grid, x's digits in dynamic LDS.
 #include "w4_gemv_impl.h"
 
-#define W4_GEMV_KERNEL(NAME, MODE, US)                                                          \
-  extern "C" __global__ __launch_bounds__(64 * AMMON_W4_SET * US) void NAME(ammon_k_gemv p, uint32_t nwg) { \
-    extern __shared__ u32x4 lds[];                                                              \
-    W4Gemv<MODE, US> pass;                                                                      \
-    pass.run(p, nwg, (uint8_t *)lds);                                                           \
+// KS waves of a set, NW of a workgroup
+#define W4_GEMV_KERNEL(NAME, MODE, KS, NW)                                                     \
+  extern "C" __global__ __launch_bounds__(64 * NW, 4) void NAME(ammon_k_gemv p, uint32_t nwg) { \
+    extern __shared__ u32x4 lds[];                                                             \
+    W4Gemv<MODE, KS, NW> pass;                                                                 \
+    pass.run(p, nwg, (uint8_t *)lds);                                                          \
   }
-#define W4_GEMV_MODES(SUFFIX, US)                                        \
-  W4_GEMV_KERNEL(ammon_w4_gemv_plain##SUFFIX, AMMON_GEMV_PLAIN, US)      \
-  W4_GEMV_KERNEL(ammon_w4_gemv_residual##SUFFIX, AMMON_GEMV_RESIDUAL, US) \
-  W4_GEMV_KERNEL(ammon_w4_gemv_swiglu##SUFFIX, AMMON_GEMV_SWIGLU, US)    \
-  W4_GEMV_KERNEL(ammon_w4_gemv_qkv##SUFFIX, AMMON_GEMV_QKV, US)          \
-  W4_GEMV_KERNEL(ammon_w4_gemv_plain_argmax##SUFFIX, AMMON_GEMV_PLAIN_ARGMAX, US)
+#define W4_GEMV_MODES(SUFFIX, KS, NW)                                         \
+  W4_GEMV_KERNEL(ammon_w4_gemv_plain##SUFFIX, AMMON_GEMV_PLAIN, KS, NW)       \
+  W4_GEMV_KERNEL(ammon_w4_gemv_residual##SUFFIX, AMMON_GEMV_RESIDUAL, KS, NW) \
+  W4_GEMV_KERNEL(ammon_w4_gemv_swiglu##SUFFIX, AMMON_GEMV_SWIGLU, KS, NW)     \
+  W4_GEMV_KERNEL(ammon_w4_gemv_qkv##SUFFIX, AMMON_GEMV_QKV, KS, NW)           \
+  W4_GEMV_KERNEL(ammon_w4_gemv_plain_argmax##SUFFIX, AMMON_GEMV_PLAIN_ARGMAX, KS, NW)
 
-W4_GEMV_MODES(_s1, 1)
-W4_GEMV_MODES(_s2, 2)
+W4_GEMV_MODES(_k8, 8, 8)
+W4_GEMV_MODES(_k2, 2, 8)
+W4_GEMV_MODES(_k8_wide, 8, 16)

@@ -10,23 +10,27 @@
 // are scaled by s_w s_x 256^digit, exact too, and added up over the groups in fp32 with one
 // rounding each.
 //
-// A workgroup has US sets of 8 waves.  A set takes a unit of 16 virtual rows (a panel; SwiGLU: 8
-// gate and the same 8 up rows) at a time; its waves take the chunks of U groups in turn, and their
-// sums meet in LDS.  Each wave has two chunks in registers: one is multiplied while the other is
-// on its way, and is then requested anew.
+// A workgroup of NW waves has sets of KS.  A set takes a unit of 16 virtual rows (a panel; SwiGLU:
+// 8 gate and the same 8 up rows) at a time; its waves take the chunks of U groups in turn, and
+// their sums meet in LDS.  Each wave has two chunks in registers: one is multiplied while the other
+// is on its way, and is then requested anew.
+//
+// The norm's factor is one for the whole row: it is applied to the results, so that the digits
+// (of w x) do not wait for the sum of squares.
 #pragma once
 
 #include "argmax_impl.h"
 #include "w4_impl.h"
 
-template <int MODE, uint32_t US> struct W4Gemv {
-  static constexpr uint32_t U = AMMON_W4_CHUNK;         // groups a register buffer holds
-  static constexpr uint32_t KS = AMMON_W4_SET;          // waves of a set
-  static constexpr uint32_t THREADS = 64 * KS * US;
+template <int MODE, uint32_t KS, uint32_t NW> struct W4Gemv {
+  static constexpr uint32_t U = AMMON_W4_CHUNK;  // groups a register buffer holds
+  static constexpr uint32_t US = NW / KS;        // sets
+  static constexpr uint32_t THREADS = 64 * NW;
   static constexpr int D = 4;
 
   ammon_k_gemv p;
   uint32_t lane, wave, set, groups, chunks;  // chunks: a wave's of a unit
+  float factor;                      // the norm's
   uint8_t *digits;                   // LDS: [groups][2 halves][4 digits][64 bytes]
   float *scales;                     // LDS: [groups][4], s_x 256^digit / 16 (the codes are 16 c)
   // operands' addresses in the current unit
@@ -64,13 +68,16 @@ template <int MODE, uint32_t US> struct W4Gemv {
   }
 
   // The groups of this wave's chunk c of a unit; past the last group, that one (x is zeros there).
+  // Codes are read once; scales are parts of lines that other chunks read too and stay in the
+  // caches (as nontemporal loads they cost 4-10% of a long matrix's time; as two 16-byte loads of
+  // two groups each, where groups are even, nothing was gained).
   AMMON_DEV void load(const Unit &u, uint32_t c, Buffer &b) const {
     const uint32_t first = (c * KS + wave) * U;
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
       const uint32_t g = min(first + i, groups - 1);
       b.codes[i] = __builtin_nontemporal_load((const u32x4 *)(u.codes + (size_t)g * 1024));
-      b.scales[i] = __builtin_nontemporal_load((const u32x2 *)(u.scales + (size_t)g * 8));
+      b.scales[i] = *(const u32x2 *)(u.scales + (size_t)g * 8);
     }
   }
 
@@ -146,7 +153,7 @@ template <int MODE, uint32_t US> struct W4Gemv {
         ss = fmaf(f, f, ss);
       }
   }
-  AMMON_DEV void put(uint32_t c, const u32x4 (&x)[2], const u32x4 (&w)[2], float scale) const {
+  AMMON_DEV void put(uint32_t c, const u32x4 (&x)[2], const u32x4 (&w)[2]) const {
     float h[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = __uint_as_float(x[e / 4][e % 4]);
@@ -156,7 +163,7 @@ template <int MODE, uint32_t US> struct W4Gemv {
         const float f = p.norm_dtype == AMMON_K_F32 ? __uint_as_float(w[e / 4][e % 4])
                         : e % 2                     ? bf16_hi(w[0][e / 2])
                                                     : bf16_lo(w[0][e / 2]);
-        h[e] = f * (scale * h[e]);
+        h[e] = f * h[e];
       }
     }
     uint2 d[D];
@@ -167,35 +174,29 @@ template <int MODE, uint32_t US> struct W4Gemv {
     for (int k = 0; k < D; ++k) *(uint2 *)(at + 64 * k) = d[k];
     if (i == 0) *(float4 *)(scales + 4 * g) = make_float4(s * 0.0625f, s * 16.f, s * 4096.f, s * 1048576.f);
   }
+  // (and, for a norm, the waves' sums of squares to red [NW])
   AMMON_DEV void stage(const Staged &st, float *red) const {
     const uint32_t tid = threadIdx.x, eights = chunks * KS * U * 16;
-    float scale = 1.f;
-    if (p.norm_w) {
-      float ss = 0.f;
-#pragma unroll
-      for (int r = 0; r < R; ++r) square(st.x[r], ss);
-      for (uint32_t c = tid + R * THREADS; c < eights; c += THREADS) {
-        u32x4 v[2];
-        load_x(c, v);
-        square(v, ss);
-      }
-      ss = wave_sum(ss);
-      if (lane == 0) red[threadIdx.x >> 6] = ss;
-      __syncthreads();
-      ss = red[0];
-#pragma unroll
-      for (uint32_t w = 1; w < KS * US; ++w) ss += red[w];
-      scale = 1.0f / sqrtf(ss / (float)p.n + p.eps);
-    }
+    float ss = 0.f;
     // (a block's 16 lanes go together: eights and the stride are multiples of 16)
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (tid + r * THREADS < eights) put(tid + r * THREADS, st.x[r], st.w[r], scale);
+      if (tid + r * THREADS < eights) {
+        if (p.norm_w) square(st.x[r], ss);
+        put(tid + r * THREADS, st.x[r], st.w[r]);
+      }
     for (uint32_t c = tid + R * THREADS; c < eights; c += THREADS) {
       u32x4 v[2], w[2];
       load_x(c, v);
-      if (p.norm_w) load_w(c, w);
-      put(c, v, w, scale);
+      if (p.norm_w) {
+        load_w(c, w);
+        square(v, ss);
+      }
+      put(c, v, w);
+    }
+    if (p.norm_w) {
+      ss = wave_sum(ss);
+      if (lane == 0) red[threadIdx.x >> 6] = ss;
     }
   }
 
@@ -205,7 +206,7 @@ template <int MODE, uint32_t US> struct W4Gemv {
     float v = red[r];
 #pragma unroll
     for (uint32_t w = 1; w < KS; ++w) v += red[16 * w + r];
-    return v;
+    return v * factor;
   }
   AMMON_DEV void finish(uint32_t u, const float *red, uint32_t pos, float &cand_v, uint32_t &cand_i) const {
     const uint32_t e = lane;
@@ -259,7 +260,7 @@ template <int MODE, uint32_t US> struct W4Gemv {
   }
 
   AMMON_DEV void run(const ammon_k_gemv &params, uint32_t nwg, uint8_t *lds) {
-    __shared__ float red[2][US][KS][16];
+    __shared__ float red[2][US][KS][16], squares[NW];
     p = params;
     lane = threadIdx.x & 63;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -290,8 +291,15 @@ template <int MODE, uint32_t US> struct W4Gemv {
     Buffer b0, b1;
     request(b0);
     if (total > 1) request(b1);
-    stage(st, &red[0][0][0][0]);
+    stage(st, squares);
     __syncthreads();
+    factor = 1.f;
+    if (p.norm_w) {
+      float ss = squares[0];
+#pragma unroll
+      for (uint32_t k = 1; k < NW; ++k) ss += squares[k];
+      factor = 1.0f / sqrtf(ss / (float)p.n + p.eps);
+    }
     float cand_v = 0.f;
     uint32_t cand_i = ARGMAX_NONE;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -305,7 +313,10 @@ template <int MODE, uint32_t US> struct W4Gemv {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = group_sum16(acc[i], 4);
       if ((lane & 15) == 0) *(f32x4 *)&r[wave][4 * (lane >> 4)] = sum;
-      __syncthreads();
+      if (KS > 1)
+        __syncthreads();
+      else
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the wave's own)
       const uint32_t u = unit_of(round);
       if (wave == round % KS && u < units) finish(u, &r[0][0], pos, cand_v, cand_i);
       acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -334,7 +345,7 @@ template <int MODE, uint32_t US> struct W4Gemv {
       if (lane == 0) sv[w] = cand_v, si[w] = cand_i;
       __syncthreads();
       if (threadIdx.x == 0) {
-        for (uint32_t k = 1; k < KS * US; ++k) cand_merge(cand_v, cand_i, sv[k], si[k]);
+        for (uint32_t k = 1; k < NW; ++k) cand_merge(cand_v, cand_i, sv[k], si[k]);
         st_out(p.cand_v + blockIdx.x, cand_v);
         st_out(p.cand_i + blockIdx.x, cand_i);
       }

@@ -88,23 +88,34 @@ template <int DIGITS> AMMON_DEV float q8_digits(const float (&x)[8], uint2 (&dig
     s = __uint_as_float((uint32_t)(k + 127) << 23);
     inv = __uint_as_float((uint32_t)(127 - k) << 23);
   }
-  uint32_t b[DIGITS][8];
+  // the digits of q as the bytes of a word: with 128 added to all but the highest they are what
+  // carries leave, and flipping those top bits takes the 128 off again
+  constexpr uint32_t BIAS = DIGITS == 4 ? 0x00808080u : DIGITS == 3 ? 0x00008080u : 0u;
+  uint32_t b[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float f = rintf(x[e] * inv);
     if (DIGITS == 1) f = fminf(fmaxf(f, -127.f), 127.f);
-    int q = bad ? 0 : (int)f;
-#pragma unroll
-    for (int p = 0; p < DIGITS; ++p) {
-      b[p][e] = (uint32_t)q & 255u;
-      q = (q + 128) >> 8;
-    }
+    const uint32_t q = bad ? 0u : (uint32_t)(int)f;
+    b[e] = (q + BIAS) ^ BIAS;
   }
+  // four words' bytes, by digit
+  auto four = [&](const uint32_t *w, uint32_t (&out)[4]) {
+    // bytes of (y : x): x 0..3, y 4..7
+    const uint32_t x01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // d0 d0' d1 d1'
+    const uint32_t x23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    out[0] = __builtin_amdgcn_perm(x23, x01, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(x23, x01, 0x07060302u);
+    const uint32_t y01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t y23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    out[2] = __builtin_amdgcn_perm(y23, y01, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(y23, y01, 0x07060302u);
+  };
+  uint32_t lo[4], hi[4];
+  four(b, lo);
+  four(b + 4, hi);
 #pragma unroll
-  for (int p = 0; p < DIGITS; ++p) {
-    digits[p].x = b[p][0] | b[p][1] << 8 | b[p][2] << 16 | b[p][3] << 24;
-    digits[p].y = b[p][4] | b[p][5] << 8 | b[p][6] << 16 | b[p][7] << 24;
-  }
+  for (int p = 0; p < DIGITS; ++p) digits[p] = make_uint2(lo[p], hi[p]);
   return bad ? __uint_as_float(W4_NAN) : s;
 }
 

@@ -76,7 +76,8 @@ struct Kernels {
   hipFunction_t w4_load = nullptr;
   hipFunction_t q8_rows[2] = {};
   hipFunction_t q8_load[2] = {};
-  hipFunction_t w4_gemv[2][kGemvModes + 1] = {};  // [sets - 1][mode], PLAIN_ARGMAX last
+  hipFunction_t w4_gemv[3][kGemvModes + 1] = {};  // [sets of 8, of 2, of 8 in workgroups of 16 waves][mode],
+                                                  // PLAIN_ARGMAX last
   hipFunction_t w4_gemm[2][kW4Tiles][kGemvModes] = {};
 };
 

@@ -207,11 +207,12 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
     R(8, name, k.q8_load[q]);
   }
-  for (int u = 0; u < 2; ++u)
+  const char *w4_sets[] = {"k8", "k2", "k8_wide"};
+  for (int i = 0; i < 3; ++i)
     for (int m = 0; m <= kGemvModes; ++m) {
       char name[96];
-      snprintf(name, sizeof name, "ammon_w4_gemv_%s_s%d", m < kGemvModes ? modes[m] : "plain_argmax", u + 1);
-      R(9, name, k.w4_gemv[u][m]);
+      snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_sets[i]);
+      R(9, name, k.w4_gemv[i][m]);
     }
   const char *w4_tiles[kW4Tiles] = {"t16", "t64"};
   for (int q = 0; q < 2; ++q)

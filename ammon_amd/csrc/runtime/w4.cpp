@@ -229,12 +229,14 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   AMMON_CHECK(!overlaps(a.x, (size_t)a.n * 4, a.y, ybytes), "%s: y overlaps x", what);
   AMMON_CHECK(!a.residual || !overlaps(a.x, (size_t)a.n * 4, a.residual, ybytes), "%s: residual overlaps x", what);
   if (a.mode == AMMON_GEMV_QKV) TRY(qkv_check(what, a.d, a.kv_dim));
-  // x's digits and scales, whole rounds of chunks
-  const uint32_t round = AMMON_W4_SET * AMMON_W4_CHUNK;
-  const size_t lds = (size_t)cdiv(cdiv(a.n, 128), round) * round * (4 * 128 + 16);
-  AMMON_CHECK(lds + 2048 <= (size_t)rt->info.max_shared_per_block,
-              "%s: reduction length n=%u needs %zu bytes of LDS; the device allows %d", what, a.n, lds + 2048,
-              rt->info.max_shared_per_block);
+  // x's digits and scales, whole rounds of a set's chunks
+  auto lds_of = [&](uint32_t ks) {
+    const uint32_t round = ks * AMMON_W4_CHUNK;
+    return (size_t)cdiv(cdiv(a.n, 128), round) * round * (4 * 128 + 16);
+  };
+  AMMON_CHECK(lds_of(8) + 4096 <= (size_t)rt->info.max_shared_per_block,
+              "%s: reduction length n=%u needs %zu bytes of LDS; the device allows %d", what, a.n,
+              lds_of(8) + 4096, rt->info.max_shared_per_block);
   ammon_k_gemv p = {};
   p.w0 = a.w0;
   p.w1 = a.w1;
@@ -261,25 +263,23 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   p.cand_v = a.cand_v;
   p.cand_i = a.cand_i;
   VALIDATE_ONLY();
-  // Two workgroups of one set per CU, which share nothing, or where x's digits are too long for
-  // that one of two sets, which share them.  One per CU where that leaves fewer of the last
-  // round's idle.
+  // Sets of 8 waves, in workgroups of one, two per CU; where x's digits leave room for one only,
+  // in workgroups of two.  A set meets at a barrier after every unit: with three rounds and more of
+  // four times as many sets of 2 they are the faster (128256 x 4096: 42.7 us, sets of 8 45.0; but
+  // 57344 x 8192, 1.75 rounds: 41.4 and 39.2, since a round's last units leave waves idle).
   const uint32_t cus = (uint32_t)std::max(rt->info.compute_units, 1);
-  const uint32_t sets = 2 * (lds + 1024) <= kLdsPerCu ? 1 : 2;
-  uint32_t grid = 0;
-  double best = 0;
-  for (uint32_t per_cu = sets == 1 ? 2 : 1; per_cu >= 1; --per_cu) {
-    uint32_t g = std::min(cdiv(p.row_blocks, sets), cus * per_cu);
-    if (a.mode == AMMON_GEMV_PLAIN_ARGMAX) g = std::min(g, a.cand_cap);
-    const double busy = p.row_blocks / ((double)g * sets * cdiv(p.row_blocks, g * sets));
-    if (busy > best + 1e-9) best = busy, grid = g;
-  }
+  const bool wide = 2 * (lds_of(8) + 4096) > kLdsPerCu;
+  const bool pairs = !wide && p.row_blocks >= 3 * 8 * cus;
+  const uint32_t sets = wide ? 2 : pairs ? 4 : 1;
+  uint32_t grid = std::min(cdiv(p.row_blocks, sets), cus * (wide ? 1 : 2));
+  if (a.mode == AMMON_GEMV_PLAIN_ARGMAX) grid = std::min(grid, a.cand_cap);
   if (grid_out) *grid_out = grid;
   DeviceGuard guard(rt->device);
   void *args[] = {&p, &grid};
   const hipError_t e =
-      hipModuleLaunchKernel(rt->k.w4_gemv[sets - 1][a.mode], grid, 1, 1, 64 * AMMON_W4_SET * sets, 1, 1,
-                            (uint32_t)lds, stream ? (hipStream_t)stream : rt->stream, args, nullptr);
+      hipModuleLaunchKernel(rt->k.w4_gemv[wide ? 2 : pairs][a.mode], grid, 1, 1, wide ? 1024 : 512, 1, 1,
+                            (uint32_t)lds_of(pairs ? 2 : 8),
+                            stream ? (hipStream_t)stream : rt->stream, args, nullptr);
   if (e != hipSuccess) return hip_error(e, what);
   return AMMON_OK;
 }
