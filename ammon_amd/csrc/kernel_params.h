@@ -120,7 +120,6 @@ typedef struct {
   void *w4;                 /* panels: kernels/w4_impl.h */
   void *out;                /* load: [d, n] fp32 or bf16 */
   uint32_t d, n, dtype;
-  uint32_t vec;             /* store: w's rows in 16-byte (bf16: 8-byte) pieces */
 } ammon_k_w4;
 
 /* Rows of digits made and read back. */
@@ -131,7 +130,7 @@ typedef struct {
   const void *w;            /* [n] RMSNorm weight or NULL (no norm) */
   void *rows;               /* panels: kernels/w4_impl.h */
   uint32_t tokens, n, w_dtype;
-  uint32_t w_vec, vec;      /* w; x, residual and sum: in 16-byte (bf16: 8-byte) pieces */
+  uint32_t vec;             /* load: n a multiple of 4 */
   float eps;
 } ammon_k_q8;
 

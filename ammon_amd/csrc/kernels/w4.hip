@@ -12,12 +12,9 @@ extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_w4_store(ammon_k_w4
     const uint32_t r = blockIdx.x * 16 + row;
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (r < p.d) {
-      const size_t at = (size_t)r * p.n;
-      const void *src = p.dtype == AMMON_K_BF16 ? (const void *)((const uint16_t *)p.w + at)
-                                                : (const void *)((const float *)p.w + at);
-      w4_load8(src, p.dtype, g * 16 + i, p.n, p.vec != 0, x);
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t k = g * W4_GROUP + 8 * i + e;
+      x[e] = r < p.d && k < p.n ? load_elem(p.w, p.dtype, (size_t)r * p.n + k) : 0.f;
     }
     const uint32_t top = abs_max16(x);
     float s = bf16_to_f32(f32_to_bf16(__uint_as_float(top) / 7.0f));
@@ -92,129 +89,151 @@ AMMON_DEV double wave_sum_f64(double v) {
 
 // One workgroup a token.  h = x + residual, to sum; v = w (h / sqrt(mean(h^2) + eps)); the digits
 // of v.  The mean is a sum in 64 bits, so that its order does not show in 32: the digits are the
-// definition's to the last one.  Without w, the digits of x.
-template <int DIGITS> AMMON_DEV void q8_rows(const ammon_k_q8 &p) {
+// definition's to the last one.  Without w, the digits of x.  A row of up to 4096 R numbers is held
+// in registers, everything it needs requested at once: R = 1, 2 or 4, by its length, since registers
+// bound how many tokens a CU has in flight (2048 tokens of 4096: 32 us with R = 4).
+//
+// A panel's 16 tokens are 16 bytes each of a line, so the workgroups of a panel go to one XCD (they
+// are dealt out to the eight in turn), whose L2 makes whole lines of their stores.
+constexpr uint32_t Q8_WG = 512;
+template <int DIGITS, int R> AMMON_DEV void q8_rows(const ammon_k_q8 &p) {
 #pragma clang fp contract(off)
-  constexpr int R = 4;  // eights of a row that a thread keeps in registers
-  __shared__ double red[AMMON_WAVES];
-  const uint32_t t = blockIdx.x, tid = threadIdx.x, blocks = w4_groups(p.n), eights = blocks * 16;
-  const float *x = p.x + (size_t)t * p.n;
-  const float *res = p.residual ? p.residual + (size_t)t * p.n : nullptr;
-  float *sum = p.residual ? p.sum + (size_t)t * p.n : nullptr;
-  const bool vec = p.vec != 0;
-  auto load = [&](uint32_t c, float (&v)[8]) {
-    w4_load8(x, c, p.n, vec, v);
-    if (!res) return;
-    float r[8];
-    w4_load8(res, c, p.n, vec, r);
+  __shared__ double red[Q8_WG / 64];
+  const uint32_t tid = threadIdx.x, blocks = w4_groups(p.n), eights = blocks * 16;
+  const uint32_t q = blockIdx.x >> 3, t = ((q >> 4) * 8 + (blockIdx.x & 7)) * 16 + (q & 15);
+  if (t >= p.tokens) return;
+  const size_t row = (size_t)t * p.n;
+  const W4Row x(p.x + row, AMMON_K_F32, p.n), w(p.w, p.w_dtype, p.n);
+  const W4Row res(p.residual ? p.residual + row : p.x, AMMON_K_F32, p.residual ? p.n : 0);
+  const W4Row sum(p.residual ? p.sum + row : p.sum, AMMON_K_F32, p.residual ? p.n : 0);
+  auto add = [&](u32x4 (&v)[2], const u32x4 (&r)[2]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] + r[e];
+    for (int e = 0; e < 8; ++e)
+      v[e / 4][e % 4] = __float_as_uint(__uint_as_float(v[e / 4][e % 4]) + __uint_as_float(r[e / 4][e % 4]));
   };
-  auto keep = [&](uint32_t c, const float (&v)[8]) {
-    if (!sum) return;
-    const uint32_t k = 8 * c;
+  double ss = 0.0;
+  auto square = [&](const u32x4 (&v)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (vec && k + 4 * h < p.n) {
-        *(float4 *)(sum + k + 4 * h) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-      } else if (!vec) {
-        for (int e = 4 * h; e < 4 * h + 4; ++e)
-          if (k + e < p.n) sum[k + e] = v[e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      const double h = (double)__uint_as_float(v[e / 4][e % 4]);
+      ss = fma(h, h, ss);
     }
   };
-  float v[R][8];
+  u32x4 v[R][2], u[R][2], f[R][2];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (tid + r * AMMON_WG < eights) load(tid + r * AMMON_WG, v[r]);
+  for (int r = 0; r < R; ++r) {
+    if (r * Q8_WG >= eights) break;  // (uniform)
+    x.load(tid + r * Q8_WG, v[r]);
+    if (p.residual) res.load(tid + r * Q8_WG, u[r]);
+    if (p.w) w.load(tid + r * Q8_WG, f[r]);
+  }
   float scale = 1.f;
   if (p.w) {
-    double ss = 0.0;
-    auto add = [&](const float (&h)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fma((double)h[e], (double)h[e], ss);
-    };
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (tid + r * AMMON_WG < eights) {
-        keep(tid + r * AMMON_WG, v[r]);
-        add(v[r]);
+    for (int r = 0; r < R; ++r) {
+      if (r * Q8_WG >= eights) break;
+      if (p.residual) {
+        add(v[r], u[r]);
+        sum.store(tid + r * Q8_WG, v[r]);
       }
-    for (uint32_t c = tid + R * AMMON_WG; c < eights; c += AMMON_WG) {
-      float h[8];
-      load(c, h);
-      keep(c, h);
-      add(h);
+      square(v[r]);
+    }
+    for (uint32_t c = tid + R * Q8_WG; c < eights; c += Q8_WG) {
+      u32x4 h[2], g[2];
+      x.load(c, h);
+      if (p.residual) {
+        res.load(c, g);
+        add(h, g);
+        sum.store(c, h);
+      }
+      square(h);
     }
     ss = wave_sum_f64(ss);
     if ((tid & 63) == 0) red[tid >> 6] = ss;
     __syncthreads();
     ss = red[0];
 #pragma unroll
-    for (int w = 1; w < AMMON_WAVES; ++w) ss += red[w];
+    for (uint32_t k = 1; k < Q8_WG / 64; ++k) ss += red[k];
     scale = (float)(1.0 / sqrt(ss / (double)p.n + (double)p.eps));
   }
-  auto put = [&](uint32_t c, float (&h)[8]) {
-    if (p.w) {
-      float w[8];
-      w4_load8(p.w, p.w_dtype, c, p.n, p.w_vec != 0, w);
+  auto put = [&](uint32_t c, const u32x4 (&h)[2], const u32x4 (&g)[2]) {
+    float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = w[e] * (scale * h[e]);
+    for (int e = 0; e < 8; ++e) {
+      y[e] = __uint_as_float(h[e / 4][e % 4]);
+      if (p.w) y[e] = w.number(g, e) * (scale * y[e]);
     }
     uint2 digits[DIGITS];
-    const float s = q8_digits<DIGITS>(h, digits);
-    q8_put<DIGITS>(p.rows, blocks, t, c / 16, c & 15, digits, s);
+    const float s = q8_digits<DIGITS>(y, digits);
+    if (c < eights) q8_put<DIGITS>(p.rows, blocks, t, c / 16, c & 15, digits, s);
   };
   // (a block's 16 lanes go together: eights and the stride are multiples of 16)
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (tid + r * AMMON_WG < eights) put(tid + r * AMMON_WG, v[r]);
-  for (uint32_t c = tid + R * AMMON_WG; c < eights; c += AMMON_WG) {
-    float h[8];
+  for (int r = 0; r < R; ++r) {
+    if (r * Q8_WG >= eights) break;
+    put(tid + r * Q8_WG, v[r], f[r]);
+  }
+  for (uint32_t c = tid + R * Q8_WG; c < eights; c += Q8_WG) {
+    u32x4 h[2], g[2];
     // (with a sum, its own numbers, which this thread wrote: x may be where they went)
-    if (sum)
-      w4_load8(sum, c, p.n, vec, h);
+    if (p.residual)
+      sum.load(c, h);
     else
-      load(c, h);
-    put(c, h);
+      x.load(c, h);
+    if (p.w) w.load(c, g);
+    put(c, h, g);
   }
 }
-extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_q8_rows_1(ammon_k_q8 p) { q8_rows<1>(p); }
-extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_q8_rows_3(ammon_k_q8 p) { q8_rows<3>(p); }
+#define Q8_ROWS_KERNEL(DIGITS, R, OCC)                                                                   \
+  extern "C" __global__ __launch_bounds__(Q8_WG, OCC) void ammon_q8_rows_##DIGITS##_r##R(ammon_k_q8 p) { \
+    q8_rows<DIGITS, R>(p);                                                                               \
+  }
+Q8_ROWS_KERNEL(1, 1, 8)
+Q8_ROWS_KERNEL(1, 2, 6)
+Q8_ROWS_KERNEL(1, 4, 4)
+Q8_ROWS_KERNEL(3, 1, 8)
+Q8_ROWS_KERNEL(3, 2, 6)
+Q8_ROWS_KERNEL(3, 4, 4)
 
-// Rows back as fp32 [tokens, n]: a thread eight numbers of a row.
+// Rows back as fp32 [tokens, n]: a wave a block of a panel, a thread its piece of 32 numbers of a
+// token, as the digits lie.
 template <int DIGITS> AMMON_DEV void q8_load(const ammon_k_q8 &p) {
-  const uint32_t blocks = w4_groups(p.n), eights = (p.n + 7) / 8;
-  const uint64_t total = (uint64_t)p.tokens * eights;
-  for (uint64_t u = (uint64_t)blockIdx.x * AMMON_WG + threadIdx.x; u < total;
-       u += (uint64_t)gridDim.x * AMMON_WG) {
-    const uint32_t t = (uint32_t)(u / eights), c = (uint32_t)(u % eights), g = c / 16, i = c & 15;
-    const uint8_t *panel = (const uint8_t *)p.rows + (size_t)(t / 16) * blocks * q8_block_bytes(DIGITS);
-    const uint8_t *at = panel + (size_t)g * 2048 * DIGITS + ((i >> 1) & 1) * 1024 + (i >> 2) * 256 +
-                        (t & 15) * 16 + (i & 1) * 8;
-    const float s = ((const float *)(panel + (size_t)blocks * 2048 * DIGITS))[g * 16 + (t & 15)];
-    uint2 d[DIGITS];
+  const uint32_t blocks = w4_groups(p.n), lane = threadIdx.x & 63, tok = lane & 15, j = lane >> 4;
+  const uint64_t total = (uint64_t)((p.tokens + 15) / 16) * blocks;
+  for (uint64_t u = (uint64_t)blockIdx.x * AMMON_WAVES + threadIdx.x / 64; u < total;
+       u += (uint64_t)gridDim.x * AMMON_WAVES) {
+    const uint32_t panel = (uint32_t)(u / blocks), g = (uint32_t)(u % blocks), t = panel * 16 + tok;
+    const uint8_t *base = (const uint8_t *)p.rows + (size_t)panel * blocks * q8_block_bytes(DIGITS);
+    const uint8_t *at = base + (size_t)g * 2048 * DIGITS + lane * 16;
+    u32x4 d[DIGITS][2];
 #pragma unroll
-    for (int k = 0; k < DIGITS; ++k) d[k] = *(const uint2 *)(at + 2048 * k);
-    float v[8];
+    for (int k = 0; k < DIGITS; ++k)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int q = 0;
+      for (int h = 0; h < 2; ++h) d[k][h] = *(const u32x4 *)(at + 2048 * k + 1024 * h);
+    const float s = ((const float *)(base + (size_t)blocks * 2048 * DIGITS))[g * 16 + tok];
+    if (t >= p.tokens) continue;
+    const uint32_t first = g * W4_GROUP + 32 * j;
+    float *out = p.sum + (size_t)t * p.n + first;
 #pragma unroll
-      for (int k = DIGITS - 1; k >= 0; --k)
-        q = q * 256 + ((int)((e < 4 ? d[k].x : d[k].y) << (24 - 8 * (e & 3))) >> 24);
-      v[e] = (float)q * s;
-    }
-    float *out = p.sum + (size_t)t * p.n + 8 * c;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (p.vec && 8 * c + 4 * h < p.n) {
-        *(float4 *)(out + 4 * h) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-      } else if (!p.vec) {
-        for (int e = 4 * h; e < 4 * h + 4; ++e)
-          if (8 * c + e < p.n) out[e] = v[e];
+      for (int i = 0; i < 4; ++i) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          int q = 0;
+#pragma unroll
+          for (int k = DIGITS - 1; k >= 0; --k) q = q * 256 + ((int)(d[k][h][i] << (24 - 8 * e)) >> 24);
+          v[e] = (float)q * s;
+        }
+        const uint32_t k = 16 * h + 4 * i;
+        if (p.vec && first + k < p.n) {
+          *(f32x4a4 *)(out + k) = v;
+        } else if (!p.vec) {
+          for (uint32_t e = 0; e < 4; ++e)
+            if (first + k + e < p.n) out[k + e] = v[e];
+        }
       }
-    }
   }
 }
 extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_q8_load_1(ammon_k_q8 p) { q8_load<1>(p); }

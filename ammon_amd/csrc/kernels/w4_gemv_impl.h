@@ -105,43 +105,12 @@ template <int MODE, uint32_t KS, uint32_t NW> struct W4Gemv {
   struct Staged {
     u32x4 x[R][2], w[R][2];
   };
-  AMMON_DEV static u32x4 four(const __amdgpu_buffer_rsrc_t &r, uint32_t at, bool vec) {
-    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
-    return u32x4{__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0), __builtin_amdgcn_raw_buffer_load_b32(r, at + 4, 0, 0),
-                 __builtin_amdgcn_raw_buffer_load_b32(r, at + 8, 0, 0),
-                 __builtin_amdgcn_raw_buffer_load_b32(r, at + 12, 0, 0)};
-  }
-  // (past the end buffers read as zero)
-  AMMON_DEV void load_x(uint32_t c, u32x4 (&v)[2]) const {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.x, p.n * 4);
-    const bool vec = (p.n & 3u) == 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) v[h] = four(r, 32 * c + 16 * h, vec);
-  }
-  AMMON_DEV void load_w(uint32_t c, u32x4 (&v)[2]) const {  // bf16: v[0], raw
-    if (p.norm_dtype == AMMON_K_F32) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(p.norm_w, p.n * 4);
-      const bool vec = (p.n & 3u) == 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) v[h] = four(r, 32 * c + 16 * h, vec);
-    } else {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(p.norm_w, p.n * 2);
-      if ((p.n & 7u) == 0 && ((uintptr_t)p.norm_w & 3u) == 0) {
-        v[0] = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * c, 0, 0);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[0][e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e, 0, 0) |
-                    (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e + 2, 0, 0) << 16;
-      }
-      v[1] = u32x4{0, 0, 0, 0};
-    }
-  }
   AMMON_DEV void begin(Staged &s) const {
+    const W4Row x(p.x, AMMON_K_F32, p.n), w(p.norm_w, p.norm_dtype, p.n);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      load_x(threadIdx.x + r * THREADS, s.x[r]);
-      if (p.norm_w) load_w(threadIdx.x + r * THREADS, s.w[r]);
+      x.load(threadIdx.x + r * THREADS, s.x[r]);
+      if (p.norm_w) w.load(threadIdx.x + r * THREADS, s.w[r]);
     }
   }
   AMMON_DEV static void square(const u32x4 (&v)[2], float &ss) {
@@ -153,18 +122,13 @@ template <int MODE, uint32_t KS, uint32_t NW> struct W4Gemv {
         ss = fmaf(f, f, ss);
       }
   }
-  AMMON_DEV void put(uint32_t c, const u32x4 (&x)[2], const u32x4 (&w)[2]) const {
+  AMMON_DEV void put(uint32_t c, const u32x4 (&x)[2], const W4Row &wr, const u32x4 (&w)[2]) const {
     float h[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = __uint_as_float(x[e / 4][e % 4]);
     if (p.norm_w) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = p.norm_dtype == AMMON_K_F32 ? __uint_as_float(w[e / 4][e % 4])
-                        : e % 2                     ? bf16_hi(w[0][e / 2])
-                                                    : bf16_lo(w[0][e / 2]);
-        h[e] = f * h[e];
-      }
+      for (int e = 0; e < 8; ++e) h[e] = wr.number(w, e) * h[e];
     }
     uint2 d[D];
     const float s = q8_digits<D>(h, d);
@@ -177,22 +141,23 @@ template <int MODE, uint32_t KS, uint32_t NW> struct W4Gemv {
   // (and, for a norm, the waves' sums of squares to red [NW])
   AMMON_DEV void stage(const Staged &st, float *red) const {
     const uint32_t tid = threadIdx.x, eights = chunks * KS * U * 16;
+    const W4Row xr(p.x, AMMON_K_F32, p.n), wr(p.norm_w, p.norm_dtype, p.n);
     float ss = 0.f;
     // (a block's 16 lanes go together: eights and the stride are multiples of 16)
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (tid + r * THREADS < eights) {
         if (p.norm_w) square(st.x[r], ss);
-        put(tid + r * THREADS, st.x[r], st.w[r]);
+        put(tid + r * THREADS, st.x[r], wr, st.w[r]);
       }
     for (uint32_t c = tid + R * THREADS; c < eights; c += THREADS) {
       u32x4 v[2], w[2];
-      load_x(c, v);
+      xr.load(c, v);
       if (p.norm_w) {
-        load_w(c, w);
+        wr.load(c, w);
         square(v, ss);
       }
-      put(c, v, w);
+      put(c, v, wr, w);
     }
     if (p.norm_w) {
       ss = wave_sum(ss);

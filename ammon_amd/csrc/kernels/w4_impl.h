@@ -119,32 +119,54 @@ template <int DIGITS> AMMON_DEV float q8_digits(const float (&x)[8], uint2 (&dig
   return bad ? __uint_as_float(W4_NAN) : s;
 }
 
-// Numbers 8 c .. + 7 of a row of n, zeros past its end.  vec: 16-byte aligned, n a multiple of 4.
-AMMON_DEV void w4_load8(const float *x, uint32_t c, uint32_t n, bool vec, float (&v)[8]) {
-  const uint32_t k = 8 * c;
-  if (vec) {
+// A row of n numbers, read and written eight at a time through a buffer resource: past its end it
+// reads as zeros and is not written, without a branch.  fp32, or bf16 as it lies (v[0]).
+struct W4Row {
+  __amdgpu_buffer_rsrc_t r;
+  bool bf16, vec;  // vec: whole 16-byte pieces
+  AMMON_DEV W4Row(const void *base, uint32_t dtype, uint32_t n) {
+    bf16 = dtype == AMMON_K_BF16;
+    r = make_rsrc(base, n * (bf16 ? 2 : 4));
+    vec = bf16 ? (n & 7u) == 0 && ((uintptr_t)base & 3u) == 0 : (n & 3u) == 0;
+  }
+  AMMON_DEV void load(uint32_t c, u32x4 (&v)[2]) const {
+    if (bf16) {
+      if (vec) {
+        v[0] = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * c, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[0][e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e, 0, 0) |
+                    (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, 16 * c + 4 * e + 2, 0, 0) << 16;
+      }
+      v[1] = u32x4{0, 0, 0, 0};
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (vec) {
+          v[h] = __builtin_amdgcn_raw_buffer_load_b128(r, 32 * c + 16 * h, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[h][e] = __builtin_amdgcn_raw_buffer_load_b32(r, 32 * c + 16 * h + 4 * e, 0, 0);
+        }
+      }
+    }
+  }
+  AMMON_DEV float number(const u32x4 (&v)[2], int e) const {
+    if (!bf16) return __uint_as_float(v[e / 4][e % 4]);
+    return e % 2 ? bf16_hi(v[0][e / 2]) : bf16_lo(v[0][e / 2]);
+  }
+  AMMON_DEV void store(uint32_t c, const u32x4 (&v)[2]) const {  // fp32
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 q = k + 4 * h < n ? ld_in4(x + k + 4 * h) : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+      if (vec) {
+        __builtin_amdgcn_raw_buffer_store_b128(v[h], r, 32 * c + 16 * h, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          __builtin_amdgcn_raw_buffer_store_b32(v[h][e], r, 32 * c + 16 * h + 4 * e, 0, 0);
+      }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = k + e < n ? ld_in(x + k + e) : 0.f;
   }
-}
-AMMON_DEV void w4_load8(const void *w, uint32_t dtype, uint32_t c, uint32_t n, bool vec, float (&v)[8]) {
-  if (dtype == AMMON_K_F32) return w4_load8((const float *)w, c, n, vec, v);
-  const uint32_t k = 8 * c;
-  if (vec) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint2 q = k + 4 * h < n ? *(const uint2 *)((const uint16_t *)w + k + 4 * h) : make_uint2(0u, 0u);
-      v[4 * h] = bf16_lo(q.x), v[4 * h + 1] = bf16_hi(q.x);
-      v[4 * h + 2] = bf16_lo(q.y), v[4 * h + 3] = bf16_hi(q.y);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = k + e < n ? bf16_to_f32(((const uint16_t *)w)[k + e]) : 0.f;
-  }
-}
+};

@@ -74,7 +74,7 @@ struct Kernels {
   // 4-bit weights and rows of digits: [Q8, Q24]
   hipFunction_t w4_store = nullptr;
   hipFunction_t w4_load = nullptr;
-  hipFunction_t q8_rows[2] = {};
+  hipFunction_t q8_rows[2][3] = {};  // [..][rows of 4096, 8192 and more numbers]
   hipFunction_t q8_load[2] = {};
   hipFunction_t w4_gemv[3][kGemvModes + 1] = {};  // [sets of 8, of 2, of 8 in workgroups of 16 waves][mode],
                                                   // PLAIN_ARGMAX last

@@ -202,8 +202,10 @@ static ammon_status load_kernels(ammon_runtime *rt) {
   R(8, "ammon_w4_load", k.w4_load);
   for (int q = 0; q < 2; ++q) {
     char name[96];
-    snprintf(name, sizeof name, "ammon_q8_rows_%d", q ? 3 : 1);
-    R(8, name, k.q8_rows[q]);
+    for (int r = 0; r < 3; ++r) {
+      snprintf(name, sizeof name, "ammon_q8_rows_%d_r%d", q ? 3 : 1, 1 << r);
+      R(8, name, k.q8_rows[q][r]);
+    }
     snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
     R(8, name, k.q8_load[q]);
   }

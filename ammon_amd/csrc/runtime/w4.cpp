@@ -13,11 +13,6 @@ constexpr uint64_t kMaxWorkgroups = (1ull << 32) / kWorkgroup - 1;
 
 bool valid_digits(ammon_dtype d) { return d == AMMON_Q8 || d == AMMON_Q24; }
 
-// 16-byte (bf16: 8-byte) pieces of rows of n.
-bool pieces(const void *base, ammon_dtype dt, uint32_t n) {
-  return n % 4 == 0 && ((uintptr_t)base & (dt == AMMON_BF16 ? 7u : 15u)) == 0;
-}
-
 ammon_status shape_check(const char *what, uint32_t rows, uint32_t n) {
   AMMON_CHECK(rows > 0 && n > 0, "%s: empty shape (%u rows of %u)", what, rows, n);
   AMMON_CHECK(cdiv(rows, 16) <= kMaxWorkgroups, "%s: %u rows are too many", what, rows);
@@ -180,7 +175,7 @@ ammon_status q8_rows(ammon_runtime *rt, ammon_stream stream, const float *x, con
   AMMON_CHECK(x && out, "%s: NULL x or rows", what);
   AMMON_CHECK(valid_digits(dtype), "%s: rows are AMMON_Q8 or AMMON_Q24, not dtype %d", what, (int)dtype);
   TRY(shape_check(what, tokens, n));
-  AMMON_CHECK(tokens <= kMaxWorkgroups, "%s: %u tokens are too many", what, tokens);
+  AMMON_CHECK(tokens <= kMaxWorkgroups / 2 - 128, "%s: %u tokens are too many", what, tokens);
   TRY(aligned(what, out, "rows"));
   const size_t bytes = (size_t)tokens * n * 4, to = ammon_q8_bytes(dtype, tokens, n);
   AMMON_CHECK(!overlaps(x, bytes, out, to) && !(residual && overlaps(residual, bytes, out, to)) &&
@@ -205,10 +200,15 @@ ammon_status q8_rows(ammon_runtime *rt, ammon_stream stream, const float *x, con
   p.tokens = tokens;
   p.n = n;
   p.w_dtype = (uint32_t)w_dtype;
-  p.w_vec = w && pieces(w, w_dtype, n);
-  p.vec = pieces(x, AMMON_F32, n) && (!residual || (pieces(residual, AMMON_F32, n) && pieces(sum, AMMON_F32, n)));
   p.eps = eps;
-  return launch(rt, stream, rt->k.q8_rows[dtype == AMMON_Q24], tokens, 1, 0, p, what);
+  // (a workgroup a token, of whole panels for each of the eight XCDs)
+  DeviceGuard guard(rt->device);
+  void *args[] = {&p};
+  const hipError_t e = hipModuleLaunchKernel(
+      rt->k.q8_rows[dtype == AMMON_Q24][n <= 4096 ? 0 : n <= 8192 ? 1 : 2], cdiv(tokens, 128) * 128, 1, 1,
+      2 * kWorkgroup, 1, 1, 0, stream ? (hipStream_t)stream : rt->stream, args, nullptr);
+  if (e != hipSuccess) return hip_error(e, what);
+  return AMMON_OK;
 }
 
 }  // namespace
@@ -306,7 +306,6 @@ ammon_status ammon_w4_store(ammon_runtime *rt, ammon_stream stream, const void *
   p.d = d;
   p.n = n;
   p.dtype = (uint32_t)w_dtype;
-  p.vec = pieces(w, w_dtype, n);
   return launch(rt, stream, rt->k.w4_store, cdiv(d, 16), std::min(cdiv(n, 128), 65535u), 0, p, "w4_store");
 }
 
@@ -366,10 +365,10 @@ ammon_status ammon_q8_load(ammon_runtime *rt, ammon_stream stream, const void *r
   p.sum = out;
   p.tokens = tokens;
   p.n = n;
-  p.vec = pieces(out, AMMON_F32, n);
-  const uint64_t eights = (uint64_t)tokens * cdiv(n, 8);
+  p.vec = n % 4 == 0;
+  const uint64_t waves = (uint64_t)cdiv(tokens, 16) * cdiv(n, 128);
   return launch(rt, stream, rt->k.q8_load[dtype == AMMON_Q24],
-                (uint32_t)std::min<uint64_t>((eights + kWorkgroup - 1) / kWorkgroup, 1u << 20), 1, 0, p, "q8_load");
+                (uint32_t)std::min<uint64_t>((waves + kWaves - 1) / kWaves, 1u << 20), 1, 0, p, "q8_load");
 }
 
 ammon_status ammon_prefill_gemm_w4(ammon_runtime *rt, ammon_stream stream, const void *w, uint32_t d, uint32_t n,
