@@ -195,45 +195,44 @@ Q8_ROWS_KERNEL(3, 1, 8)
 Q8_ROWS_KERNEL(3, 2, 6)
 Q8_ROWS_KERNEL(3, 4, 4)
 
-// Rows back as fp32 [tokens, n]: a wave a block of a panel, a thread its piece of 32 numbers of a
-// token, as the digits lie.
+// Rows back as fp32 [tokens, n]: a wave a block of a panel, a piece of eight tokens at a time: lane
+// l has numbers 4 (l % 8) .. + 3 of the piece of token l / 8, so that a store is eight whole lines.
 template <int DIGITS> AMMON_DEV void q8_load(const ammon_k_q8 &p) {
-  const uint32_t blocks = w4_groups(p.n), lane = threadIdx.x & 63, tok = lane & 15, j = lane >> 4;
+  const uint32_t blocks = w4_groups(p.n), lane = threadIdx.x & 63, f = lane & 7;
   const uint64_t total = (uint64_t)((p.tokens + 15) / 16) * blocks;
   for (uint64_t u = (uint64_t)blockIdx.x * AMMON_WAVES + threadIdx.x / 64; u < total;
        u += (uint64_t)gridDim.x * AMMON_WAVES) {
-    const uint32_t panel = (uint32_t)(u / blocks), g = (uint32_t)(u % blocks), t = panel * 16 + tok;
+    const uint32_t panel = (uint32_t)(u / blocks), g = (uint32_t)(u % blocks);
     const uint8_t *base = (const uint8_t *)p.rows + (size_t)panel * blocks * q8_block_bytes(DIGITS);
-    const uint8_t *at = base + (size_t)g * 2048 * DIGITS + lane * 16;
-    u32x4 d[DIGITS][2];
+    const uint8_t *at = base + (size_t)g * 2048 * DIGITS + (f >> 2) * 1024 + (f & 3) * 4;
+    const float *scales = (const float *)(base + (size_t)blocks * 2048 * DIGITS) + g * 16;
+    uint32_t d[8][DIGITS];
 #pragma unroll
-    for (int k = 0; k < DIGITS; ++k)
+    for (uint32_t i = 0; i < 8; ++i)  // piece i / 2, tokens 8 (i % 2) ..
 #pragma unroll
-      for (int h = 0; h < 2; ++h) d[k][h] = *(const u32x4 *)(at + 2048 * k + 1024 * h);
-    const float s = ((const float *)(base + (size_t)blocks * 2048 * DIGITS))[g * 16 + tok];
-    if (t >= p.tokens) continue;
-    const uint32_t first = g * W4_GROUP + 32 * j;
-    float *out = p.sum + (size_t)t * p.n + first;
+      for (int k = 0; k < DIGITS; ++k)
+        d[i][k] = *(const uint32_t *)(at + 2048 * k + (i / 2) * 256 + ((i & 1) * 8 + (lane >> 3)) * 16);
+    const float s[2] = {scales[lane >> 3], scales[8 + (lane >> 3)]};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t t = panel * 16 + (i & 1) * 8 + (lane >> 3), k0 = g * W4_GROUP + (i / 2) * 32 + 4 * f;
+      f32x4 v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 v;
+      for (int e = 0; e < 4; ++e) {
+        int q = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          int q = 0;
-#pragma unroll
-          for (int k = DIGITS - 1; k >= 0; --k) q = q * 256 + ((int)(d[k][h][i] << (24 - 8 * e)) >> 24);
-          v[e] = (float)q * s;
-        }
-        const uint32_t k = 16 * h + 4 * i;
-        if (p.vec && first + k < p.n) {
-          *(f32x4a4 *)(out + k) = v;
-        } else if (!p.vec) {
-          for (uint32_t e = 0; e < 4; ++e)
-            if (first + k + e < p.n) out[k + e] = v[e];
-        }
+        for (int k = DIGITS - 1; k >= 0; --k) q = q * 256 + ((int)(d[i][k] << (24 - 8 * e)) >> 24);
+        v[e] = (float)q * s[i & 1];
       }
+      float *out = p.sum + (size_t)t * p.n + k0;
+      if (t >= p.tokens) continue;
+      if (p.vec && k0 < p.n) {
+        *(f32x4a4 *)out = v;
+      } else if (!p.vec) {
+        for (uint32_t e = 0; e < 4; ++e)
+          if (k0 + e < p.n) out[e] = v[e];
+      }
+    }
   }
 }
 extern "C" __global__ __launch_bounds__(AMMON_WG) void ammon_q8_load_1(ammon_k_q8 p) { q8_load<1>(p); }
