@@ -1,27 +1,30 @@
 // w4_prefill.hip -- kernels of w4_prefill_impl.h's tiles.
 #include "w4_prefill_impl.h"
 
-#define W4_GEMM_KERNEL(NAME, DIGITS, MODE, RT, CT, KS)                           \
-  extern "C" __global__ __launch_bounds__(AMMON_WG) void NAME(ammon_k_gemm p) { \
-    w4_gemm<DIGITS, MODE, RT, CT, KS>(p);                                        \
+#define W4_GEMM_MODES(KERNEL, DIGITS, SUFFIX, ...)                                                        \
+  KERNEL(ammon_w4_gemm_plain_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_PLAIN, __VA_ARGS__)       \
+  KERNEL(ammon_w4_gemm_residual_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_RESIDUAL, __VA_ARGS__) \
+  KERNEL(ammon_w4_gemm_swiglu_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_SWIGLU, __VA_ARGS__)     \
+  KERNEL(ammon_w4_gemm_qkv_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_QKV, __VA_ARGS__)
+
+// token panels, waves
+#define W4_SHORT_KERNEL(NAME, DIGITS, MODE, CT, SPLIT)                               \
+  extern "C" __global__ __launch_bounds__(64 * SPLIT) void NAME(ammon_k_gemm p) { \
+    w4_gemm_short<DIGITS, MODE, CT, SPLIT>(p);                                     \
   }
-#define W4_GEMM_MODES(DIGITS, SUFFIX, RT, CT, KS)                                              \
-  W4_GEMM_KERNEL(ammon_w4_gemm_plain_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_PLAIN, RT, CT, KS)       \
-  W4_GEMM_KERNEL(ammon_w4_gemm_residual_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_RESIDUAL, RT, CT, KS) \
-  W4_GEMM_KERNEL(ammon_w4_gemm_swiglu_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_SWIGLU, RT, CT, KS)     \
-  W4_GEMM_KERNEL(ammon_w4_gemm_qkv_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_QKV, RT, CT, KS)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t16, 1, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t32, 2, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16, 1, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t32, 2, 8)
 
-W4_GEMM_MODES(1, t16, 2, 1, 4)
-W4_GEMM_MODES(3, t16, 2, 1, 4)
-
-#define W4_BIG_KERNEL(NAME, DIGITS, MODE, RT, CT)                                   \
-  extern "C" __global__ __launch_bounds__(AMMON_WG, 2) void NAME(ammon_k_gemm p) { \
+// panels of rows per wave, token panels, workgroups per CU.  The long tile shares a wave's codes or the tokens' digits
+// between more products: of one digit, whose sums' scaling keeps the vector units busy, the codes
+// (2048 tokens x 28672 x 4096: 314 us, 64-token tiles 335); of three the digits (689 and 792 us).
+#define W4_BIG_KERNEL(NAME, DIGITS, MODE, RT, CT, OCC)                                \
+  extern "C" __global__ __launch_bounds__(AMMON_WG, OCC) void NAME(ammon_k_gemm p) { \
     w4_gemm_big<DIGITS, MODE, RT, CT>(p);                                          \
   }
-#define W4_BIG_MODES(DIGITS, SUFFIX, RT, CT)                                               \
-  W4_BIG_KERNEL(ammon_w4_gemm_plain_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_PLAIN, RT, CT)       \
-  W4_BIG_KERNEL(ammon_w4_gemm_residual_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_RESIDUAL, RT, CT) \
-  W4_BIG_KERNEL(ammon_w4_gemm_swiglu_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_SWIGLU, RT, CT)     \
-  W4_BIG_KERNEL(ammon_w4_gemm_qkv_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_QKV, RT, CT)
-W4_BIG_MODES(1, t64, 4, 4)
-W4_BIG_MODES(3, t64, 4, 4)
+W4_GEMM_MODES(W4_BIG_KERNEL, 1, t64, 2, 4, 3)
+W4_GEMM_MODES(W4_BIG_KERNEL, 1, long, 2, 8, 3)
+W4_GEMM_MODES(W4_BIG_KERNEL, 3, t64, 2, 4, 3)
+W4_GEMM_MODES(W4_BIG_KERNEL, 3, long, 4, 4, 2)

@@ -11,12 +11,12 @@
 #include "qkv_store.h"
 #include "w4_impl.h"
 
-// RT panels of rows per wave x CT panels of tokens; KS = 1: the four waves have panels of their
-// own, KS = 4: they split the groups of the same ones, and wave 0 adds the four sums in order.
-template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t KS> struct W4Tile {
+// RT panels of rows per wave x CT panels of tokens.  SPLIT 1: the workgroup's four waves have panels
+// of their own; otherwise it has SPLIT waves, which split the groups of the same ones.
+template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct W4Tile {
   static constexpr bool GATED = MODE == AMMON_GEMV_SWIGLU;
-  static constexpr uint32_t RO = GATED ? RT / 2 : RT;          // panels of results per wave
-  static constexpr uint32_t RW = RO * (AMMON_WAVES / KS);      // ... per workgroup
+  static constexpr uint32_t RO = GATED ? RT / 2 : RT;                    // panels of results per wave
+  static constexpr uint32_t RW = RO * (SPLIT == 1 ? AMMON_WAVES : 1);    // ... per workgroup
   static_assert(!GATED || RT % 2 == 0, "gate and up panels go together");
 
   ammon_k_gemm p;
@@ -35,11 +35,11 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t KS> struct W4
       gbeg = min(ks * p.kchunks, groups);
       gend = min(gbeg + p.kchunks, groups);
     }
-    const uint32_t first = rb * RW + (KS == 1 ? wave * RO : 0);
-    if (KS > 1) {
-      const uint32_t per = (gend - gbeg + KS - 1) / KS;
-      gbeg = min(gbeg + wave * per, gend);
-      gend = min(gbeg + per, gend);
+    const uint32_t first = rb * RW + (SPLIT == 1 ? wave * RO : 0);
+    if (SPLIT > 1) {  // as evenly as whole groups go
+      const uint32_t n = gend - gbeg, per = n / SPLIT, more = n % SPLIT;
+      gbeg += wave * per + min(wave, more);
+      gend = gbeg + per + (wave < more ? 1 : 0);
     }
     const size_t bytes = (size_t)groups * W4_PANEL_BYTES;
     const uint32_t panels = ((GATED ? p.d : p.rows) + 15) / 16;
@@ -78,125 +78,152 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t KS> struct W4
     return min(c, last) * (groups * q8_block_bytes(DIGITS)) + groups * (2048 * DIGITS);
   }
 
+  // A group's operands straight from memory.
+  struct Group {
+    u32x4 a[RT];
+    u32x2 s[RT];
+    i32x4 b[CT][DIGITS][2];
+    float sx[CT];
+  };
+  AMMON_DEV void load(uint32_t g, Group &o) const {
+#pragma unroll
+    for (uint32_t j = 0; j < RT; ++j) {
+      o.a[j] = codes(j, g);
+      o.s[j] = scales(j, g);
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < CT; ++c) {
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          o.b[c][d][h] = __builtin_bit_cast(
+              i32x4, __builtin_amdgcn_raw_buffer_load_b128(x, lane * 16, digits_at(c, g, 2 * d + h), 0));
+      o.sx[c] = __uint_as_float(
+          __builtin_amdgcn_raw_buffer_load_b32(x, (lane & 15) * 4, scales_at(c) + g * 64, 0));
+    }
+  }
+  AMMON_DEV void multiply(const Group &o, f32x4 (&acc)[RT][CT]) const {
+#pragma unroll
+    for (uint32_t j = 0; j < RT; ++j) {
+      const i32x4 lo = w4_half0(o.a[j]), hi = w4_half1(o.a[j]);
+      const float sw[4] = {bf16_lo(o.s[j][0]), bf16_hi(o.s[j][0]), bf16_lo(o.s[j][1]), bf16_hi(o.s[j][1])};
+#pragma unroll
+      for (uint32_t c = 0; c < CT; ++c) {
+        i32x4 t[DIGITS];
+#pragma unroll
+        for (int d = 0; d < DIGITS; ++d)
+          t[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, o.b[c][d][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DIGITS; ++d)
+          t[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, o.b[c][d][1], t[d], 0, 0, 0);
+        const float sx = o.sx[c] * 0.0625f;  // (the codes are 16 c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][c][r] = fmaf(joined(t, r), sx * sw[r], acc[j][c][r]);
+      }
+    }
+  }
+  // Row r's sums of the digits as one number (a digit's is at most 2^21: two of them fit a word).
+  AMMON_DEV static float joined(const i32x4 *t, int r) {
+    if (DIGITS == 1) return (float)t[0][r];
+    return fmaf((float)((t[DIGITS - 1][r] << 8) + t[DIGITS / 2][r]), 256.f, (float)t[0][r]);
+  }
+
   AMMON_DEV void run(f32x4 (&acc)[RT][CT]) const {
 #pragma unroll
     for (uint32_t j = 0; j < RT; ++j)
 #pragma unroll
       for (uint32_t c = 0; c < CT; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t g = gbeg; g < gend; ++g) {
-      u32x4 a[RT];
-      u32x2 s[RT];
-#pragma unroll
-      for (uint32_t j = 0; j < RT; ++j) {
-        a[j] = codes(j, g);
-        s[j] = scales(j, g);
+    if (gbeg >= gend) return;
+    const uint32_t end = gend - 1;
+    if constexpr (CT * DIGITS <= 6) {  // the next group on its way (more do not fit the registers)
+      Group o0, o1;
+      load(gbeg, o0);
+      for (uint32_t g = gbeg; g < gend; g += 2) {
+        load(min(g + 1, end), o1);
+        multiply(o0, acc);
+        if (g + 1 >= gend) break;
+        load(min(g + 2, end), o0);
+        multiply(o1, acc);
       }
-#pragma unroll
-      for (uint32_t c = 0; c < CT; ++c) {
-        i32x4 b[DIGITS][2];
-#pragma unroll
-        for (int d = 0; d < DIGITS; ++d)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            b[d][h] = __builtin_bit_cast(
-                i32x4, __builtin_amdgcn_raw_buffer_load_b128(x, lane * 16, digits_at(c, g, 2 * d + h), 0));
-        const float sx = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(x, (lane & 15) * 4,
-                                                                              scales_at(c) + g * 64, 0)) *
-                         0.0625f;  // (the codes are 16 c)
-#pragma unroll
-        for (uint32_t j = 0; j < RT; ++j) {
-          i32x4 t[DIGITS];
-#pragma unroll
-          for (int d = 0; d < DIGITS; ++d) {
-            t[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half0(a[j]), b[d][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
-            t[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w4_half1(a[j]), b[d][1], t[d], 0, 0, 0);
-          }
-          const float sw[4] = {bf16_lo(s[j][0]), bf16_hi(s[j][0]), bf16_lo(s[j][1]), bf16_hi(s[j][1])};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            // (a digit's sum is at most 2^21: two of them fit a word)
-            const float f = DIGITS == 1
-                                ? (float)t[0][r]
-                                : fmaf((float)((t[DIGITS - 1][r] << 8) + t[DIGITS / 2][r]), 256.f, (float)t[0][r]);
-            acc[j][c][r] = fmaf(f, sx * sw[r], acc[j][c][r]);
-          }
-        }
+    } else {
+      for (uint32_t g = gbeg; g < gend; ++g) {
+        Group o;
+        load(g, o);
+        multiply(o, acc);
       }
     }
   }
 
   AMMON_DEV void store(const f32x4 (&acc)[RT][CT], uint32_t ks) const {
-    const uint32_t rq = 4 * (lane >> 4);
-    const bool split = p.ksplit > 1;
 #pragma unroll
     for (uint32_t j = 0; j < RO; ++j)
 #pragma unroll
-      for (uint32_t c = 0; c < CT; ++c) {
-        const uint32_t t = tok0 + 16 * c + (lane & 15), v = 16 * panel[j] + rq;
-        if (t >= p.tokens) continue;
-        if (MODE == AMMON_GEMV_QKV && !split) {
+      for (uint32_t c = 0; c < CT; ++c) put(panel[j], c, acc[j][c], acc[j + RT - RO][c], ks);
+  }
+  // A tile's results (gated: gate and up).
+  AMMON_DEV void put(uint32_t pan, uint32_t c, const f32x4 &a, const f32x4 &up, uint32_t ks) const {
+    const uint32_t t = tok0 + 16 * c + (lane & 15), v = 16 * pan + 4 * (lane >> 4);
+    const bool split = p.ksplit > 1;
+    if (t >= p.tokens) return;
+    if (MODE == AMMON_GEMV_QKV && !split) {
 #pragma unroll
-          for (int i = 0; i < 4; i += 2)
-            if (v + i < p.rows) qkv_store_pair(p, t, v + i, acc[j][c][i], acc[j][c][i + 1]);
-          continue;
-        }
-        const uint32_t width = split ? p.rows : p.d;
-        float *y = (split ? p.ws + (size_t)ks * p.tokens * p.rows : p.y) + (size_t)t * width + v;
-        const float *res = p.residual + (size_t)t * width + v;
-        f32x4 out = acc[j][c];
-        if (GATED) {
+      for (int i = 0; i < 4; i += 2)
+        if (v + i < p.rows) qkv_store_pair(p, t, v + i, a[i], a[i + 1]);
+      return;
+    }
+    const uint32_t width = split ? p.rows : p.d;
+    float *y = (split ? p.ws + (size_t)ks * p.tokens * p.rows : p.y) + (size_t)t * width + v;
+    const float *res = p.residual + (size_t)t * width + v;
+    f32x4 out = a;
+    if (GATED) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float gate = acc[j][c][i], up = acc[j + RT - RO][c][i];
-            float f = gate * (1.0f / (1.0f + expf(-gate)));
-            out[i] = f * up;
-          }
-        }
-        const bool add = MODE == AMMON_GEMV_RESIDUAL && !split;
-        if ((width & 3u) == 0 && v < width) {
-          if (add) out = *(const f32x4a4 *)res + out;
-          *(f32x4a4 *)y = out;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (v + i < width) y[i] = add ? res[i] + out[i] : out[i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float f = a[i] * (1.0f / (1.0f + expf(-a[i])));
+        out[i] = f * up[i];
       }
+    }
+    const bool add = MODE == AMMON_GEMV_RESIDUAL && !split;
+    if (v + 3 < width) {  // (at any float: the last rows of an odd matrix go one by one)
+      if (add) out = *(const f32x4a4 *)res + out;
+      *(f32x4a4 *)y = out;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i < width) y[i] = add ? res[i] + out[i] : out[i];
+    }
   }
 };
 
-template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t KS>
-AMMON_DEV void w4_gemm(const ammon_k_gemm &p) {
-  using T = W4Tile<DIGITS, MODE, RT, CT, KS>;
-  // id = ((row-block group, reduction range), token tile, XCD), as the prefill GEMMs' grid
+// Short prompts: one panel (gated: one of each) per workgroup, its groups split over SPLIT waves,
+// whose sums meet in LDS and are added in wave order, wave c those of token panel c.
+template <int DIGITS, int MODE, uint32_t CT, uint32_t SPLIT> AMMON_DEV void w4_gemm_short(const ammon_k_gemm &p) {
+  constexpr uint32_t RT = MODE == AMMON_GEMV_SWIGLU ? 2 : 1;
+  using T = W4Tile<DIGITS, MODE, RT, CT, SPLIT>;
+  static_assert(CT <= SPLIT, "a wave a token panel");
+  __shared__ f32x4 part[SPLIT][RT][CT][64];
+  // id = (eight panels, token tile, XCD): the token tiles of a panel are adjacent on one XCD
   const uint32_t tiles = (p.tokens + 16 * CT - 1) / (16 * CT);
-  const uint32_t ksplit = p.ksplit > 1 ? p.ksplit : 1;
-  const uint32_t q = blockIdx.x >> 3;
-  const uint32_t tt = q % tiles, ks = (q / tiles) % ksplit;
-  const uint32_t rb = (q / tiles / ksplit) * 8 + (blockIdx.x & 7u);
+  const uint32_t q = blockIdx.x >> 3, tt = q % tiles, rb = (q / tiles) * 8 + (blockIdx.x & 7u);
   const uint32_t panels = ((T::GATED ? p.d : p.rows) + 15) / 16;
-  if (rb * T::RW >= panels) return;  // padding of the last group (uniform)
-  T tile(p, rb, tt, ks);
+  if (rb >= panels) return;  // padding of the last eight (uniform)
+  T tile(p, rb, tt, 0);
   f32x4 acc[RT][CT];
   tile.run(acc);
-  if constexpr (KS > 1) {
-    __shared__ f32x4 part[KS - 1][RT][CT][64];
-    if (tile.wave) {
 #pragma unroll
-      for (uint32_t j = 0; j < RT; ++j)
+  for (uint32_t j = 0; j < RT; ++j)
 #pragma unroll
-        for (uint32_t c = 0; c < CT; ++c) part[tile.wave - 1][j][c][tile.lane] = acc[j][c];
-    }
-    __syncthreads();
-    if (tile.wave) return;
+    for (uint32_t c = 0; c < CT; ++c) part[tile.wave][j][c][tile.lane] = acc[j][c];
+  __syncthreads();
+  if (tile.wave >= CT) return;
+  f32x4 sum[RT];
 #pragma unroll
-    for (uint32_t j = 0; j < RT; ++j)
+  for (uint32_t j = 0; j < RT; ++j) {
+    sum[j] = part[0][j][tile.wave][tile.lane];
 #pragma unroll
-      for (uint32_t c = 0; c < CT; ++c)
-#pragma unroll
-        for (uint32_t w = 0; w + 1 < KS; ++w) acc[j][c] += part[w][j][c][tile.lane];
+    for (uint32_t w = 1; w < SPLIT; ++w) sum[j] += part[w][j][tile.wave][tile.lane];
   }
-  tile.store(acc, ks);
+  tile.put(rb, tile.wave, sum[0], sum[RT - 1], 0);
 }
 
 // Long prompts: the same tiles with the tokens' digits staged in LDS, which the four waves share.
@@ -210,6 +237,10 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT> struct W4Big : W4Tile<
   static_assert(CT % 4 == 0, "scales' requests: four panels each");
   using T::T;
 
+  // Groups that codes are requested ahead.  They come from farther away than the digits, and a
+  // group of one digit is over sooner (28672 x 4096, 41 tokens: 26.8 us with 1, 22.9 with 2; of
+  // three digits 8% slower with 2, for the registers).
+  static constexpr uint32_t N = DIGITS == 1 ? 2 : 1;
   struct A {
     u32x4 codes[RT];
     u32x2 scales[RT];
@@ -272,13 +303,7 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT> struct W4Big : W4Tile<
         const uint32_t j = step % S * 2 + i;
         const i32x4 *u = t[step & 1][i];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // (a digit's sum is at most 2^21: two of them fit a word)
-          const float f = DIGITS == 1
-                              ? (float)u[0][r]
-                              : fmaf((float)((u[DIGITS - 1][r] << 8) + u[DIGITS / 2][r]), 256.f, (float)u[0][r]);
-          acc[j][c][r] = fmaf(f, sx[c & 1] * sw[j][r], acc[j][c][r]);
-        }
+        for (int r = 0; r < 4; ++r) acc[j][c][r] = fmaf(T::joined(u, r), sx[c & 1] * sw[j][r], acc[j][c][r]);
         // (added up here: the compiler moves it past the loop's branch else, and every tile's sums
         // wait in registers)
         asm volatile("" : "+v"(acc[j][c]));
@@ -324,22 +349,31 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT> struct W4Big : W4Tile<
 #pragma unroll
       for (uint32_t c = 0; c < CT; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (this->gbeg >= this->gend) return;
-    A a0, a1;
+    const uint32_t end = this->gend - 1;
+    A a[N + 1];
+    load(this->gbeg, a[0]);
     stage(this->gbeg, lds);
-    load(this->gbeg, a0);
-    const uint32_t last = this->gend - 1;
+    if (N == 2) load(min(this->gbeg + 1, end), a[1]);
     auto turn = [&](uint32_t g, const A &now, A &next, uint32_t b) {
-      wait_vmcnt<0>();
-      __syncthreads();  // group g has landed; the other buffer is consumed
+      // group g's digits have landed (with N = 2, what was requested before the last codes)
+      wait_vmcnt<N == 2 ? 2 * RT : 0>();
+      __syncthreads();  // every wave's; the other buffer is consumed
       // (after the last group, that one again: no branch)
-      stage(min(g + 1, last), lds + (b ^ 1) * BYTES);
-      load(min(g + 1, last), next);
+      stage(min(g + 1, end), lds + (b ^ 1) * BYTES);
+      __builtin_amdgcn_sched_barrier(0);
+      load(min(g + N, end), next);
       __builtin_amdgcn_sched_barrier(0);
       multiply(now, lds + b * BYTES, acc);
     };
-    for (uint32_t g = this->gbeg; g < this->gend; g += 2) {
-      turn(g, a0, a1, 0);
-      if (g + 1 < this->gend) turn(g + 1, a1, a0, 1);
+    for (uint32_t g = this->gbeg, b = 0;; b ^= 1) {
+      turn(g, a[0], a[N], b);
+      if (++g >= this->gend) break;
+      turn(g, a[1], a[0], b ^= 1);
+      if (++g >= this->gend) break;
+      if constexpr (N == 2) {
+        turn(g, a[2], a[1], b ^= 1);
+        if (++g >= this->gend) break;
+      }
     }
     wait_vmcnt<0>();  // (requests into LDS end with the workgroup that made them)
   }
@@ -348,13 +382,14 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT> struct W4Big : W4Tile<
 template <int DIGITS, int MODE, uint32_t RT, uint32_t CT> AMMON_DEV void w4_gemm_big(const ammon_k_gemm &p) {
   using T = W4Big<DIGITS, MODE, RT, CT>;
   __shared__ u32x4 lds[2 * T::BYTES / 16];
+  // id = (eight (row block, reduction range), token tile, XCD): the token tiles of a row block's
+  // range are adjacent on one XCD, whose L2 keeps its codes
   const uint32_t tiles = (p.tokens + 16 * CT - 1) / (16 * CT);
   const uint32_t ksplit = p.ksplit > 1 ? p.ksplit : 1;
-  const uint32_t q = blockIdx.x >> 3;
-  const uint32_t tt = q % tiles, ks = (q / tiles) % ksplit;
-  const uint32_t rb = (q / tiles / ksplit) * 8 + (blockIdx.x & 7u);
-  const uint32_t panels = ((T::GATED ? p.d : p.rows) + 15) / 16;
-  if (rb * T::RW >= panels) return;  // padding of the last group (uniform)
+  const uint32_t q = blockIdx.x >> 3, tt = q % tiles, rr = (q / tiles) * 8 + (blockIdx.x & 7u);
+  const uint32_t blocks = (((T::GATED ? p.d : p.rows) + 15) / 16 + T::RW - 1) / T::RW;
+  const uint32_t rb = rr % blocks, ks = rr / blocks;
+  if (ks >= ksplit) return;  // padding of the last eight (uniform)
   T tile(p, rb, tt, ks);
   f32x4 acc[RT][CT];
   tile.run(acc, (char *)lds);

@@ -23,8 +23,9 @@ constexpr int kAttGroups = 4;  // GMAX = 1, 2, 4, 8
 constexpr int kGemvModes = 4;
 // KV4 variants: ceil(head / 32).
 constexpr int kKv4Groups = 4;
-// W4 GEMM tiles: w4_prefill.hip's suffixes.
-constexpr int kW4Tiles = 2;
+// W4 GEMM tiles, as w4_prefill.hip has them: one panel of rows x 16, 32 tokens; 8 panels x 64
+// tokens; the long one (Q8: 8 x 128 tokens, Q24: 16 x 64).
+constexpr int kW4Tiles = 4;
 // Bytes of a KV4 row per group of 32 numbers: 16 of codes, 4 of scale and bias.
 constexpr size_t kKv4RowBytes = 20;
 

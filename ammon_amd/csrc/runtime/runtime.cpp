@@ -216,7 +216,7 @@ static ammon_status load_kernels(ammon_runtime *rt) {
       snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_sets[i]);
       R(9, name, k.w4_gemv[i][m]);
     }
-  const char *w4_tiles[kW4Tiles] = {"t16", "t64"};
+  const char *w4_tiles[kW4Tiles] = {"t16", "t32", "t64", "long"};
   for (int q = 0; q < 2; ++q)
     for (int t = 0; t < kW4Tiles; ++t)
       for (int m = 0; m < kGemvModes; ++m) {

@@ -109,15 +109,59 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
   p.seq = a.seq;
   p.kv_dtype = (uint32_t)a.kv_dtype;
   p.kv_rows = a.kv_rows;
-  const int tile = a.tokens > 16;
-  const uint32_t ct = tile ? 4 : 1, gated = a.mode == AMMON_GEMV_SWIGLU ? 2 : 1;
-  const uint32_t per = (tile ? 16 : 2) / gated;  // panels of results per workgroup
-  const uint64_t panels = cdiv(gated == 2 ? a.d : a.rows, 16);
-  const uint64_t grid = (uint64_t)cdiv(cdiv(panels, per), 8) * 8 * cdiv(a.tokens, 16 * ct);
-  AMMON_CHECK(grid <= kMaxWorkgroups, "%s: grid too large", what);
+  const bool gated = a.mode == AMMON_GEMV_SWIGLU, q24 = a.x_dtype == AMMON_Q24;
+  const uint64_t panels = cdiv(gated ? a.d : a.rows, 16);
+  // Of the tiles, the last two optionally with the reduction split into 2, 4 or 8 ranges (a
+  // workspace, no SwiGLU), the one with the least estimated time, in us: a launch takes 3.5 and a
+  // workgroup the table's time per group of 128, alone on its CU or (the big tiles) as one of
+  // several that take turns; a split adds a second launch and the sums' traffic.  Measured at
+  // 4096 x 4096, 6144 x 4096, 4096 x 14336, 5003 x 2080, 1024 x 8192, 288 x 288 and (SwiGLU)
+  // 28672 x 4096 and 5632 x 2048, 1 to 2048 tokens, both digit types, every tile and split.  E.g. of
+  // 6144 x 4096, 41 tokens of Q24: 16-token tiles 16.5 us (estimate 16.8), 32-token tiles 17.2
+  // (17.9), long tiles in eight ranges 14.9 (14.6), whole 56.
+  static const double alone[2][kW4Tiles] = {{0.042, 0.065, 0.48, 0.99}, {0.083, 0.15, 0.98, 1.65}};
+  static const double turn[2][kW4Tiles] = {{0.042, 0.065, 0.377, 0.693}, {0.083, 0.15, 0.88, 1.54}};
+  static const double swiglu[2][2] = {{0.1, 0.145}, {0.16, 0.28}};  // the first two's, two matrices
+  static const uint32_t panels_of[2][kW4Tiles] = {{1, 1, 8, 8}, {1, 1, 8, 16}};
+  static const uint32_t tokens_of[2][kW4Tiles] = {{16, 32, 64, 128}, {16, 32, 64, 64}};
+  const uint32_t groups = cdiv(a.n, 128), cus = (uint32_t)std::max(rt->info.compute_units, 1);
+  int tile = 0;
+  uint32_t ksplit = 1, per = 1;  // per: panels of results per workgroup
+  double best = 1e300;
+  for (int t = 0; t < kW4Tiles; ++t) {
+    const uint32_t pp = t >= 2 && gated ? panels_of[q24][t] / 2 : panels_of[q24][t];
+    for (uint32_t k = 1; k <= 8; k *= 2) {
+      const uint64_t sums = (uint64_t)k * a.tokens * a.rows * 4;
+      if (k > 1 && (t < 2 || gated || !a.ws || sums > a.ws_bytes || sums > (64ull << 20) || groups < 4 * k)) break;
+      // (the XCDs get row blocks' ranges in turn)
+      const uint64_t wgs = (uint64_t)cdiv((uint64_t)cdiv(panels, pp) * k, 8) * 8 * cdiv(a.tokens, tokens_of[q24][t]);
+      const uint64_t turns = (wgs + cus - 1) / cus;
+      const double group = t < 2 && gated ? swiglu[q24][t] : turns > 1 ? turn[q24][t] : alone[q24][t];
+      const double us = 3.5 + (double)turns * cdiv(groups, k) * group + (k > 1 ? 2.5 + sums / 4e6 : 0);
+      if (us < best) best = us, tile = t, ksplit = k, per = pp;
+    }
+  }
+  const uint32_t tb = tokens_of[q24][tile];
+  if (ksplit > 1) {
+    p.ws = (float *)a.ws;
+    p.ksplit = ksplit;
+    p.kchunks = cdiv(groups, ksplit);
+  }
+  const uint64_t grid = (uint64_t)cdiv((uint64_t)cdiv(panels, per) * ksplit, 8) * 8 * cdiv(a.tokens, tb);
+  AMMON_CHECK(grid * (tile < 2 ? 2 : 1) <= kMaxWorkgroups, "%s: grid too large", what);
   VALIDATE_ONLY();
-  return launch(rt, stream, rt->k.w4_gemm[a.x_dtype == AMMON_Q24][tile][a.mode], (uint32_t)grid, 1, 0, p,
-                what);
+  DeviceGuard guard(rt->device);
+  void *args[] = {&p};
+  const hipError_t e = hipModuleLaunchKernel(rt->k.w4_gemm[q24][tile][a.mode], (uint32_t)grid, 1, 1,
+                                             tile < 2 ? 512 : 256, 1, 1, 0,
+                                             stream ? (hipStream_t)stream : rt->stream, args, nullptr);
+  if (e != hipSuccess) return hip_error(e, what);
+  if (ksplit == 1) return AMMON_OK;
+  // the ranges' sums (QKV: per row pair, then the rotation and stores)
+  const bool pairs = a.mode == AMMON_GEMV_QKV;
+  const uint64_t elems = (uint64_t)a.tokens * (pairs ? a.rows / 2 : a.d);
+  return launch(rt, stream, pairs ? rt->k.gemm_reduce_qkv : rt->k.gemm_reduce,
+                (uint32_t)std::min<uint64_t>((elems + kWorkgroup - 1) / kWorkgroup, cus * 4ull), 1, 0, p, what);
 }
 
 ammon_status w4_qkv(ammon_runtime *rt, ammon_stream stream, const void *x, ammon_dtype x_dtype,
