@@ -191,8 +191,8 @@ ammon_status ammon_checkpoint_probe(const char *path, ammon_llama_config *cfg, u
 ammon_status ammon_checkpoint_load(ammon_runtime *rt, const char *path, ammon_dtype w_dtype,
                                    ammon_checkpoint **out) {
   AMMON_CHECK(rt && path && out, "checkpoint_load: NULL argument");
-  AMMON_CHECK(w_dtype == AMMON_F32 || w_dtype == AMMON_BF16, "checkpoint_load: unknown dtype %d",
-              (int)w_dtype);
+  AMMON_CHECK(w_dtype == AMMON_F32 || w_dtype == AMMON_BF16 || w_dtype == AMMON_W4,
+              "checkpoint_load: unknown dtype %d", (int)w_dtype);
   ammon_checkpoint *c = new ammon_checkpoint();
   try {
     c->rt = ammon::Runtime::create(rt->device);
@@ -210,7 +210,7 @@ ammon_status ammon_checkpoint_load(ammon_runtime *rt, const char *path, ammon_dt
     const ammon_llama_config &g = c->hd.cfg;
     const uint32_t L = g.n_layers, D = g.dim, H = g.hidden, V = g.vocab;
     const uint32_t head = D / g.n_heads, kvd = head * g.n_kv_heads;
-    const bool bf = w_dtype == AMMON_BF16;
+    const bool w4 = w_dtype == AMMON_W4, bf = w_dtype == AMMON_BF16;
     const ammon::DType wt = bf ? ammon::DType::BF16 : ammon::DType::F32;
     // every tensor is checked against the 32-bit element count of a Shape
     // before anything is allocated or streamed into it
@@ -224,55 +224,79 @@ ammon_status ammon_checkpoint_load(ammon_runtime *rt, const char *path, ammon_dt
       c->bufs.push_back(ammon::Tensor::zeros(c->rt, ammon::Shape::vector((uint32_t)n), dt));
       return c->bufs.back().data();
     };
+    // `count` matrices [d, n]
+    auto matrices = [&](uint32_t count, uint32_t d, uint32_t n) -> void * {
+      if (!w4) return make((uint64_t)count * d * n, wt);
+      c->bufs.push_back(ammon::Tensor::zeros(c->rt, ammon::Shape::from_dims({count, d, n}), ammon::DType::W4));
+      return c->bufs.back().data();
+    };
     ammon_llama_weights &w = c->w;
-    w.tok_emb = make((uint64_t)V * D, wt);
+    w.tok_emb = make((uint64_t)V * D, w4 ? ammon::DType::BF16 : wt);
     w.rms_att = (const float *)make((uint64_t)L * D, ammon::DType::F32);
     w.rms_ffn = (const float *)make((uint64_t)L * D, ammon::DType::F32);
     w.rms_final = (const float *)make(D, ammon::DType::F32);
-    w.wq = make((uint64_t)L * D * D, wt);
-    w.wk = make((uint64_t)L * kvd * D, wt);
-    w.wv = make((uint64_t)L * kvd * D, wt);
-    w.wo = make((uint64_t)L * D * D, wt);
-    w.w1 = make((uint64_t)L * H * D, wt);
-    w.w2 = make((uint64_t)L * D * H, wt);
-    w.w3 = make((uint64_t)L * H * D, wt);
-    w.wcls = c->hd.shared ? w.tok_emb : make((uint64_t)V * D, wt);
+    w.wq = matrices(L, D, D);
+    w.wk = matrices(L, kvd, D);
+    w.wv = matrices(L, kvd, D);
+    w.wo = matrices(L, D, D);
+    w.w1 = matrices(L, H, D);
+    w.w2 = matrices(L, D, H);
+    w.w3 = matrices(L, H, D);
+    w.wcls = c->hd.shared && !w4 ? w.tok_emb : matrices(1, V, D);
     FILE *f = file.f;
     ammon_runtime *r = c->rt.raw();
     Stager stager(r);
-    auto mat = [&](const void *dst, uint64_t n, const char *what) {
-      stager.stream(f, (void *)dst, n, bf, what);
+    // W4: a matrix at a time through an fp32 buffer (everything on one stream)
+    ammon::Tensor staged;
+    if (w4) staged = ammon::Tensor::zeros(c->rt, ammon::Shape::vector(std::max({V, H, D}) * D), ammon::DType::F32);
+    auto mat = [&](const void *dst, uint32_t count, uint32_t d, uint32_t n, const char *what) {
+      if (!w4) return stager.stream(f, (void *)dst, (uint64_t)count * d * n, bf, what);
+      for (uint32_t i = 0; i < count; ++i) {
+        stager.stream(f, staged.data(), (uint64_t)d * n, false, what);
+        ammon::check(ammon_w4_store(r, nullptr, staged.data(), AMMON_F32, d, n,
+                                    (char *)dst + i * ammon_w4_bytes(d, n)),
+                     what);
+      }
+    };
+    // the table, and a W4 classifier that shares its numbers
+    auto table = [&] {
+      const long at = std::ftell(f);
+      stager.stream(f, (void *)w.tok_emb, (uint64_t)V * D, bf || w4, "token_embedding");
+      if (!w4 || !c->hd.shared) return;
+      if (at < 0 || std::fseek(f, at, SEEK_SET) != 0)
+        throw ammon::Error(AMMON_E_VALIDATION, "checkpoint: cannot read the embedding table again");
+      mat(w.wcls, 1, V, D, "token_embedding");
     };
     auto vec = [&](const void *dst, uint64_t n, const char *what) {
       stager.stream(f, (void *)dst, n, false, what);
     };
     if (c->hd.format == AMMON_CHECKPOINT_LEGACY) {
-      mat(w.tok_emb, (uint64_t)V * D, "token_embedding");
+      table();
       vec(w.rms_att, (uint64_t)L * D, "rms_att");
-      mat(w.wq, (uint64_t)L * D * D, "wq");
-      mat(w.wk, (uint64_t)L * kvd * D, "wk");
-      mat(w.wv, (uint64_t)L * kvd * D, "wv");
-      mat(w.wo, (uint64_t)L * D * D, "wo");
+      mat(w.wq, L, D, D, "wq");
+      mat(w.wk, L, kvd, D, "wk");
+      mat(w.wv, L, kvd, D, "wv");
+      mat(w.wo, L, D, D, "wo");
       vec(w.rms_ffn, (uint64_t)L * D, "rms_ffn");
-      mat(w.w1, (uint64_t)L * H * D, "w1");
-      mat(w.w2, (uint64_t)L * D * H, "w2");
-      mat(w.w3, (uint64_t)L * H * D, "w3");
+      mat(w.w1, L, H, D, "w1");
+      mat(w.w2, L, D, H, "w2");
+      mat(w.w3, L, H, D, "w3");
       vec(w.rms_final, D, "rms_final");
       skip(f, (uint64_t)g.max_seq * head * 4);  // freq_cis_real + freq_cis_imag
-      if (!c->hd.shared) mat(w.wcls, (uint64_t)V * D, "classifier");
+      if (!c->hd.shared) mat(w.wcls, 1, V, D, "classifier");
     } else {
       vec(w.rms_att, (uint64_t)L * D, "rms_att");
       vec(w.rms_ffn, (uint64_t)L * D, "rms_ffn");
       vec(w.rms_final, D, "rms_final");
-      mat(w.tok_emb, (uint64_t)V * D, "token_embedding");
-      mat(w.wq, (uint64_t)L * D * D, "wq");
-      mat(w.wk, (uint64_t)L * kvd * D, "wk");
-      mat(w.wv, (uint64_t)L * kvd * D, "wv");
-      mat(w.wo, (uint64_t)L * D * D, "wo");
-      mat(w.w1, (uint64_t)L * H * D, "w1");
-      mat(w.w2, (uint64_t)L * D * H, "w2");
-      mat(w.w3, (uint64_t)L * H * D, "w3");
-      if (!c->hd.shared) mat(w.wcls, (uint64_t)V * D, "classifier");
+      table();
+      mat(w.wq, L, D, D, "wq");
+      mat(w.wk, L, kvd, D, "wk");
+      mat(w.wv, L, kvd, D, "wv");
+      mat(w.wo, L, D, D, "wo");
+      mat(w.w1, L, H, D, "w1");
+      mat(w.w2, L, D, H, "w2");
+      mat(w.w3, L, H, D, "w3");
+      if (!c->hd.shared) mat(w.wcls, 1, V, D, "classifier");
     }
     ammon::check(ammon_stream_synchronize(r, nullptr), "checkpoint upload");
     *out = c;

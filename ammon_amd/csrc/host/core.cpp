@@ -15,11 +15,19 @@ void check(ammon_status st, const std::string &context) {
 }
 
 size_t dtype_size(DType d) {
-  if (d == DType::KV4) throw Error(AMMON_E_VALIDATION, "KV4 elements have no size of their own");
+  if (d == DType::KV4 || d == DType::W4)
+    throw Error(AMMON_E_VALIDATION, std::string(d == DType::W4 ? "W4" : "KV4") + " elements have no size of their own");
   return d == DType::BF16 ? 2 : 4;
 }
 
 size_t storage_bytes(const Shape &shape, DType dtype) {
+  if (dtype == DType::W4) {
+    const size_t r = shape.rank();
+    if (r < 2) throw Error(AMMON_E_VALIDATION, "a W4 tensor is [.., d, n], not " + shape.str());
+    size_t bytes = ammon_w4_bytes(shape.dims[r - 2], shape.dims[r - 1]);
+    for (size_t i = 0; i + 2 < r; ++i) bytes *= shape.dims[i];
+    return bytes;
+  }
   if (dtype != DType::KV4) return shape.numel() * dtype_size(dtype);
   const size_t r = shape.rank();
   if (r < 3) throw Error(AMMON_E_VALIDATION, "a KV4 tensor is [.., kv_heads, seq, head], not " + shape.str());
@@ -88,6 +96,8 @@ TensorView TensorView::narrow(size_t axis, uint32_t start, uint32_t len) const {
   }
   if (dtype_ == DType::KV4 && axis + 3 >= shape_.rank())
     throw Error(AMMON_E_VALIDATION, "narrow: a KV4 cache " + shape_.str() + " is not divisible");
+  if (dtype_ == DType::W4 && axis + 2 >= shape_.rank())
+    throw Error(AMMON_E_VALIDATION, "narrow: a W4 matrix " + shape_.str() + " is not divisible");
   Shape inner = Shape{{shape_.dims.begin() + axis + 1, shape_.dims.end()}};
   if (dtype_ == DType::KV4) inner.dims.insert(inner.dims.begin(), 1);  // (one of a stack)
   Shape s = shape_;
@@ -98,10 +108,10 @@ TensorView TensorView::narrow(size_t axis, uint32_t start, uint32_t len) const {
 TensorView TensorView::reshape(std::vector<uint32_t> dims) const {
   Shape s = Shape::from_dims(std::move(dims));
   const size_t r = shape_.rank(), t = s.rank();
-  const bool same_caches =
-      dtype_ != DType::KV4 ||
-      (r >= 3 && t >= 3 && std::equal(shape_.dims.end() - 3, shape_.dims.end(), s.dims.end() - 3));
-  if (s.numel() != numel() || !same_caches) {
+  const size_t own = dtype_ == DType::KV4 ? 3 : dtype_ == DType::W4 ? 2 : 0;  // dims that stay
+  const bool same = r >= own && t >= own &&
+                    std::equal(shape_.dims.end() - own, shape_.dims.end(), s.dims.end() - own);
+  if (s.numel() != numel() || !same) {
     throw Error(AMMON_E_VALIDATION, "cannot reshape " + shape_.str() + " to " + s.str());
   }
   return TensorView(ptr_, s, dtype_);

@@ -40,6 +40,11 @@ void expect_float(const std::string &k, const TensorView &v, const char *param) 
     fail(k + ": parameter `" + std::string(param) + "` must be f32 or bf16");
 }
 
+// A projection matrix's storage.
+void expect_matrix(const std::string &k, const TensorView &v, const char *param) {
+  if (v.dtype() != DType::W4) expect_float(k, v, param);
+}
+
 // A KV cache's storage.
 void expect_cache(const std::string &k, const TensorView &v, const char *param) {
   if (v.dtype() != DType::KV4) expect_float(k, v, param);
@@ -313,7 +318,8 @@ void greedy_lm_head(Scheme &s, const std::string &label, TensorView weight, Tens
   if (prompt.numel() < n_prompt) fail(k + ": prompt shorter than n_prompt");
   ammon_decode_step *st = (ammon_decode_step *)step.data();
   const uint32_t max_tokens = tokens.numel_u32();
-  const ammon_dtype wd = weight.dtype() == DType::BF16 ? AMMON_BF16 : AMMON_F32;
+  expect_matrix(k, weight, "weight");
+  const ammon_dtype wd = abi(weight.dtype());
   const ammon_dtype nd = norm_weight.dtype() == DType::BF16 ? AMMON_BF16 : AMMON_F32;
   const size_t scratch_bytes = scratch.nbytes();
   s.record(label, [=](ammon_stream stream) {
@@ -377,7 +383,7 @@ void TensorKernels::matmul_into(Scheme &s, const std::string &label, TensorView 
                            " elements, expected `n` = " + std::to_string(n));
   if (out.numel() != d) fail(k + ": parameter `out` has " + std::to_string(out.numel()) +
                              " elements, expected `d` = " + std::to_string(d));
-  expect_float(k, a, "a");
+  expect_matrix(k, a, "a");
   expect_f32(k, b, "b");
   expect_f32(k, out, "out");
   ammon_runtime *rt = s.runtime().raw();

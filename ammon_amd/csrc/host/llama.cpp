@@ -54,6 +54,8 @@ class LlamaModel : public AutoregressiveModel {
   void record_token(Scheme &s, bool greedy = false, uint32_t n_prompt = 0);
   void ensure_decode_scheme(uint32_t n_prompt);
   void ensure_prefill(uint32_t n);
+  void prefill_layers(uint32_t n, uint32_t ctx, uint32_t split, size_t part_bytes);
+  void prefill_layers_w4(uint32_t n, uint32_t ctx, uint32_t split, size_t part_bytes);
   const float *rope_table();
   void deposit(uint32_t token, uint32_t pos, ammon_stream stream);
   void copy_step(ammon_decode_step *slot, uint32_t token, uint32_t pos, ammon_stream stream);
@@ -80,13 +82,14 @@ class LlamaModel : public AutoregressiveModel {
   // prompt prefill scratch, [capacity, width] rows
   uint32_t pf_cap_ = 0;
   Tensor pf_ids_, pf_x_, pf_xn_, pf_q_, pf_k_, pf_v_, pf_att_, pf_hb_, pf_partial_, pf_ws_;
+  Tensor pf_xq_, pf_hq_;  // W4: rows of digits, of dim or q_dim and of hidden numbers
 };
 
 DType dt(ammon_dtype d) { return (DType)d; }
 
 TensorView view(const void *base, DType d, size_t layer, std::vector<uint32_t> dims) {
   Shape s = Shape::from_dims(std::move(dims));
-  return TensorView((char *)base + layer * s.numel() * dtype_size(d), s, d);
+  return TensorView((char *)base + layer * storage_bytes(s, d), s, d);
 }
 
 AttentionOptions attention_options(const ammon_llama_config &c) {
@@ -122,7 +125,8 @@ LlamaModel::LlamaModel(const Runtime &rt, const ammon_llama_config &c, const amm
   if (!w.tok_emb || !w.rms_att || !w.rms_ffn || !w.wq || !w.wk || !w.wv || !w.wo || !w.w1 ||
       !w.w2 || !w.w3 || !w.rms_final || !w.wcls)
     throw Error(AMMON_E_VALIDATION, "llama: a weight pointer is NULL");
-  tok_emb_ = view(w.tok_emb, wd, 0, {c.vocab, c.dim});
+  // (rows are gathered from a table of numbers)
+  tok_emb_ = view(w.tok_emb, wd == DType::W4 ? DType::BF16 : wd, 0, {c.vocab, c.dim});
   rms_final_ = view(w.rms_final, DType::F32, 0, {c.dim});
   wcls_ = view(w.wcls, wd, 0, {c.vocab, c.dim});
   for (uint32_t l = 0; l < c.n_layers; ++l) {
@@ -296,6 +300,13 @@ void LlamaModel::ensure_prefill(uint32_t n) {
   pf_ids_ = Tensor::zeros(rt_, Shape::vector(cap), DType::I32);
   pf_x_ = Tensor::zeros(rt_, Shape::from_dims({cap, c_.dim}), DType::F32);
   pf_xn_ = Tensor::zeros(rt_, Shape::from_dims({cap, c_.dim}), DType::F32);
+  if (c_.w_dtype == AMMON_W4) {
+    auto digits = [&](uint32_t width) {
+      return Tensor::zeros(rt_, Shape::vector((uint32_t)(ammon_q8_bytes(AMMON_Q24, cap, width) / 4)), DType::F32);
+    };
+    pf_xq_ = digits(std::max(c_.dim, q_dim_));
+    pf_hq_ = digits(c_.hidden);
+  }
   pf_q_ = Tensor::zeros(rt_, Shape::from_dims({cap, q_dim_}), DType::F32);
   if (c_.kv_dtype == AMMON_KV4) {  // rows for the cache
     pf_k_ = Tensor::zeros(rt_, Shape::from_dims({cap, kv_dim_}), DType::F32);
@@ -311,44 +322,14 @@ void LlamaModel::ensure_prefill(uint32_t n) {
   pf_cap_ = cap;
 }
 
-// Positions start..start+n-1 through every layer at once: embed rows, then
-// per layer rmsnorm rows, QKV GEMM (RoPE + cache stores at start + t; KV4: rows,
-// then their stores),
-// token-batched attention, wo GEMM + residual, rmsnorm rows, gate/up GEMM +
-// SwiGLU, w2 GEMM + residual; the final norm and LM head for the last row.
-void LlamaModel::prefill(const int32_t *tokens, uint32_t n, uint32_t start, float *logits) {
-  if (n == 0) throw Error(AMMON_E_VALIDATION, "prefill: no tokens");
-  if ((uint64_t)start + n > c_.max_seq)
-    throw Error(AMMON_E_VALIDATION, "prefill: start_pos + n exceeds max_seq");
-  for (uint32_t i = 0; i < n; ++i)
-    if (tokens[i] < 0 || (uint32_t)tokens[i] >= c_.vocab)
-      throw Error(AMMON_E_VALIDATION, "prefill: token " + std::to_string(tokens[i]) +
-                                          " outside the vocab");
-  ensure_prefill(n);
+// The layers of a prefill: rows x [n, dim] at positions up to ctx.
+void LlamaModel::prefill_layers(uint32_t n, uint32_t ctx, uint32_t split, size_t part_bytes) {
   ammon_runtime *rt = rt_.raw();
   ammon_stream st = stream_;
   const ammon_dtype wd = c_.w_dtype, kvd = c_.kv_dtype;
-  const uint32_t ctx = start + n;
-  // split: as many units as the device holds twice, over the context
-  const uint32_t target = 2u * (uint32_t)std::max(rt->info.compute_units, 1);
-  uint32_t split = 16;
-  while (split < AMMON_ATTENTION_MAX_SPLIT &&
-         ((uint64_t)c_.n_kv_heads * n * ammon_attention_splits(ctx, split) > target ||
-          ammon_attention_splits(ctx, split) > AMMON_ATTENTION_MAX_SPLITS))
-    split *= 2;
-  // attention partials [n][q_heads][splits over ctx][head + 2], grown on demand
-  const size_t part_bytes = ammon_attention_prefill_scratch_bytes(n, c_.n_heads, head_, ctx, split);
-  if (!pf_partial_.data() || pf_partial_.nbytes() < part_bytes)
-    pf_partial_ = Tensor::zeros(rt_, Shape::vector((uint32_t)(part_bytes / 4)), DType::F32);
   float *x = (float *)pf_x_.data(), *xn = (float *)pf_xn_.data();
   float *q = (float *)pf_q_.data(), *att = (float *)pf_att_.data(), *hb = (float *)pf_hb_.data();
   const float *table = rope_table();
-  deposit((uint32_t)tokens[0], start, st);
-  check(ammon_memcpy(rt, pf_ids_.data(), tokens, sizeof(int32_t) * n, AMMON_COPY_H2D, st),
-        "prefill ids");
-  check(ammon_embed_rows(rt, st, tok_emb_.data(), wd, c_.vocab, c_.dim,
-                         (const uint32_t *)pf_ids_.data(), n, x),
-        "prefill embed");
   const ammon_decode_step *step = (const ammon_decode_step *)step_.data();
   for (uint32_t l = 0; l < c_.n_layers; ++l) {
     const CausalAttentionBlockWeights &aw = attn_w_[l];
@@ -389,6 +370,106 @@ void LlamaModel::prefill(const int32_t *tokens, uint32_t n, uint32_t start, floa
                                 pf_ws_.data(), pf_ws_.nbytes()),
           "prefill w2");
   }
+}
+
+// ... with W4 weights, whose products take rows of digits: the norms make them (adding the block's
+// output to x as they go), the attention's and the SwiGLU's outputs are stored as such.
+void LlamaModel::prefill_layers_w4(uint32_t n, uint32_t ctx, uint32_t split, size_t part_bytes) {
+  ammon_runtime *rt = rt_.raw();
+  ammon_stream st = stream_;
+  const ammon_dtype kvd = c_.kv_dtype;
+  float *x = (float *)pf_x_.data(), *out = (float *)pf_xn_.data();
+  float *q = (float *)pf_q_.data(), *att = (float *)pf_att_.data(), *hb = (float *)pf_hb_.data();
+  void *xq = pf_xq_.data(), *hq = pf_hq_.data();
+  const float *table = rope_table();
+  const ammon_decode_step *step = (const ammon_decode_step *)step_.data();
+  auto norm = [&](bool add, const TensorView &w) {
+    check(ammon_rmsnorm_q8(rt, st, x, add ? out : nullptr, add ? x : nullptr, w.data(), AMMON_F32, c_.eps, n,
+                           c_.dim, xq, AMMON_Q24),
+          "prefill rmsnorm");
+  };
+  for (uint32_t l = 0; l < c_.n_layers; ++l) {
+    const CausalAttentionBlockWeights &aw = attn_w_[l];
+    const SwiGluBlockWeights &fw = ffn_w_[l];
+    KvLayer kv = cache_.layer(l);
+    norm(l > 0, aw.norm);
+    if (kvd == AMMON_KV4) {
+      float *kn = (float *)pf_k_.data(), *vn = (float *)pf_v_.data();
+      check(ammon_prefill_qkv_rope_w4(rt, st, xq, AMMON_Q24, n, aw.query.data(), aw.key.data(),
+                                      aw.value.data(), c_.dim, c_.n_heads, c_.n_kv_heads, head_, q, kn, vn,
+                                      c_.max_seq, step, table, pf_ws_.data(), pf_ws_.nbytes()),
+            "prefill qkv");
+      check(ammon_kv4_store(rt, st, kn, vn, n, c_.n_kv_heads, head_, kv.key.data(), kv.value.data(),
+                            c_.max_seq, step),
+            "prefill store");
+    } else {
+      check(ammon_prefill_qkv_rope_store_w4(rt, st, xq, AMMON_Q24, n, aw.query.data(), aw.key.data(),
+                                            aw.value.data(), c_.dim, c_.n_heads, c_.n_kv_heads, head_, q,
+                                            kv.key.data(), kv.value.data(), kvd, c_.max_seq, step, table,
+                                            pf_ws_.data(), pf_ws_.nbytes()),
+            "prefill qkv");
+    }
+    check(ammon_attention_prefill(rt, st, q, n, c_.n_heads, kv.key.data(), kv.value.data(), kvd,
+                                  c_.n_kv_heads, head_, c_.max_seq, step, ctx, split,
+                                  (float *)pf_partial_.data(), part_bytes, att),
+          "prefill attention");
+    check(ammon_q8_store(rt, st, att, n, q_dim_, xq, AMMON_Q24), "prefill rows");
+    check(ammon_prefill_gemm_w4(rt, st, aw.output.data(), c_.dim, q_dim_, xq, AMMON_Q24, n, out, nullptr,
+                                pf_ws_.data(), pf_ws_.nbytes()),
+          "prefill wo");
+    norm(true, fw.norm);
+    check(ammon_prefill_gate_up_swiglu_w4(rt, st, xq, AMMON_Q24, n, fw.gate.data(), fw.up.data(), c_.dim,
+                                          c_.hidden, hb),
+          "prefill gate/up");
+    check(ammon_q8_store(rt, st, hb, n, c_.hidden, hq, AMMON_Q24), "prefill rows");
+    check(ammon_prefill_gemm_w4(rt, st, fw.down.data(), c_.dim, c_.hidden, hq, AMMON_Q24, n, out, nullptr,
+                                pf_ws_.data(), pf_ws_.nbytes()),
+          "prefill w2");
+  }
+  float *last = x + (size_t)(n - 1) * c_.dim;  // the one row that is read on
+  check(ammon_add(rt, st, last, out + (size_t)(n - 1) * c_.dim, last, c_.dim), "prefill residual");
+}
+
+// Positions start..start+n-1 through every layer at once: embed rows, then
+// per layer rmsnorm rows, QKV GEMM (RoPE + cache stores at start + t; KV4: rows,
+// then their stores),
+// token-batched attention, wo GEMM + residual, rmsnorm rows, gate/up GEMM +
+// SwiGLU, w2 GEMM + residual; the final norm and LM head for the last row.
+void LlamaModel::prefill(const int32_t *tokens, uint32_t n, uint32_t start, float *logits) {
+  if (n == 0) throw Error(AMMON_E_VALIDATION, "prefill: no tokens");
+  if ((uint64_t)start + n > c_.max_seq)
+    throw Error(AMMON_E_VALIDATION, "prefill: start_pos + n exceeds max_seq");
+  for (uint32_t i = 0; i < n; ++i)
+    if (tokens[i] < 0 || (uint32_t)tokens[i] >= c_.vocab)
+      throw Error(AMMON_E_VALIDATION, "prefill: token " + std::to_string(tokens[i]) +
+                                          " outside the vocab");
+  ensure_prefill(n);
+  ammon_runtime *rt = rt_.raw();
+  ammon_stream st = stream_;
+  const ammon_dtype wd = c_.w_dtype;
+  const uint32_t ctx = start + n;
+  // split: as many units as the device holds twice, over the context
+  const uint32_t target = 2u * (uint32_t)std::max(rt->info.compute_units, 1);
+  uint32_t split = 16;
+  while (split < AMMON_ATTENTION_MAX_SPLIT &&
+         ((uint64_t)c_.n_kv_heads * n * ammon_attention_splits(ctx, split) > target ||
+          ammon_attention_splits(ctx, split) > AMMON_ATTENTION_MAX_SPLITS))
+    split *= 2;
+  // attention partials [n][q_heads][splits over ctx][head + 2], grown on demand
+  const size_t part_bytes = ammon_attention_prefill_scratch_bytes(n, c_.n_heads, head_, ctx, split);
+  if (!pf_partial_.data() || pf_partial_.nbytes() < part_bytes)
+    pf_partial_ = Tensor::zeros(rt_, Shape::vector((uint32_t)(part_bytes / 4)), DType::F32);
+  float *x = (float *)pf_x_.data();
+  deposit((uint32_t)tokens[0], start, st);
+  check(ammon_memcpy(rt, pf_ids_.data(), tokens, sizeof(int32_t) * n, AMMON_COPY_H2D, st),
+        "prefill ids");
+  check(ammon_embed_rows(rt, st, tok_emb_.data(), (ammon_dtype)tok_emb_.dtype(), c_.vocab, c_.dim,
+                         (const uint32_t *)pf_ids_.data(), n, x),
+        "prefill embed");
+  if (wd == AMMON_W4)
+    prefill_layers_w4(n, ctx, split, part_bytes);
+  else
+    prefill_layers(n, ctx, split, part_bytes);
   check(ammon_gemv_rmsnorm(rt, st, x + (size_t)(n - 1) * c_.dim, rms_final_.data(), AMMON_F32,
                            c_.eps, wcls_.data(), wd, c_.vocab, c_.dim, (float *)logits_.data()),
         "prefill lm head");

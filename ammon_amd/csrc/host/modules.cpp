@@ -255,8 +255,10 @@ void CausalAttentionBlock::record(Scheme &s, TensorView x, const CausalAttention
     // output projection that follows, from position 4096 on (measured at the
     // Llama-3-8B shape: 12-13 us per token gained at 4096 and 8000 positions,
     // 37-64 us lost at 2048 and below)
-    const void *wo = w.output.data();
-    const ammon_dtype wo_dt = abi(w.output.dtype());
+    // (W4 rows are a quarter as long, and not warmed)
+    const bool warm = w.output.dtype() != DType::W4;
+    const void *wo = warm ? w.output.data() : nullptr;
+    const ammon_dtype wo_dt = warm ? abi(w.output.dtype()) : AMMON_F32;
     s.record("attn_combine", [=](ammon_stream stream) {
       return ammon_attention_combine_warm(rt, stream, partial, q_heads, head, seq, st, split, xb,
                                           wo, wo_dt, hidden, q_heads * head, 0, 4096);

@@ -15,7 +15,7 @@ import ctypes
 import numpy as np
 
 from . import _abi
-from ._abi import BF16, F32, KV4, call
+from ._abi import BF16, F32, KV4, W4, call
 from .runtime import Runtime
 
 WEIGHT_NAMES = ("tok_emb", "rms_att", "rms_ffn", "wq", "wk", "wv", "wo", "w1", "w2", "w3",
@@ -35,7 +35,30 @@ def weight_shapes(cfg) -> dict:
 
 
 def weight_dtype(cfg, name: str) -> int:
-    return F32 if name.startswith("rms") else cfg.w_dtype
+    if name.startswith("rms"):
+        return F32
+    return BF16 if cfg.w_dtype == W4 and name == "tok_emb" else cfg.w_dtype
+
+
+def _bf16(a: np.ndarray) -> np.ndarray:
+    """fp32 numbers as bf16 bit patterns, rounded to nearest even (NaN stays NaN)."""
+    u = np.ascontiguousarray(a, np.float32).view(np.uint32)
+    r = ((u.astype(np.uint64) + 0x7fff + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where((u & 0x7fffffff) > 0x7f800000, np.uint16(0x7fc0), r)
+
+
+def upload_w4(rt: Runtime, a: np.ndarray):
+    """Matrices [.., d, n] (fp32, or bf16 bit patterns) as AMMON_W4, one after the other."""
+    a = np.ascontiguousarray(a)
+    d, n = a.shape[-2:]
+    size, dt = int(_abi.lib.ammon_w4_bytes(d, n)), BF16 if a.dtype == np.uint16 else F32
+    stack = a.reshape(-1, d, n)
+    out, staged = rt.alloc(size * len(stack)), rt.alloc(stack[0].nbytes)
+    for i, m in enumerate(stack):
+        staged.upload(m)
+        call("ammon_w4_store", rt.handle, None, staged, dt, d, n, out.offset(i * size))
+        rt.synchronize()
+    return out
 
 
 class CheckpointConfig:
@@ -110,8 +133,16 @@ class LlamaModel:
 
     @classmethod
     def from_host(cls, rt: Runtime, cfg, host_weights: dict, **kw) -> "LlamaModel":
-        """Upload host arrays (storage dtype: fp32, or bf16 bit patterns)."""
-        dev = {n: rt.upload(np.ascontiguousarray(host_weights[n])) for n in WEIGHT_NAMES}
+        """Upload host arrays (storage dtype: fp32, or bf16 bit patterns; for W4 either, quantised
+        on the device)."""
+        dev = {}
+        for name in WEIGHT_NAMES:
+            a, dt = np.ascontiguousarray(host_weights[name]), weight_dtype(cfg, name)
+            if dt == W4:
+                dev[name] = upload_w4(rt, a)
+            else:
+                to_bf16 = cfg.w_dtype == W4 and dt == BF16 and a.dtype != np.uint16
+                dev[name] = rt.upload(_bf16(a) if to_bf16 else a)
         return cls(rt, cfg, dev, **kw)
 
     @classmethod
@@ -121,6 +152,16 @@ class LlamaModel:
         for i, (name, shape) in enumerate(weight_shapes(cfg).items()):
             n = int(np.prod(shape))
             dt = weight_dtype(cfg, name)
+            if dt == W4:
+                d, m = shape[-2:]
+                size = int(_abi.lib.ammon_w4_bytes(d, m))
+                buf, numbers = rt.alloc(size * (n // (d * m))), rt.alloc(d * m * 2)
+                for j in range(n // (d * m)):  # a matrix at a time; a layer's own stream of numbers
+                    rt.fill_normal(numbers, BF16, d * m, seed, 1000 * (j + 1) + i, 0.0, std)
+                    call("ammon_w4_store", rt.handle, None, numbers, BF16, d, m, buf.offset(j * size))
+                rt.synchronize()
+                dev[name] = buf
+                continue
             buf = rt.alloc(n * (2 if dt == BF16 else 4))
             if name.startswith("rms"):
                 rt.fill(buf, F32, n, 1.0)

@@ -45,10 +45,10 @@ class Error : public std::runtime_error {
 // Throws ammon::Error with the library's message when `st` is not AMMON_OK.
 void check(ammon_status st, const std::string &context = {});
 
-// Storage dtypes.  F32 / BF16 / KV4 are the ABI's ammon_dtype values; U32 / I32
+// Storage dtypes.  F32 / BF16 / KV4 / W4 are the ABI's ammon_dtype values; U32 / I32
 // are host-layer index types (DecodeStep parcels, token ids).
-enum class DType { F32 = AMMON_F32, BF16 = AMMON_BF16, U32 = 2, I32 = 3, KV4 = AMMON_KV4 };
-// Bytes of an element; KV4 has none (throws): its rows are 20 bytes per 32 numbers.
+enum class DType { F32 = AMMON_F32, BF16 = AMMON_BF16, U32 = 2, I32 = 3, KV4 = AMMON_KV4, W4 = AMMON_W4 };
+// Bytes of an element; KV4 and W4 have none (throws): rows and panels of rows are their units.
 size_t dtype_size(DType d);
 
 // ---- runtime -----------------------------------------------------------------
@@ -84,7 +84,7 @@ struct Shape {
 };
 
 // Bytes of a contiguous tensor.  KV4 tensors are stacked caches [.., kv_heads, seq, head],
-// each at a multiple of 16 bytes.
+// each at a multiple of 16 bytes; W4 tensors stacked matrices [.., d, n].
 size_t storage_bytes(const Shape &shape, DType dtype);
 
 // Non-owning device view: pointer, shape, storage dtype.
@@ -99,10 +99,10 @@ class TensorView {
   uint32_t numel_u32() const;
   size_t nbytes() const { return storage_bytes(shape_, dtype_); }
   // Sub-range [start, start + len) along `axis` of a contiguous view
-  // (Goldy TensorView::narrow).  KV4: of whole caches only.
+  // (Goldy TensorView::narrow).  KV4: of whole caches only; W4: of whole matrices.
   TensorView narrow(size_t axis, uint32_t start, uint32_t len) const;
   // Same storage, new dims with the same element count (TensorView::reshape).
-  // KV4: the caches' own [kv_heads, seq, head] stay.
+  // KV4: the caches' own [kv_heads, seq, head] stay; W4: the matrices' [d, n].
   TensorView reshape(std::vector<uint32_t> dims) const;
 
  private:

@@ -13,7 +13,9 @@
  *     then rms_att, rms_ffn, rms_final, token_embedding, wq, wk, wv, wo, w1,
  *     w2, w3, classifier (when not shared).
  * The file is streamed through a pinned staging buffer; weights land in
- * w_dtype (bf16: round to nearest even), norm weights in fp32.
+ * w_dtype (bf16: round to nearest even; W4: quantised on the device as
+ * ammon_w4_store does, the embedding table in bf16 and a shared classifier as a
+ * W4 matrix of its own), norm weights in fp32.
  */
 #ifndef AMMON_AMMON_CHECKPOINT_H
 #define AMMON_AMMON_CHECKPOINT_H

@@ -26,7 +26,10 @@ typedef struct ammon_llama_config {
   uint32_t dim, n_layers, n_heads, n_kv_heads, hidden, vocab, max_seq;
   float theta; /* RoPE base; the reference's default is 10000 */
   float eps;   /* RMSNorm epsilon; the reference's literal is 1e-5 */
-  ammon_dtype w_dtype;  /* embedding table and projection matrices */
+  ammon_dtype w_dtype;  /* embedding table and projection matrices: AMMON_F32, AMMON_BF16, or
+                           AMMON_W4 (then the table is AMMON_BF16, each layer's matrix
+                           ammon_w4_bytes after the one before, and prompts take
+                           AMMON_Q24 rows) */
   ammon_dtype kv_dtype; /* KV cache storage: AMMON_F32, AMMON_BF16 or AMMON_KV4 */
   uint32_t use_graph;   /* replay each token as a captured HIP graph */
   uint32_t split_len;   /* attention split length; 0 picks one sized to the
@@ -35,7 +38,7 @@ typedef struct ammon_llama_config {
 } ammon_llama_config;
 
 typedef struct ammon_llama_weights {
-  const void *tok_emb;    /* [vocab, dim]                  w_dtype */
+  const void *tok_emb;    /* [vocab, dim]                  w_dtype (W4: bf16) */
   const float *rms_att;   /* [L, dim]                      fp32    */
   const float *rms_ffn;   /* [L, dim]                      fp32    */
   const void *wq;         /* [L, n_heads*head, dim]        w_dtype */

@@ -1,5 +1,8 @@
 """4-bit weights and rows of 8-bit digits without a device: sizes, refusals before a runtime is
 touched, and the numpy restatement's own properties."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -70,3 +73,20 @@ def test_rows_that_are_not_finite_or_tiny():
         assert not q[:2].any() and not q[2].any() and q[3].any()
     codes, s = w4.w4_quantise(x)
     assert np.isnan(s[0, 0]) and np.isnan(s[1, 1]) and not s[2].any() and np.isfinite(s[3]).all()
+
+
+def run_cpp(*tests):
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_bin", "w4_test")
+    if not os.path.exists(path):
+        pytest.fail(f"{path} is not built (run __graft_entry__.build())")
+    r = subprocess.run([path, *tests], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "0 failed" in r.stdout, r.stdout + r.stderr
+
+
+def test_cpp_shapes():
+    run_cpp("storage_bytes_of_w4", "views_of_w4")
+
+
+@pytest.mark.gpu
+def test_cpp_linear():
+    run_cpp("linear_over_w4")
