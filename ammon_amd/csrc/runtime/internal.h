@@ -26,6 +26,9 @@ constexpr int kKv4Groups = 4;
 // W4 GEMM tiles, as w4_prefill.hip has them: one panel of rows x 16, 32 tokens; 8 panels x 64
 // tokens; the long one (Q8: 8 x 128 tokens, Q24: 16 x 64).
 constexpr int kW4Tiles = 4;
+// W4 GEMV: sets of 8 waves with one chunk each, with more, of 2, of 8 in workgroups of 16, and waves
+// side by side
+enum { kW4One, kW4Sets, kW4Pairs, kW4Wide, kW4Flat, kW4Ways };
 // Bytes of a KV4 row per group of 32 numbers: 16 of codes, 4 of scale and bias.
 constexpr size_t kKv4RowBytes = 20;
 
@@ -77,8 +80,7 @@ struct Kernels {
   hipFunction_t w4_load = nullptr;
   hipFunction_t q8_rows[2][3] = {};  // [..][rows of 4096, 8192 and more numbers]
   hipFunction_t q8_load[2] = {};
-  hipFunction_t w4_gemv[3][kGemvModes + 1] = {};  // [sets of 8, of 2, of 8 in workgroups of 16 waves][mode],
-                                                  // PLAIN_ARGMAX last
+  hipFunction_t w4_gemv[kW4Ways][kGemvModes + 1] = {};  // [..][mode], PLAIN_ARGMAX last
   hipFunction_t w4_gemm[2][kW4Tiles][kGemvModes] = {};
 };
 

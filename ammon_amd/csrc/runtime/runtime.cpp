@@ -209,11 +209,11 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
     R(8, name, k.q8_load[q]);
   }
-  const char *w4_sets[] = {"k8", "k2", "k8_wide"};
-  for (int i = 0; i < 3; ++i)
+  const char *w4_ways[] = {"k8_one", "k8", "k2", "k8_wide", "flat"};
+  for (int i = 0; i < kW4Ways; ++i)
     for (int m = 0; m <= kGemvModes; ++m) {
       char name[96];
-      snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_sets[i]);
+      snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_ways[i]);
       R(9, name, k.w4_gemv[i][m]);
     }
   const char *w4_tiles[kW4Tiles] = {"t16", "t32", "t64", "long"};

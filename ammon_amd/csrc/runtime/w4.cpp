@@ -307,22 +307,33 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   p.cand_v = a.cand_v;
   p.cand_i = a.cand_i;
   VALIDATE_ONLY();
+  // Where a CU has between 64 and 384 groups (14336 x 4096 twice, 224: 12.3 us, as sets 14.4; 10240 x
+  // 8192, 160: 10.4 and 14.7; 4096 x 14336, 112: 8.4 and 9.6), its waves take them side by side.  With
+  // fewer the sixteen waves' own costs show (4096 x 4096, 32: 5.0 and 3.7; 6144 x 4096, 48: 5.3 and
+  // 4.8), with more the sets' order of reading, one panel after the other on the whole device (57344
+  // x 8192, 896: 41.8 and 38.4; 8192 x 28672, 448: 22.4 and 22.1).
   // Sets of 8 waves, in workgroups of one, two per CU; where x's digits leave room for one only,
   // in workgroups of two.  A set meets at a barrier after every unit: with three rounds and more of
-  // four times as many sets of 2 they are the faster (128256 x 4096: 42.7 us, sets of 8 45.0; but
+  // four times as many sets of 2 they are the faster (128256 x 4096: 40.9 us, sets of 8 45.0; but
   // 57344 x 8192, 1.75 rounds: 41.4 and 39.2, since a round's last units leave waves idle).
   const uint32_t cus = (uint32_t)std::max(rt->info.compute_units, 1);
-  const bool wide = 2 * (lds_of(8) + 4096) > kLdsPerCu;
-  const bool pairs = !wide && p.row_blocks >= 3 * 8 * cus;
-  const uint32_t sets = wide ? 2 : pairs ? 4 : 1;
-  uint32_t grid = std::min(cdiv(p.row_blocks, sets), cus * (wide ? 1 : 2));
-  if (a.mode == AMMON_GEMV_PLAIN_ARGMAX) grid = std::min(grid, a.cand_cap);
+  const uint32_t cap = a.mode == AMMON_GEMV_PLAIN_ARGMAX ? a.cand_cap : UINT32_MAX;
+  const uint64_t a_cu = (uint64_t)p.row_blocks * cdiv(a.n, 128) / cus;
+  int way = 2 * (lds_of(8) + 4096) > kLdsPerCu ? kW4Wide : p.row_blocks >= 3 * 8 * cus ? kW4Pairs : kW4Sets;
+  uint32_t grid = std::min({cdiv(p.row_blocks, way == kW4Wide ? 2 : way == kW4Pairs ? 4 : 1),
+                            cus * (way == kW4Wide ? 1 : 2), cap});
+  if (way == kW4Sets && grid == p.row_blocks && a.n <= 8 * 128 * AMMON_W4_CHUNK) way = kW4One;
+  if (p.row_blocks >= cus && a_cu >= 64 && a_cu <= 384 &&
+      cdiv(p.row_blocks, std::min(cus, cap)) <= AMMON_W4_UNITS) {
+    way = kW4Flat;
+    grid = std::min(cus, cap);
+  }
   if (grid_out) *grid_out = grid;
   DeviceGuard guard(rt->device);
-  void *args[] = {&p, &grid};
+  void *args[] = {&p.w0, &p.x, &p.norm_w, &p.n, &p.norm_dtype, &p.row_blocks, &grid, &p.w1, &p.w2, &p};
   const hipError_t e =
-      hipModuleLaunchKernel(rt->k.w4_gemv[wide ? 2 : pairs][a.mode], grid, 1, 1, wide ? 1024 : 512, 1, 1,
-                            (uint32_t)lds_of(pairs ? 2 : 8),
+      hipModuleLaunchKernel(rt->k.w4_gemv[way][a.mode], grid, 1, 1, way >= kW4Wide ? 1024 : 512, 1, 1,
+                            (uint32_t)lds_of(way == kW4Pairs ? 2 : way == kW4Flat ? 1 : 8),
                             stream ? (hipStream_t)stream : rt->stream, args, nullptr);
   if (e != hipSuccess) return hip_error(e, what);
   return AMMON_OK;

@@ -241,7 +241,10 @@ def test_rmsnorm_q8_rows_that_are_not_finite(rt):
 
 # ---- one token -----------------------------------------------------------------------------------
 GEMV = [(1, 1), (16, 128), (17, 129), (288, 288), (70, 1000), (96, 4096), (33, 14336), (4128, 512),
-        (20, 36864), (9000, 8192)]
+        (20, 36864), (9000, 8192),
+        # many groups a CU, of units that waves share: one unit and two, two groups a unit, no whole
+        # pieces of x, more of x than a workgroup keeps
+        (4100, 8300), (131072, 200), (4800, 9001), (4096, 20000)]
 
 
 @pytest.mark.parametrize("d,n", GEMV)
@@ -279,7 +282,8 @@ def norm_of(x, w, wdt):
     return np.asarray(oracle.widen(w, wdt), np.float64) * h / np.sqrt((h * h).mean(-1, keepdims=True) + EPS)
 
 
-@pytest.mark.parametrize("d,n", [(1, 1), (288, 288), (70, 1000), (200, 4096), (17, 9000), (8400, 256)])
+@pytest.mark.parametrize("d,n", [(1, 1), (288, 288), (70, 1000), (200, 4096), (17, 9000), (8400, 256),
+                                 (4100, 8300), (4800, 9001), (4096, 20000)])
 @pytest.mark.parametrize("wdt", [F32, BF16])
 def test_gemv_rmsnorm(rt, d, n, wdt):
     w, x = Weights(rt, d, n), stream(1, n)
@@ -298,7 +302,8 @@ def swiglu_of(g, u, gbar, ubar):
     return want, 1.1 * gbar * (np.abs(u) + ubar) + np.abs(s) * ubar + 6 * 2.0**-23 * np.abs(want)
 
 
-@pytest.mark.parametrize("hidden,dim", [(1, 1), (8, 128), (40, 300), (768, 288), (24, 8192), (4200, 256)])
+@pytest.mark.parametrize("hidden,dim", [(1, 1), (8, 128), (40, 300), (768, 288), (24, 8192), (4200, 256),
+                                        (2060, 8300), (7001, 1500)])
 def test_gate_up_swiglu(rt, hidden, dim):
     a, b, x = Weights(rt, hidden, dim, 1), Weights(rt, hidden, dim, 11), stream(1, dim)
     nw = (1 + 0.2 * oracle.normal(dim, 5)).astype(np.float32)
@@ -390,7 +395,7 @@ def test_qkv_rope_store(rt, heads, kv_heads, head, kvd):
         np.testing.assert_array_equal(c.download(b.shape, dt), b)
 
 
-@pytest.mark.parametrize("vocab,dim", [(1, 64), (100, 300), (9000, 256)])
+@pytest.mark.parametrize("vocab,dim", [(1, 64), (100, 300), (9000, 256), (70001, 500), (5000, 9000)])
 def test_greedy_lm_head(rt, vocab, dim):
     w, x = Weights(rt, vocab, dim), stream(1, dim)
     nw = (1 + 0.2 * oracle.normal(dim, 5)).astype(np.float32)
@@ -432,6 +437,20 @@ def test_gemv_x_of_any_size(rt, scale):
     call("ammon_gemv", rt.handle, None, w.dev, W4, 64, 512, up(rt, x), y, None)
     call("ammon_gemv", rt.handle, None, w.dev, W4, 64, 512, up(rt, x * np.float32(scale)), z, None)
     np.testing.assert_array_equal(y.download(64) * np.float32(scale), z.download(64))
+
+
+def test_qkv_rope_of_many_groups(rt):
+    """The q, k and v matrices' units shared by waves side by side: as the three products, turned."""
+    n, seq, pos, heads, kv_heads, head = 4300, 30, 7, 36, 4, 96
+    ws, x = qkv_weights(rt, heads, kv_heads, head, n), stream(1, n)
+    table = oracle.rope_table(10000.0, head, seq)
+    dims = [heads * head, kv_heads * head, kv_heads * head]
+    assert sum(dims) // 16 >= 256
+    out = [rt.alloc(d * 4) for d in dims]
+    call("ammon_qkv_rope", rt.handle, None, up(rt, x), None, F32, 0.0, *[m.dev for m in ws], W4, n, heads,
+         kv_heads, head, *out, seq, rt.step(0, pos), up(rt, table))
+    for o, d, (want, bar) in zip(out, dims, qkv_of(x.astype(np.float64), ws, table[pos:pos + 1], head, 0)):
+        close(o.download((1, d)), want, bar)
 
 
 # ---- prompts -------------------------------------------------------------------------------------
