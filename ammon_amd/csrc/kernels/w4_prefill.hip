@@ -1,21 +1,27 @@
 // w4_prefill.hip -- kernels of w4_prefill_impl.h's tiles.
 #include "w4_prefill_impl.h"
 
-#define W4_GEMM_MODES(KERNEL, DIGITS, SUFFIX, ...)                                                        \
+#define W4_GEMM_UNGATED(KERNEL, DIGITS, SUFFIX, ...)                                             \
   KERNEL(ammon_w4_gemm_plain_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_PLAIN, __VA_ARGS__)       \
   KERNEL(ammon_w4_gemm_residual_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_RESIDUAL, __VA_ARGS__) \
-  KERNEL(ammon_w4_gemm_swiglu_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_SWIGLU, __VA_ARGS__)     \
   KERNEL(ammon_w4_gemm_qkv_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_QKV, __VA_ARGS__)
+#define W4_GEMM_MODES(KERNEL, DIGITS, SUFFIX, ...)    \
+  W4_GEMM_UNGATED(KERNEL, DIGITS, SUFFIX, __VA_ARGS__) \
+  KERNEL(ammon_w4_gemm_swiglu_q##DIGITS##_##SUFFIX, DIGITS, AMMON_GEMV_SWIGLU, __VA_ARGS__)
 
-// token panels, waves
-#define W4_SHORT_KERNEL(NAME, DIGITS, MODE, CT, SPLIT)                               \
+// panels of results, token panels, waves
+#define W4_SHORT_KERNEL(NAME, DIGITS, MODE, PANELS, CT, SPLIT)                    \
   extern "C" __global__ __launch_bounds__(64 * SPLIT) void NAME(ammon_k_gemm p) { \
-    w4_gemm_short<DIGITS, MODE, CT, SPLIT>(p);                                     \
+    w4_gemm_short<DIGITS, MODE, PANELS, CT, SPLIT>(p);                            \
   }
-W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t16, 1, 8)
-W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t32, 2, 8)
-W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16, 1, 8)
-W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t32, 2, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t16, 1, 1, 8)
+W4_GEMM_UNGATED(W4_SHORT_KERNEL, 1, t16_deep, 1, 1, 16)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t16_x4, 4, 1, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 1, t32_x2, 2, 2, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16, 1, 1, 8)
+W4_GEMM_UNGATED(W4_SHORT_KERNEL, 3, t16_deep, 1, 1, 16)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16_x2, 2, 1, 8)
+W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16_x4, 4, 1, 8)
 
 // panels of rows per wave, token panels, workgroups per CU.  The long tile shares a wave's codes or the tokens' digits
 // between more products: of one digit, whose sums' scaling keeps the vector units busy, the codes

@@ -78,6 +78,11 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct
     return min(c, last) * (groups * q8_block_bytes(DIGITS)) + groups * (2048 * DIGITS);
   }
 
+  // This lane's place in a token panel's digits; past the last token, past the end (zeros, not read).
+  AMMON_DEV uint32_t token_lane(uint32_t c) const {
+    return tok0 + 16 * c + (lane & 15) < p.tokens ? lane * 16 : 0x80000000u;
+  }
+
   // A group's operands straight from memory.
   struct Group {
     u32x4 a[RT];
@@ -98,7 +103,7 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           o.b[c][d][h] = __builtin_bit_cast(
-              i32x4, __builtin_amdgcn_raw_buffer_load_b128(x, lane * 16, digits_at(c, g, 2 * d + h), 0));
+              i32x4, __builtin_amdgcn_raw_buffer_load_b128(x, token_lane(c), digits_at(c, g, 2 * d + h), 0));
       o.sx[c] = __uint_as_float(
           __builtin_amdgcn_raw_buffer_load_b32(x, (lane & 15) * 4, scales_at(c) + g * 64, 0));
     }
@@ -195,18 +200,19 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct
   }
 };
 
-// Short prompts: one panel (gated: one of each) per workgroup, its groups split over SPLIT waves,
-// whose sums meet in LDS and are added in wave order, wave c those of token panel c.
-template <int DIGITS, int MODE, uint32_t CT, uint32_t SPLIT> AMMON_DEV void w4_gemm_short(const ammon_k_gemm &p) {
-  constexpr uint32_t RT = MODE == AMMON_GEMV_SWIGLU ? 2 : 1;
+// Short prompts: PANELS panels of results (gated: of each matrix) per workgroup, their groups split
+// over SPLIT waves, whose sums meet in LDS and are added in wave order, a wave a panel and tokens'.
+template <int DIGITS, int MODE, uint32_t PANELS, uint32_t CT, uint32_t SPLIT>
+AMMON_DEV void w4_gemm_short(const ammon_k_gemm &p) {
+  constexpr uint32_t RT = MODE == AMMON_GEMV_SWIGLU ? 2 * PANELS : PANELS;
   using T = W4Tile<DIGITS, MODE, RT, CT, SPLIT>;
-  static_assert(CT <= SPLIT, "a wave a token panel");
+  static_assert(PANELS * CT <= SPLIT, "a wave a panel and tokens'");
   __shared__ f32x4 part[SPLIT][RT][CT][64];
-  // id = (eight panels, token tile, XCD): the token tiles of a panel are adjacent on one XCD
+  // id = (eight blocks of rows, token tile, XCD): the token tiles of a block are adjacent on one XCD
   const uint32_t tiles = (p.tokens + 16 * CT - 1) / (16 * CT);
   const uint32_t q = blockIdx.x >> 3, tt = q % tiles, rb = (q / tiles) * 8 + (blockIdx.x & 7u);
   const uint32_t panels = ((T::GATED ? p.d : p.rows) + 15) / 16;
-  if (rb >= panels) return;  // padding of the last eight (uniform)
+  if (rb * PANELS >= panels) return;  // padding of the last eight (uniform)
   T tile(p, rb, tt, 0);
   f32x4 acc[RT][CT];
   tile.run(acc);
@@ -215,15 +221,16 @@ template <int DIGITS, int MODE, uint32_t CT, uint32_t SPLIT> AMMON_DEV void w4_g
 #pragma unroll
     for (uint32_t c = 0; c < CT; ++c) part[tile.wave][j][c][tile.lane] = acc[j][c];
   __syncthreads();
-  if (tile.wave >= CT) return;
-  f32x4 sum[RT];
+  if (tile.wave >= PANELS * CT) return;
+  const uint32_t j = tile.wave % PANELS, c = tile.wave / PANELS;
+  f32x4 sum[2];
 #pragma unroll
-  for (uint32_t j = 0; j < RT; ++j) {
-    sum[j] = part[0][j][tile.wave][tile.lane];
+  for (uint32_t m = 0; m < RT / PANELS; ++m) {
+    sum[m] = part[0][j + m * PANELS][c][tile.lane];
 #pragma unroll
-    for (uint32_t w = 1; w < SPLIT; ++w) sum[j] += part[w][j][tile.wave][tile.lane];
+    for (uint32_t w = 1; w < SPLIT; ++w) sum[m] += part[w][j + m * PANELS][c][tile.lane];
   }
-  tile.put(rb, tile.wave, sum[0], sum[RT - 1], 0);
+  tile.put(rb * PANELS + j, c, sum[0], sum[RT / PANELS - 1], 0);
 }
 
 // Long prompts: the same tiles with the tokens' digits staged in LDS, which the four waves share.

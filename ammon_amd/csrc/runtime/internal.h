@@ -25,7 +25,7 @@ constexpr int kGemvModes = 4;
 constexpr int kKv4Groups = 4;
 // W4 GEMM tiles, as w4_prefill.hip has them: one panel of rows x 16, 32 tokens; 8 panels x 64
 // tokens; the long one (Q8: 8 x 128 tokens, Q24: 16 x 64).
-constexpr int kW4Tiles = 4;
+constexpr int kW4Tiles = 6;  // the last two are the big ones
 // W4 GEMV: sets of 8 waves with one chunk each, with more, of 2, of 8 in workgroups of 16, and waves
 // side by side
 enum { kW4One, kW4Sets, kW4Pairs, kW4Wide, kW4Flat, kW4Ways };

@@ -216,12 +216,14 @@ static ammon_status load_kernels(ammon_runtime *rt) {
       snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_ways[i]);
       R(9, name, k.w4_gemv[i][m]);
     }
-  const char *w4_tiles[kW4Tiles] = {"t16", "t32", "t64", "long"};
+  const char *w4_tiles[2][kW4Tiles] = {{"t16", "t16_deep", "t16_x4", "t32_x2", "t64", "long"},
+                                       {"t16", "t16_deep", "t16_x2", "t16_x4", "t64", "long"}};
   for (int q = 0; q < 2; ++q)
     for (int t = 0; t < kW4Tiles; ++t)
       for (int m = 0; m < kGemvModes; ++m) {
+        if (t == 1 && m == AMMON_GEMV_SWIGLU) continue;  // (none)
         char name[96];
-        snprintf(name, sizeof name, "ammon_w4_gemm_%s_q%d_%s", modes[m], q ? 3 : 1, w4_tiles[t]);
+        snprintf(name, sizeof name, "ammon_w4_gemm_%s_q%d_%s", modes[m], q ? 3 : 1, w4_tiles[q][t]);
         R(10, name, k.w4_gemm[q][t][m]);
       }
 #undef R

@@ -112,48 +112,64 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
   const bool gated = a.mode == AMMON_GEMV_SWIGLU, q24 = a.x_dtype == AMMON_Q24;
   const uint64_t panels = cdiv(gated ? a.d : a.rows, 16);
   // Of the tiles, the last two optionally with the reduction split into 2, 4 or 8 ranges (a
-  // workspace, no SwiGLU), the one with the least estimated time, in us: a launch takes 3.5 and a
-  // workgroup the table's time per group of 128, alone on its CU or (the big tiles) as one of
-  // several that take turns; a split adds a second launch and the sums' traffic.  Measured at
-  // 4096 x 4096, 6144 x 4096, 4096 x 14336, 5003 x 2080, 1024 x 8192, 288 x 288 and (SwiGLU)
-  // 28672 x 4096 and 5632 x 2048, 1 to 2048 tokens, both digit types, every tile and split.  E.g. of
-  // 6144 x 4096, 41 tokens of Q24: 16-token tiles 16.5 us (estimate 16.8), 32-token tiles 17.2
-  // (17.9), long tiles in eight ranges 14.9 (14.6), whole 56.
-  static const double alone[2][kW4Tiles] = {{0.042, 0.065, 0.48, 0.99}, {0.083, 0.15, 0.98, 1.65}};
-  static const double turn[2][kW4Tiles] = {{0.042, 0.065, 0.377, 0.693}, {0.083, 0.15, 0.88, 1.54}};
-  static const double swiglu[2][2] = {{0.1, 0.145}, {0.16, 0.28}};  // the first two's, two matrices
-  static const uint32_t panels_of[2][kW4Tiles] = {{1, 1, 8, 8}, {1, 1, 8, 16}};
-  static const uint32_t tokens_of[2][kW4Tiles] = {{16, 32, 64, 128}, {16, 32, 64, 64}};
+  // workspace, no SwiGLU), the one with the least estimated time, in us: a launch takes 3.5 (of
+  // sixteen waves 3.85); a group of 128 takes a CU's first workgroup `first` and each further one `more` (the big ones, of
+  // which several take turns, `more` each as soon as there are two); a split adds a second launch
+  // and the sums' traffic.  Fitted to 4096 x 4096, 6144 x 4096, 4096 x 14336, 10240 x 8192, 8192 x
+  // 28672, 5003 x 2080, 1024 x 8192, 128256 x 4096, 288 x 288 and (SwiGLU) 28672 x 4096, 11264 x 2048
+  // and 57344 x 8192, 1 to 2048 tokens, both digit types, every tile and split: the tile so chosen
+  // is on average 1.4% slower than the best one, and at most 22%.  E.g. of 6144 x 4096, 41 tokens of
+  // Q24: 16-token tiles 15.5 us, of two panels 13.0, of four 12.4 (estimate 13.5), long tiles in
+  // eight ranges 14.7, whole 56.
+  struct Tile {
+    uint32_t panels, tokens, waves;
+    double first, more, first_gated, more_gated;
+  };
+  static const Tile tiles[2][kW4Tiles] = {{{1, 16, 8, 0.039, 0.044, 0.082, 0.081},
+                                           {1, 16, 16, 0.035, 0.049, 0, 0},
+                                           {4, 16, 8, 0.118, 0.112, 0.312, 0.254},
+                                           {2, 32, 8, 0.094, 0.088, 0.207, 0.166},
+                                           {8, 64, 4, 0.48, 0.377, 0.48, 0.377},
+                                           {8, 128, 4, 0.99, 0.693, 0.99, 0.693}},
+                                          {{1, 16, 8, 0.070, 0.089, 0.127, 0.126},
+                                           {1, 16, 16, 0.066, 0.093, 0, 0},
+                                           {2, 16, 8, 0.106, 0.110, 0.210, 0.181},
+                                           {4, 16, 8, 0.163, 0.156, 0.361, 0.329},
+                                           {8, 64, 4, 0.98, 0.88, 0.98, 0.88},
+                                           {16, 64, 4, 1.65, 1.54, 1.65, 1.54}}};
   const uint32_t groups = cdiv(a.n, 128), cus = (uint32_t)std::max(rt->info.compute_units, 1);
-  int tile = 0;
+  const Tile *tile = nullptr;
   uint32_t ksplit = 1, per = 1;  // per: panels of results per workgroup
   double best = 1e300;
-  for (int t = 0; t < kW4Tiles; ++t) {
-    const uint32_t pp = t >= 2 && gated ? panels_of[q24][t] / 2 : panels_of[q24][t];
+  for (int i = 0; i < kW4Tiles; ++i) {
+    const Tile *t = &tiles[q24][i];
+    const bool big = i >= kW4Tiles - 2;
+    if (i == 1 && gated) continue;
+    const uint32_t pp = big && gated ? t->panels / 2 : t->panels;
     for (uint32_t k = 1; k <= 8; k *= 2) {
       const uint64_t sums = (uint64_t)k * a.tokens * a.rows * 4;
-      if (k > 1 && (t < 2 || gated || !a.ws || sums > a.ws_bytes || sums > (64ull << 20) || groups < 4 * k)) break;
+      if (k > 1 && (!big || gated || !a.ws || sums > a.ws_bytes || sums > (64ull << 20) || groups < 4 * k)) break;
       // (the XCDs get row blocks' ranges in turn)
-      const uint64_t wgs = (uint64_t)cdiv((uint64_t)cdiv(panels, pp) * k, 8) * 8 * cdiv(a.tokens, tokens_of[q24][t]);
+      const uint64_t wgs = (uint64_t)cdiv((uint64_t)cdiv(panels, pp) * k, 8) * 8 * cdiv(a.tokens, t->tokens);
       const uint64_t turns = (wgs + cus - 1) / cus;
-      const double group = t < 2 && gated ? swiglu[q24][t] : turns > 1 ? turn[q24][t] : alone[q24][t];
-      const double us = 3.5 + (double)turns * cdiv(groups, k) * group + (k > 1 ? 2.5 + sums / 4e6 : 0);
+      const double first = gated ? t->first_gated : t->first, more = gated ? t->more_gated : t->more;
+      const double group = big ? (turns > 1 ? (double)turns * more : first) : first + (double)(turns - 1) * more;
+      const double us = (t->waves == 16 ? 3.85 : 3.5) + cdiv(groups, k) * group + (k > 1 ? 2.5 + sums / 4e6 : 0);
       if (us < best) best = us, tile = t, ksplit = k, per = pp;
     }
   }
-  const uint32_t tb = tokens_of[q24][tile];
   if (ksplit > 1) {
     p.ws = (float *)a.ws;
     p.ksplit = ksplit;
     p.kchunks = cdiv(groups, ksplit);
   }
-  const uint64_t grid = (uint64_t)cdiv((uint64_t)cdiv(panels, per) * ksplit, 8) * 8 * cdiv(a.tokens, tb);
-  AMMON_CHECK(grid * (tile < 2 ? 2 : 1) <= kMaxWorkgroups, "%s: grid too large", what);
+  const uint64_t grid = (uint64_t)cdiv((uint64_t)cdiv(panels, per) * ksplit, 8) * 8 * cdiv(a.tokens, tile->tokens);
+  AMMON_CHECK(grid * (tile->waves / 4) <= kMaxWorkgroups, "%s: grid too large", what);
   VALIDATE_ONLY();
   DeviceGuard guard(rt->device);
   void *args[] = {&p};
-  const hipError_t e = hipModuleLaunchKernel(rt->k.w4_gemm[q24][tile][a.mode], (uint32_t)grid, 1, 1,
-                                             tile < 2 ? 512 : 256, 1, 1, 0,
+  const hipError_t e = hipModuleLaunchKernel(rt->k.w4_gemm[q24][tile - tiles[q24]][a.mode], (uint32_t)grid, 1, 1,
+                                             64 * tile->waves, 1, 1, 0,
                                              stream ? (hipStream_t)stream : rt->stream, args, nullptr);
   if (e != hipSuccess) return hip_error(e, what);
   if (ksplit == 1) return AMMON_OK;

@@ -462,7 +462,9 @@ def workspace(rt, rows, tokens, size=None):
 
 
 GEMM = [(1, 1, 1), (16, 128, 16), (17, 129, 3), (300, 288, 17), (70, 1000, 33), (1030, 512, 65),
-        (96, 4096, 5), (260, 300, 130), (48, 14336, 64), (512, 2080, 301), (4100, 256, 40)]
+        (96, 4096, 5), (260, 300, 130), (48, 14336, 64), (512, 2080, 301), (4100, 256, 40),
+        # 16 rows of sixteen waves; 32 and 64 rows to a workgroup, tokens of one and two panels; long tiles
+        (90, 14000, 5), (9001, 300, 37), (20000, 260, 5), (4200, 2100, 130), (3000, 1000, 600)]
 
 
 @pytest.mark.parametrize("d,n,t", GEMM)
@@ -488,7 +490,8 @@ def test_prefill_gemm(rt, d, n, t, dtype, residual, ws):
 
 
 @pytest.mark.parametrize("hidden,n,t", [(1, 1, 1), (8, 128, 16), (40, 300, 17), (768, 288, 33), (1000, 512, 70),
-                                        (24, 8192, 5), (2100, 256, 130)])
+                                        (24, 8192, 5), (2100, 256, 130), (7000, 300, 20), (3001, 900, 150),
+                                        (9000, 300, 33)])
 @pytest.mark.parametrize("dtype", [Q8, Q24])
 def test_prefill_gate_up_swiglu(rt, hidden, n, t, dtype):
     a, b = Weights(rt, hidden, n, 1), Weights(rt, hidden, n, 11)
@@ -501,6 +504,18 @@ def test_prefill_gate_up_swiglu(rt, hidden, n, t, dtype):
     close(got[:t * hidden].reshape(t, hidden),
           *swiglu_of(x.numbers @ a.numbers.T, x.numbers @ b.numbers.T, *bars))
     assert set(got[t * hidden:]) == {7.0}
+
+
+@pytest.mark.parametrize("dtype", [Q8, Q24])
+def test_prefill_qkv_rope_of_long_rows(rt, dtype):
+    n, seq, pos, t, heads, head = 13000, 30, 4, 5, 6, 48
+    ws, x = qkv_weights(rt, heads, heads, head, n), Rows(rt, stream(t, n), dtype)
+    table = oracle.rope_table(10000.0, head, seq)
+    out = [rt.alloc(t * heads * head * 4) for _ in "qkv"]
+    call("ammon_prefill_qkv_rope_w4", rt.handle, None, x.dev, dtype, t, *[m.dev for m in ws], n, heads, heads, head,
+         *out, seq, rt.step(0, pos), up(rt, table), None, 0)
+    for o, (want, bar) in zip(out, qkv_of(x.numbers, ws, table[pos:pos + t], head, None)):
+        close(o.download((t, heads * head)), want, bar)
 
 
 @pytest.mark.parametrize("t", [1, 16, 20, 70])
