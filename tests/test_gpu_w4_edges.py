@@ -189,3 +189,28 @@ def test_rows_past_4_gib(rt):
     rt.synchronize()
     assert not back[0].any()
     np.testing.assert_array_equal(back[1:], few.numbers.astype(np.float32))
+
+
+@pytest.mark.parametrize("d,n", [(20, 36864), (4112, 36864), (4096, 4096), (6144, 4096), (4096, 14336), (10240, 8192),
+                                 (70000, 1000), (9000, 8192), (300, 300)])
+def test_the_same_in_every_call(rt, d, n):
+    w, x = Weights(rt, d, n, w=matrix(64, n).repeat((d + 63) // 64, 0)[:d]), up(rt, stream(1, n))
+    ys = [rt.alloc(4 * d) for _ in range(24)]
+    for y in ys * 2:
+        call("ammon_gemv", rt.handle, None, w.dev, W4, d, n, x, y, None)
+    first = ys[0].download(d)
+    for y in ys[1:]:
+        np.testing.assert_array_equal(y.download(d), first)
+
+
+@pytest.mark.parametrize("dtype", [Q8, Q24])
+@pytest.mark.parametrize("d,n,t", [(4096, 4096, 5), (96, 14336, 5), (6144, 1024, 20), (6144, 1024, 41), (1024, 8192, 200),
+                                   (3000, 1000, 600)])
+def test_prompts_the_same_in_every_call(rt, d, n, t, dtype):
+    w, x = Weights(rt, d, n, w=matrix(64, n).repeat((d + 63) // 64, 0)[:d]), Rows(rt, stream(t, n), dtype)
+    ws, ys = workspace(rt, d, t), [rt.alloc(4 * t * d) for _ in range(8)]
+    for y in ys * 2:
+        call("ammon_prefill_gemm_w4", rt.handle, None, w.dev, d, n, x.dev, dtype, t, y, None, *ws)
+    first = ys[0].download(t * d)
+    for y in ys[1:]:
+        np.testing.assert_array_equal(y.download(t * d), first)
