@@ -135,8 +135,8 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
                                            {1, 16, 16, 0.066, 0.093, 0, 0},
                                            {2, 16, 8, 0.106, 0.110, 0.210, 0.181},
                                            {4, 16, 8, 0.163, 0.156, 0.361, 0.329},
-                                           {8, 64, 4, 0.98, 0.88, 0.98, 0.88},
-                                           {16, 64, 4, 1.65, 1.54, 1.65, 1.54}}};
+                                           {8, 64, 4, 0.93, 0.83, 0.93, 0.83},
+                                           {16, 64, 4, 1.55, 1.44, 1.55, 1.44}}};
   const uint32_t groups = cdiv(a.n, 128), cus = (uint32_t)std::max(rt->info.compute_units, 1);
   const Tile *tile = nullptr;
   uint32_t ksplit = 1, per = 1;  // per: panels of results per workgroup
