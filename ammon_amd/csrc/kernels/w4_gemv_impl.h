@@ -457,7 +457,7 @@ template <int MODE> struct W4Flat : W4Token<MODE, 16> {
     typename T::Staged st;
     T::begin(st);
     lanes();
-    // units (fewer than 64: the runtime's rule) and groups; the wave's
+    // units (at most MOST, by the launch's rule) and groups; the wave's
     const uint32_t here = (p.row_blocks - blockIdx.x + nwg - 1) / nwg, total = here * groups;
     const uint32_t from = w * total / NW, count = (w + 1) * total / NW - from;
     const uint32_t unit = w * here / NW;  // from / groups
