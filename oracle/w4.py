@@ -66,24 +66,17 @@ def w4_numbers(codes, s, n):
 def w4_pack(codes, s):
     """The bytes of codes [d, groups, 128] and scales [d, groups]."""
     d, g = s.shape
-    dp = -(-d // 16) * 16
-    c = np.zeros((dp, g, GROUP), np.int8)
-    c[:d] = codes
-    sc = np.zeros((dp, g), np.float32)
+    panels = -(-d // 16)
+    c = np.zeros((panels * 16, g, GROUP), np.uint8)
+    c[:d] = codes.astype(np.int8).view(np.uint8) & 15
+    sc = np.zeros((panels * 16, g), np.float32)
     sc[:d] = s
-    out = np.zeros((dp // 16, g * 1056), np.uint8)
-    for p in range(dp // 16):
-        for r in range(16):
-            for j in range(4):
-                piece = c[16 * p + r, :, 32 * j:32 * j + 32].astype(np.uint8) & 15
-                byte = piece[:, :16] | piece[:, 16:] << 4
-                for k in range(g):
-                    at = 1024 * k + 256 * j + 16 * r
-                    out[p, at:at + 16] = byte[k]
-            for k in range(g):
-                at = 1024 * g + 2 * (((r // 4) * g + k) * 4 + r % 4)
-                u = np.float32(sc[16 * p + r, k]).view(np.uint32) >> 16
-                out[p, at:at + 2] = [u & 255, u >> 8]
+    c = c.reshape(panels, 16, g, 4, 2, 16)  # panel, row, group, piece, half, byte
+    byte = c[..., 0, :] | c[..., 1, :] << 4
+    out = np.zeros((panels, g * 1056), np.uint8)
+    out[:, :g * 1024] = byte.transpose(0, 2, 3, 1, 4).reshape(panels, -1)
+    top = (sc.view(np.uint32) >> 16).astype("<u2").reshape(panels, 4, 4, g)
+    out[:, g * 1024:] = np.ascontiguousarray(top.transpose(0, 1, 3, 2)).view(np.uint8).reshape(panels, -1)
     return out.reshape(-1)
 
 
@@ -110,25 +103,23 @@ def q_numbers(q, s, n):
 def q_pack(q, s, digits, into=None):
     """The bytes of rows; what a panel's tokens past the last one hold is kept from `into`."""
     t, b = s.shape
-    tp = -(-t // 16) * 16
+    panels = -(-t // 16)
     size = b * (2048 * digits + 64)
-    out = (np.zeros(tp // 16 * size, np.uint8) if into is None else into.copy()).reshape(tp // 16, size)
-    scales = np.ascontiguousarray(s, np.float32)
-    for i in range(t):
-        rest = q[i].astype(np.int64)  # [blocks, 128]
-        for d in range(digits):
-            low = (rest + 128) % 256 - 128
-            rest = (rest - low) // 256
-            for h in range(2):
-                for j in range(4):
-                    piece = low[:, 32 * j + 16 * h:32 * j + 16 * h + 16].astype(np.int8).view(np.uint8)
-                    for k in range(b):
-                        at = ((k * digits + d) * 2 + h) * 1024 + 256 * j + 16 * (i % 16)
-                        out[i // 16, at:at + 16] = piece[k]
-        assert not rest.any()
-        for k in range(b):
-            at = b * 2048 * digits + 4 * (16 * k + i % 16)
-            out[i // 16, at:at + 4] = np.frombuffer(scales[i, k].tobytes(), np.uint8)
+    out = (np.zeros(panels * size, np.uint8) if into is None else into.copy()).reshape(panels, size)
+    scales = np.ascontiguousarray(s, "<f4")
+    rest, low = np.asarray(q, np.int64), []
+    for _ in range(digits):
+        low.append((rest + 128) % 256 - 128)
+        rest = (rest - low[-1]) // 256
+    assert not rest.any()
+    # token, block, digit, piece, half, byte
+    numbers = np.stack(low, 2).astype(np.int8).view(np.uint8).reshape(t, b, digits, 4, 2, 16)
+    for i in range(panels):
+        n = min(16, t - 16 * i)
+        at = out[i, :b * 2048 * digits].reshape(b, digits, 2, 4, 16, 16)  # .., token, byte
+        at[:, :, :, :, :n] = numbers[16 * i:16 * i + n].transpose(1, 2, 4, 3, 0, 5)
+        at = out[i, b * 2048 * digits:].reshape(b, 16, 4)
+        at[:, :n] = np.ascontiguousarray(scales[16 * i:16 * i + n].T).view(np.uint8).reshape(b, n, 4)
     return out.reshape(-1)
 
 
