@@ -93,6 +93,7 @@ SIGNATURES = {
     "ammon_cache_store": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT, _U32, _P]),
     "ammon_kv4_store": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _U32, _P]),
     "ammon_kv4_load": (_ST, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _DT]),
+    "ammon_w4_choose": (_ST, [_P, ctypes.c_char_p, ctypes.c_char_p]),
     "ammon_w4_bytes": (_SZ, [_U32, _U32]),
     "ammon_w4_store": (_ST, [_P, _P, _P, _DT, _U32, _U32, _P]),
     "ammon_w4_load": (_ST, [_P, _P, _P, _U32, _U32, _P, _DT]),

@@ -23,12 +23,22 @@ constexpr int kAttGroups = 4;  // GMAX = 1, 2, 4, 8
 constexpr int kGemvModes = 4;
 // KV4 variants: ceil(head / 32).
 constexpr int kKv4Groups = 4;
-// W4 GEMM tiles, as w4_prefill.hip has them: one panel of rows x 16, 32 tokens; 8 panels x 64
-// tokens; the long one (Q8: 8 x 128 tokens, Q24: 16 x 64).
-constexpr int kW4Tiles = 6;  // the last two are the big ones
+// A tile of the W4 prompt products (w4_prefill.hip): panels of 16 rows and tokens per workgroup,
+// its waves, and what w4_gemm (w4.cpp) reckons with, us: a group of 128 takes a CU's first
+// workgroup `first` and each further one `more`.  Waves have the panels' groups between them, but
+// those of the big tiles panels of their own.
+struct W4Tile {
+  const char *name;
+  uint32_t panels, tokens, waves;
+  double first, more, first_gated, more_gated;  // gated: 0 where there is none
+  bool big;
+};
+constexpr int kW4Tiles = 6;
+extern const W4Tile kW4Tile[2][kW4Tiles];  // [Q8, Q24]
 // W4 GEMV: sets of 8 waves with one chunk each, with more, of 2, of 8 in workgroups of 16, and waves
 // side by side
 enum { kW4One, kW4Sets, kW4Pairs, kW4Wide, kW4Flat, kW4Ways };
+extern const char *const kW4WayName[kW4Ways];
 // Bytes of a KV4 row per group of 32 numbers: 16 of codes, 4 of scale and bias.
 constexpr size_t kKv4RowBytes = 20;
 
@@ -152,6 +162,11 @@ struct ammon_runtime {
   // 0 never, else 10 * tokens-per-tile / 16 + 16-row tiles per wave
   // (44, 42, 24, 22)
   int gemm_big = -1;
+  // W4 products (ammon_w4_choose; -1, 0: by shape): the tile per digit type (kW4Tiles: it has none of
+  // that name), the number of its reduction ranges, the way
+  int w4_tile[2] = {-1, -1};
+  uint32_t w4_ranges = 0;
+  int w4_way = -1;
   std::mutex occ_mu;
   std::map<std::pair<hipFunction_t, size_t>, uint32_t> occ_cache;
 };

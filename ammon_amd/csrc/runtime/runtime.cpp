@@ -209,21 +209,19 @@ static ammon_status load_kernels(ammon_runtime *rt) {
     snprintf(name, sizeof name, "ammon_q8_load_%d", q ? 3 : 1);
     R(8, name, k.q8_load[q]);
   }
-  const char *w4_ways[] = {"k8_one", "k8", "k2", "k8_wide", "flat"};
   for (int i = 0; i < kW4Ways; ++i)
     for (int m = 0; m <= kGemvModes; ++m) {
       char name[96];
-      snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax", w4_ways[i]);
+      snprintf(name, sizeof name, "ammon_w4_gemv_%s_%s", m < kGemvModes ? modes[m] : "plain_argmax",
+               kW4WayName[i]);
       R(9, name, k.w4_gemv[i][m]);
     }
-  const char *w4_tiles[2][kW4Tiles] = {{"t16", "t16_deep", "t16_x4", "t32_x2", "t64", "long"},
-                                       {"t16", "t16_deep", "t16_x2", "t16_x4", "t64", "long"}};
   for (int q = 0; q < 2; ++q)
     for (int t = 0; t < kW4Tiles; ++t)
       for (int m = 0; m < kGemvModes; ++m) {
-        if (t == 1 && m == AMMON_GEMV_SWIGLU) continue;  // (none)
+        if (m == AMMON_GEMV_SWIGLU && kW4Tile[q][t].first_gated == 0) continue;  // (none)
         char name[96];
-        snprintf(name, sizeof name, "ammon_w4_gemm_%s_q%d_%s", modes[m], q ? 3 : 1, w4_tiles[q][t]);
+        snprintf(name, sizeof name, "ammon_w4_gemm_%s_q%d_%s", modes[m], q ? 3 : 1, kW4Tile[q][t].name);
         R(10, name, k.w4_gemm[q][t][m]);
       }
 #undef R

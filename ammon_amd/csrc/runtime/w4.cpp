@@ -2,6 +2,8 @@
 // (AMMON_Q8, AMMON_Q24): validate, pick the variant, launch.  No counterpart in the reference.
 #include <hip/hip_runtime_api.h>
 
+#include <cstring>
+
 #include "ops_common.h"
 
 using namespace ammon_rt;
@@ -111,44 +113,29 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
   p.kv_rows = a.kv_rows;
   const bool gated = a.mode == AMMON_GEMV_SWIGLU, q24 = a.x_dtype == AMMON_Q24;
   const uint64_t panels = cdiv(gated ? a.d : a.rows, 16);
-  // Of the tiles, the last two optionally with the reduction split into 2, 4 or 8 ranges (a
+  // Of the tiles, the big ones optionally with the reduction split into 2, 4 or 8 ranges (a
   // workspace, no SwiGLU), the one with the least estimated time, in us: a launch takes 3.5 (of
-  // sixteen waves 3.85); a group of 128 takes a CU's first workgroup `first` and each further one `more` (the big ones, of
-  // which several take turns, `more` each as soon as there are two); a split adds a second launch
-  // and the sums' traffic.  Fitted to 4096 x 4096, 6144 x 4096, 4096 x 14336, 10240 x 8192, 8192 x
-  // 28672, 5003 x 2080, 1024 x 8192, 128256 x 4096, 288 x 288 and (SwiGLU) 28672 x 4096, 11264 x 2048
-  // and 57344 x 8192, 1 to 2048 tokens, both digit types, every tile and split: the tile so chosen
-  // is on average 1.4% slower than the best one, and at most 22%.  E.g. of 6144 x 4096, 41 tokens of
-  // Q24: 16-token tiles 15.5 us, of two panels 13.0, of four 12.4 (estimate 13.5), long tiles in
-  // eight ranges 14.7, whole 56.
-  struct Tile {
-    uint32_t panels, tokens, waves;
-    double first, more, first_gated, more_gated;
-  };
-  static const Tile tiles[2][kW4Tiles] = {{{1, 16, 8, 0.039, 0.044, 0.082, 0.081},
-                                           {1, 16, 16, 0.035, 0.049, 0, 0},
-                                           {4, 16, 8, 0.118, 0.112, 0.312, 0.254},
-                                           {2, 32, 8, 0.094, 0.088, 0.207, 0.166},
-                                           {8, 64, 4, 0.48, 0.377, 0.48, 0.377},
-                                           {8, 128, 4, 0.99, 0.693, 0.99, 0.693}},
-                                          {{1, 16, 8, 0.070, 0.089, 0.127, 0.126},
-                                           {1, 16, 16, 0.066, 0.093, 0, 0},
-                                           {2, 16, 8, 0.106, 0.110, 0.210, 0.181},
-                                           {4, 16, 8, 0.163, 0.156, 0.361, 0.329},
-                                           {8, 64, 4, 0.93, 0.83, 0.93, 0.83},
-                                           {16, 64, 4, 1.55, 1.44, 1.55, 1.44}}};
+  // sixteen waves 3.85); a group of 128 takes a CU's first workgroup `first` and each further one
+  // `more` (the big ones, of which several take turns, `more` each as soon as there are two); a
+  // split adds a second launch and the sums' traffic.  Fitted to 4096 x 4096, 6144 x 4096, 4096 x
+  // 14336, 10240 x 8192, 8192 x 28672, 5003 x 2080, 1024 x 8192, 128256 x 4096, 288 x 288 and
+  // (SwiGLU) 28672 x 4096, 11264 x 2048 and 57344 x 8192, 1 to 2048 tokens, both digit types, every
+  // tile and split: the tile so chosen is on average 1.4% slower than the best one, and at most 22%.
+  // E.g. of 6144 x 4096, 41 tokens of Q24: 16-token tiles 15.5 us, of two panels 13.0, of four 12.4
+  // (estimate 13.5), long tiles in eight ranges 14.7, whole 56.
   const uint32_t groups = cdiv(a.n, 128), cus = (uint32_t)std::max(rt->info.compute_units, 1);
-  const Tile *tile = nullptr;
+  const W4Tile *const tiles = kW4Tile[q24], *tile = nullptr;
   uint32_t ksplit = 1, per = 1;  // per: panels of results per workgroup
   double best = 1e300;
   for (int i = 0; i < kW4Tiles; ++i) {
-    const Tile *t = &tiles[q24][i];
-    const bool big = i >= kW4Tiles - 2;
-    if (i == 1 && gated) continue;
+    const W4Tile *t = &tiles[i];
+    const bool big = t->big;
+    if ((gated && t->first_gated == 0) || (rt->w4_tile[q24] >= 0 && rt->w4_tile[q24] != i)) continue;
     const uint32_t pp = big && gated ? t->panels / 2 : t->panels;
     for (uint32_t k = 1; k <= 8; k *= 2) {
       const uint64_t sums = (uint64_t)k * a.tokens * a.rows * 4;
       if (k > 1 && (!big || gated || !a.ws || sums > a.ws_bytes || sums > (64ull << 20) || groups < 4 * k)) break;
+      if (rt->w4_ranges && k != rt->w4_ranges) continue;
       // (the XCDs get row blocks' ranges in turn)
       const uint64_t wgs = (uint64_t)cdiv((uint64_t)cdiv(panels, pp) * k, 8) * 8 * cdiv(a.tokens, t->tokens);
       const uint64_t turns = (wgs + cus - 1) / cus;
@@ -158,6 +145,7 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
       if (us < best) best = us, tile = t, ksplit = k, per = pp;
     }
   }
+  AMMON_CHECK(tile, "%s: the tile chosen does not take this call", what);
   if (ksplit > 1) {
     p.ws = (float *)a.ws;
     p.ksplit = ksplit;
@@ -168,7 +156,7 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
   VALIDATE_ONLY();
   DeviceGuard guard(rt->device);
   void *args[] = {&p};
-  const hipError_t e = hipModuleLaunchKernel(rt->k.w4_gemm[q24][tile - tiles[q24]][a.mode], (uint32_t)grid, 1, 1,
+  const hipError_t e = hipModuleLaunchKernel(rt->k.w4_gemm[q24][tile - tiles][a.mode], (uint32_t)grid, 1, 1,
                                              64 * tile->waves, 1, 1, 0,
                                              stream ? (hipStream_t)stream : rt->stream, args, nullptr);
   if (e != hipSuccess) return hip_error(e, what);
@@ -275,6 +263,20 @@ ammon_status q8_rows(ammon_runtime *rt, ammon_stream stream, const float *x, con
 
 namespace ammon_rt {
 
+const W4Tile kW4Tile[2][kW4Tiles] = {{{"t16", 1, 16, 8, 0.039, 0.044, 0.082, 0.081, false},
+                                      {"t16_deep", 1, 16, 16, 0.035, 0.049, 0, 0, false},
+                                      {"t16_x4", 4, 16, 8, 0.118, 0.112, 0.312, 0.254, false},
+                                      {"t32_x2", 2, 32, 8, 0.094, 0.088, 0.207, 0.166, false},
+                                      {"t64", 8, 64, 4, 0.48, 0.377, 0.48, 0.377, true},
+                                      {"long", 8, 128, 4, 0.99, 0.693, 0.99, 0.693, true}},
+                                     {{"t16", 1, 16, 8, 0.070, 0.089, 0.127, 0.126, false},
+                                      {"t16_deep", 1, 16, 16, 0.066, 0.093, 0, 0, false},
+                                      {"t16_x2", 2, 16, 8, 0.106, 0.110, 0.210, 0.181, false},
+                                      {"t16_x4", 4, 16, 8, 0.163, 0.156, 0.361, 0.329, false},
+                                      {"t64", 8, 64, 4, 0.93, 0.83, 0.93, 0.83, true},
+                                      {"long", 16, 64, 4, 1.55, 1.44, 1.55, 1.44, true}}};
+const char *const kW4WayName[kW4Ways] = {"k8_one", "k8", "k2", "k8_wide", "flat"};
+
 ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, const char *what,
                      uint32_t *grid_out) {
   AMMON_CHECK(a.w0 && a.x && a.y, "%s: NULL weight, x or y", what);
@@ -322,7 +324,6 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   p.kv_rows = a.kv_rows;
   p.cand_v = a.cand_v;
   p.cand_i = a.cand_i;
-  VALIDATE_ONLY();
   // Where a CU has between 64 and 384 groups (14336 x 4096 twice, 224: 12.3 us, as sets 14.4; 10240 x
   // 8192, 160: 10.4 and 14.7; 4096 x 14336, 112: 8.4 and 9.6), its waves take them side by side.  With
   // fewer the sixteen waves' own costs show (4096 x 4096, 32: 5.0 and 3.7; 6144 x 4096, 48: 5.3 and
@@ -336,14 +337,22 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   const uint32_t cap = a.mode == AMMON_GEMV_PLAIN_ARGMAX ? a.cand_cap : UINT32_MAX;
   const uint64_t a_cu = (uint64_t)p.row_blocks * cdiv(a.n, 128) / cus;
   int way = 2 * (lds_of(8) + 4096) > kLdsPerCu ? kW4Wide : p.row_blocks >= 3 * 8 * cus ? kW4Pairs : kW4Sets;
-  uint32_t grid = std::min({cdiv(p.row_blocks, way == kW4Wide ? 2 : way == kW4Pairs ? 4 : 1),
-                            cus * (way == kW4Wide ? 1 : 2), cap});
-  if (way == kW4Sets && grid == p.row_blocks && a.n <= 8 * 128 * AMMON_W4_CHUNK) way = kW4One;
-  if (p.row_blocks >= cus && a_cu >= 64 && a_cu <= 384 &&
-      cdiv(p.row_blocks, std::min(cus, cap)) <= AMMON_W4_UNITS) {
-    way = kW4Flat;
-    grid = std::min(cus, cap);
+  auto grid_of = [&](int by) {
+    if (by == kW4Flat) return std::min({p.row_blocks, cus, cap});
+    return std::min({cdiv(p.row_blocks, by == kW4Wide ? 2 : by == kW4Pairs ? 4 : 1),
+                     cus * (by == kW4Wide ? 1 : 2), cap});
+  };
+  const bool one = a.n <= 8 * 128 * AMMON_W4_CHUNK && grid_of(kW4One) == p.row_blocks;
+  const bool flat = cdiv(p.row_blocks, grid_of(kW4Flat)) <= AMMON_W4_UNITS;
+  if (way == kW4Sets && one) way = kW4One;
+  if (p.row_blocks >= cus && a_cu >= 64 && a_cu <= 384 && flat) way = kW4Flat;
+  if (rt->w4_way >= 0) {
+    way = rt->w4_way;
+    AMMON_CHECK((one || way != kW4One) && (flat || way != kW4Flat),
+                "%s: the way chosen does not take this call", what);
   }
+  uint32_t grid = grid_of(way);
+  VALIDATE_ONLY();
   if (grid_out) *grid_out = grid;
   DeviceGuard guard(rt->device);
   void *args[] = {&p.w0, &p.x, &p.norm_w, &p.n, &p.norm_dtype, &p.row_blocks, &grid, &p.w1, &p.w2, &p};
@@ -358,6 +367,32 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
 }  // namespace ammon_rt
 
 extern "C" {
+
+ammon_status ammon_w4_choose(ammon_runtime *rt, const char *tile, const char *way) {
+  REQUIRE_RT();
+  int tiles[2] = {-1, -1}, ranges = 0, w = -1;
+  if (tile) {
+    const char *slash = std::strchr(tile, '/');
+    const std::string name = slash ? std::string(tile, slash) : tile;
+    for (int q = 0; q < 2; ++q)
+      for (tiles[q] = 0; tiles[q] < kW4Tiles && name != kW4Tile[q][tiles[q]].name;) ++tiles[q];
+    AMMON_CHECK(std::min(tiles[0], tiles[1]) < kW4Tiles, "w4_choose: no tile is called %s", name.c_str());
+    if (slash) {
+      ranges = slash[1] - '0';
+      AMMON_CHECK((ranges == 1 || ranges == 2 || ranges == 4 || ranges == 8) && !slash[2],
+                  "w4_choose: %s: ranges are 1, 2, 4 or 8", tile);
+    }
+  }
+  if (way) {
+    for (w = 0; w < kW4Ways && std::strcmp(way, kW4WayName[w]);) ++w;
+    AMMON_CHECK(w < kW4Ways, "w4_choose: no way is called %s", way);
+  }
+  rt->w4_tile[0] = tiles[0];
+  rt->w4_tile[1] = tiles[1];
+  rt->w4_ranges = (uint32_t)ranges;
+  rt->w4_way = w;
+  return AMMON_OK;
+}
 
 size_t ammon_w4_bytes(uint32_t d, uint32_t n) { return (size_t)cdiv(d, 16) * cdiv(n, 128) * 1056; }
 
