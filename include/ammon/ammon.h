@@ -303,12 +303,14 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
  * As w_dtype (w1, w3; wq, wk, wv alike) it is taken by ammon_gemv,
  * ammon_gemv_rmsnorm, ammon_gate_up_swiglu, ammon_qkv_rope(_store) and
  * ammon_greedy_lm_head: x's numbers enter as 32-bit whole numbers with a scale
- * per 128 of them (off by at most 2^-30.9 of the largest of those), their
- * products with the codes of a group are summed exactly, and the groups in fp32
- * (in an order that depends on the shape and the row, the same in every call).  An
- * x with a number that is not finite (after the norm) gives NaN.  Queries, keys and values have to be a
- * multiple of 16 rows each; n is at most 36864.  ammon_prefill_*_w4 below take
- * it for several tokens. */
+ * per 128 of them (off by at most 2^-30.9 of the largest of those, or 2^-121),
+ * their products with the codes of a group are summed exactly, and the groups in
+ * fp32 (in an order that depends on the shape and the row, the same in every
+ * call).  With a norm they are the numbers times its weight, and its factor is
+ * applied to the results; the squares are summed in fp32.  An x with a number
+ * that is not finite (after the norm's weight) gives NaN.  Queries, keys and
+ * values have to be a multiple of 16 rows each; n is at most 36864.
+ * ammon_prefill_*_w4 below take it for several tokens. */
 size_t ammon_w4_bytes(uint32_t d, uint32_t n);
 /* w [d, n] fp32 or bf16 into out. */
 ammon_status ammon_w4_store(ammon_runtime *rt, ammon_stream stream, const void *w,

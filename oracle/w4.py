@@ -132,15 +132,25 @@ def normed(x, w, eps):
 
 
 def product_bar(x, w, exact_x):
-    """How far fp32 results of rows x [t, n] (float64) times w [d, n] may be from float64's [t, d].
-    With x as Q24 in the call (exact_x False), a number of x is off by half a step, 2^-22.98 of its
-    block's largest.  A group's sum is exact, its conversion from whole numbers (of 24 bits and
-    more) and its addition round by 2^-24 of the sums so far, at most sum |w| |x|, and so do three
-    additions of digits, three of waves, seven of ranges and the residual's."""
+    """How far fp32 results of rows x [t, n] (float64) times w [d, n] may be from float64's [t, d], a
+    rounding being 2^-24 of its result.  With S = sum |w| |x|:
+
+    Rows of digits (exact_x True).  A group's digits are joined by a conversion and an addition, at
+    most 2^-24 of the group's part of S each, and added up with one more, of S: 2 + groups.  Waves
+    (of which no more than groups have any), ranges and a residual add at most 16, 7 and 1 of S:
+    2 groups + 16 in all, or less (groups + 3 + groups with fewer groups than waves).
+
+    One token (exact_x False), whose x is made 32-bit whole numbers.  A number is off by half a step,
+    2^-30.98 of its block's largest (2^-121 where that is below 2^-90).  The four digits' sums are
+    added up apart, one rounding a group, then with each other (3) and over waves (16): again within
+    2 groups + 16, but of the digits' sizes instead of |x|.  A digit's remainder is at most half a
+    unit of the digit above, so that their sizes together are at most |x| + 6.1 times the remainder
+    of the highest one, which is no larger than |x| and than 1 / 127 of the block's largest."""
     a, b = np.abs(x), np.abs(w)
-    size = a @ b.T
-    bar = (2 * groups(x.shape[1]) + 16) * 2.0**-24 * size
-    if not exact_x:
-        top = blocks(a).max(-1)  # [t, groups]
-        bar += 2.0**-22.98 * top @ blocks(b).sum(-1).T
-    return bar
+    rounding = (2 * groups(x.shape[1]) + 16) * 2.0**-24
+    if exact_x:
+        return rounding * a @ b.T
+    size = blocks(a)
+    top = size.max(-1)  # [t, groups]
+    size = (size + 6.1 * np.minimum(size, top[..., None] / 127)).reshape(len(a), -1)[:, :x.shape[1]]
+    return rounding * size @ b.T + 2.0**-30.98 * top @ blocks(b).sum(-1).T

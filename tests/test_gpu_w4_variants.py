@@ -429,6 +429,21 @@ def test_the_lower_digits_of_a_token(tuned, way, d, n, size):
     assert np.all(want > 60 * np.resize(bar, d))
 
 
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("size", [2.0**-125, 2.0**-110, 2.0**-92, 2.0**90])
+def test_tokens_of_any_size(tuned, way, size):
+    """x's numbers are at most 2^-121 off where they are smaller than 2^-90 (the weights are some 2^30,
+    so that results are normal numbers)."""
+    rt, d, n = tuned(way=way), 112, 300
+    w = Weights(rt, d, n, w=np.ldexp(matrix(d, n), 30))
+    x = (size * np.random.default_rng(2).uniform(-1, 1, (1, n))).astype(np.float32)
+    y = rt.alloc(4 * d)
+    call("ammon_gemv", rt.handle, None, w.dev, W4, d, n, up(rt, x), y, None)
+    x = x.astype(np.float64)
+    bar = w4.product_bar(x, w.numbers, False) + 2.0**-121 * np.abs(w.numbers).sum(-1)
+    close(y.download((1, d)), x @ w.numbers.T, bar)
+
+
 @pytest.mark.parametrize("d,n,way", [(288, 288, "k8_one"), (4096, 4096, "k8_one"), (9000, 2000, "k8"),
                                      (131072, 128, "k2"), (128256, 1700, "k2"), (20, 36864, "k8_wide"),
                                      (4112, 36864, "flat"), (4096, 14336, "flat"), (131072, 200, "flat"),
