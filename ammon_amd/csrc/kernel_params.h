@@ -19,9 +19,6 @@ extern "C" {
 #define AMMON_K_F32 0
 #define AMMON_K_BF16 1
 #define AMMON_K_KV4 4 /* KV caches only: kernels/kv4_impl.h */
-#define AMMON_K_W4 5  /* weights only: kernels/w4_impl.h */
-#define AMMON_K_Q8 6  /* rows of one 8-bit digit a number, and of three */
-#define AMMON_K_Q24 7
 #define AMMON_W4_CHUNK 4  /* W4 GEMV: groups of 128 that a wave takes at once */
 #define AMMON_W4_UNITS 32 /* units of 16 rows that a workgroup of waves side by side takes at most */
 #define AMMON_KV4_LOAD_ROWS 4 /* rows a lane of kv4_load takes */

@@ -232,6 +232,7 @@ template <int MODE, uint32_t KS, uint32_t NW, bool ONE> struct W4Sets : W4Token<
   using T::p, T::lane, T::w, T::groups;
   static constexpr uint32_t U = AMMON_W4_CHUNK;  // groups a register buffer holds
   static constexpr uint32_t US = NW / KS;        // sets
+  static_assert(KS > 1 && NW % KS == 0, "sets of several waves");
   uint32_t wave, set, chunks;                    // of the set; chunks: a wave's of a unit
 
   // operands' addresses in the current unit
@@ -349,10 +350,7 @@ template <int MODE, uint32_t KS, uint32_t NW, bool ONE> struct W4Sets : W4Token<
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = group_sum16(acc[i], 4);
       if ((lane & 15) == 0) *(f32x4 *)&r[wave][4 * (lane >> 4)] = sum;
-      if (KS > 1)
-        __syncthreads();
-      else
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the wave's own)
+      __syncthreads();
       const uint32_t u = unit_of(round);
       if (wave == round % KS && u < units) rows(u, &r[0][0], pos, cand_v, cand_i);
       acc = f32x4{0.f, 0.f, 0.f, 0.f};

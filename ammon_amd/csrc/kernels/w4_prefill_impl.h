@@ -155,22 +155,14 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct
       for (uint32_t c = 0; c < CT; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (gbeg >= gend) return;
     const uint32_t end = gend - 1;
-    if constexpr (CT * DIGITS <= 6) {  // the next group on its way (more do not fit the registers)
-      Group o0, o1;
-      load(gbeg, o0);
-      for (uint32_t g = gbeg; g < gend; g += 2) {
-        load(min(g + 1, end), o1);
-        multiply(o0, acc);
-        if (g + 1 >= gend) break;
-        load(min(g + 2, end), o0);
-        multiply(o1, acc);
-      }
-    } else {
-      for (uint32_t g = gbeg; g < gend; ++g) {
-        Group o;
-        load(g, o);
-        multiply(o, acc);
-      }
+    Group o0, o1;  // one multiplied, the next on its way
+    load(gbeg, o0);
+    for (uint32_t g = gbeg; g < gend; g += 2) {
+      load(min(g + 1, end), o1);
+      multiply(o0, acc);
+      if (g + 1 >= gend) break;
+      load(min(g + 2, end), o0);
+      multiply(o1, acc);
     }
   }
 

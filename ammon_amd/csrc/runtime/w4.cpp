@@ -282,6 +282,7 @@ ammon_status w4_gemv(ammon_runtime *rt, ammon_stream stream, const GemvArgs &a, 
   AMMON_CHECK(a.w0 && a.x && a.y, "%s: NULL weight, x or y", what);
   TRY(shape_check(what, a.rows, a.n));
   AMMON_CHECK(a.d > 0, "%s: empty matrix (d=%u)", what, a.d);
+  // (of the plain products gemv_at_position alone has a step, whose row of y it writes)
   AMMON_CHECK(a.mode != AMMON_GEMV_PLAIN || !a.step, "%s: takes no W4 weights", what);
   AMMON_CHECK(!a.norm_w || valid_dtype(a.norm_dtype), "%s: unknown norm dtype", what);
   AMMON_CHECK(!a.norm_w || (std::isfinite(a.eps) && a.eps >= 0.f), "%s: eps must be finite and >= 0", what);
