@@ -23,9 +23,10 @@ W4_GEMM_UNGATED(W4_SHORT_KERNEL, 3, t16_deep, 1, 1, 16)
 W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16_x2, 2, 1, 8)
 W4_GEMM_MODES(W4_SHORT_KERNEL, 3, t16_x4, 4, 1, 8)
 
-// panels of rows per wave, token panels, workgroups per CU.  The long tile shares a wave's codes or the tokens' digits
-// between more products: of one digit, whose sums' scaling keeps the vector units busy, the codes
-// (2048 tokens x 28672 x 4096: 314 us, 64-token tiles 335); of three the digits (643 us; 792 before the last 7%).
+// panels of rows per wave, token panels, workgroups per CU.  The long tile shares a wave's codes or the
+// tokens' digits between more products: of one digit, whose sums' scaling keeps the vector units
+// busy, the codes (2048 tokens x 28672 x 4096 gated: 313 us, 64-token tiles 375); of three the
+// digits (660 us, 64-token tiles 778).
 #define W4_BIG_KERNEL(NAME, DIGITS, MODE, RT, CT, OCC)                                \
   extern "C" __global__ __launch_bounds__(AMMON_WG, OCC) void NAME(ammon_k_gemm p) { \
     w4_gemm_big<DIGITS, MODE, RT, CT>(p);                                          \

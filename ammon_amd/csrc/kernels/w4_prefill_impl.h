@@ -208,10 +208,11 @@ template <int DIGITS, int MODE, uint32_t RT, uint32_t CT, uint32_t SPLIT> struct
 
 // Short prompts.  What bounds them is the digits' way from L2: a group's 1 KiB of codes meets 2 KiB
 // of digits per digit and token panel, in every workgroup.  So workgroups have as many panels of
-// rows as leave every CU one (16 tokens of three digits: 28672 x 4096 gated 24.0 us with one panel,
-// 19.1 with two, 17.2 with four; 128256 x 4096 113, 77, 59; but 4096 x 4096 5.5, 6.4, 8.3), and
-// tokens past the last one are not read (5 tokens: 24.0 to 20.1 us).  PANELS panels of results (gated: of each matrix) per workgroup, their groups split
-// over SPLIT waves, whose sums meet in LDS and are added in wave order, a wave a panel and tokens'.
+// rows as leave every CU one (16 tokens of three digits: 28672 x 4096 gated 22.9 us with one panel,
+// 18.2 with two, 16.8 with four; 128256 x 4096 135, 94, 74; but 4096 x 4096 5.7, 7.9, 8.9), and
+// tokens past the last one are not read (5 tokens: 24.0 to 20.1 us).  PANELS panels of results
+// (gated: of each matrix) per workgroup, their groups split over SPLIT waves, whose sums meet in LDS
+// and are added in wave order, a wave a panel and tokens'.
 template <int DIGITS, int MODE, uint32_t PANELS, uint32_t CT, uint32_t SPLIT>
 AMMON_DEV void w4_gemm_short(const ammon_k_gemm &p) {
   constexpr uint32_t RT = MODE == AMMON_GEMV_SWIGLU ? 2 * PANELS : PANELS;

@@ -119,10 +119,12 @@ ammon_status w4_gemm(ammon_runtime *rt, ammon_stream stream, const W4GemmArgs &a
   // `more` (the big ones, of which several take turns, `more` each as soon as there are two); a
   // split adds a second launch and the sums' traffic.  Fitted to 4096 x 4096, 6144 x 4096, 4096 x
   // 14336, 10240 x 8192, 8192 x 28672, 5003 x 2080, 1024 x 8192, 128256 x 4096, 288 x 288 and
-  // (SwiGLU) 28672 x 4096, 11264 x 2048 and 57344 x 8192, 1 to 2048 tokens, both digit types, every
-  // tile and split: the tile so chosen is on average 1.4% slower than the best one, and at most 22%.
-  // E.g. of 6144 x 4096, 41 tokens of Q24: 16-token tiles 15.5 us, of two panels 13.0, of four 12.4
-  // (estimate 13.5), long tiles in eight ranges 14.7, whole 56.
+  // (SwiGLU) 28672 x 4096, 11264 x 2048 and 57344 x 8192, 1 to 2048 tokens, both digit types.  Of 300
+  // such products, every tile and split timed, the one so chosen is 1.3% slower than the best on
+  // average, more than 10% in eight, at most 58% (1024 x 8192, 301 tokens of Q8: 64-token tiles in
+  // eight ranges 20.7 us, 32-token tiles 13.0; the next worst 22%).  E.g. of 6144 x 4096, 41 tokens
+  // of Q24: 16-token tiles 16.1 us, of two panels 13.2, of four 12.6 (estimate 13.5), long tiles in
+  // eight ranges 14.3, whole 50.8.
   const uint32_t groups = cdiv(a.n, 128), cus = (uint32_t)std::max(rt->info.compute_units, 1);
   const W4Tile *const tiles = kW4Tile[q24], *tile = nullptr;
   uint32_t ksplit = 1, per = 1;  // per: panels of results per workgroup

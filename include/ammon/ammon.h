@@ -306,7 +306,7 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
  * per 128 of them (off by at most 2^-30.9 of the largest of those, or 2^-121),
  * their products with the codes of a group are summed exactly, and the groups in
  * fp32 (in an order that depends on the shape and the row, the same in every
- * call).  With a norm they are the numbers times its weight, and its factor is
+ * call; equal rows may so differ in their last bits).  With a norm they are the numbers times its weight, and its factor is
  * applied to the results; the squares are summed in fp32.  An x with a number
  * that is not finite (after the norm's weight) gives NaN.  Queries, keys and
  * values have to be a multiple of 16 rows each; n is at most 36864.
