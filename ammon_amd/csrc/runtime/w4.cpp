@@ -376,19 +376,20 @@ ammon_status ammon_w4_choose(ammon_runtime *rt, const char *tile, const char *wa
   int tiles[2] = {-1, -1}, ranges = 0, w = -1;
   if (tile) {
     const char *slash = std::strchr(tile, '/');
-    const std::string name = slash ? std::string(tile, slash) : tile;
+    const size_t len = slash ? (size_t)(slash - tile) : std::strlen(tile);
+    auto called = [&](const char *name) { return std::strlen(name) == len && !std::strncmp(name, tile, len); };
     for (int q = 0; q < 2; ++q)
-      for (tiles[q] = 0; tiles[q] < kW4Tiles && name != kW4Tile[q][tiles[q]].name;) ++tiles[q];
-    AMMON_CHECK(std::min(tiles[0], tiles[1]) < kW4Tiles, "w4_choose: no tile is called %s", name.c_str());
+      for (tiles[q] = 0; tiles[q] < kW4Tiles && !called(kW4Tile[q][tiles[q]].name);) ++tiles[q];
+    AMMON_CHECK(std::min(tiles[0], tiles[1]) < kW4Tiles, "w4_choose: no tile is called %.40s", tile);
     if (slash) {
       ranges = slash[1] - '0';
       AMMON_CHECK((ranges == 1 || ranges == 2 || ranges == 4 || ranges == 8) && !slash[2],
-                  "w4_choose: %s: ranges are 1, 2, 4 or 8", tile);
+                  "w4_choose: %.40s: ranges are 1, 2, 4 or 8", tile);
     }
   }
   if (way) {
     for (w = 0; w < kW4Ways && std::strcmp(way, kW4WayName[w]);) ++w;
-    AMMON_CHECK(w < kW4Ways, "w4_choose: no way is called %s", way);
+    AMMON_CHECK(w < kW4Ways, "w4_choose: no way is called %.40s", way);
   }
   rt->w4_tile[0] = tiles[0];
   rt->w4_tile[1] = tiles[1];
