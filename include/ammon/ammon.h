@@ -306,10 +306,11 @@ ammon_status ammon_kv4_load(ammon_runtime *rt, ammon_stream stream, const void *
  * per 128 of them (off by at most 2^-30.9 of the largest of those, or 2^-121),
  * their products with the codes of a group are summed exactly, and the groups in
  * fp32 (in an order that depends on the shape and the row, the same in every
- * call; equal rows may so differ in their last bits).  With a norm they are the numbers times its weight, and its factor is
- * applied to the results; the squares are summed in fp32.  An x with a number
- * that is not finite (after the norm's weight) gives NaN.  Queries, keys and
- * values have to be a multiple of 16 rows each; n is at most 36864.
+ * call; equal rows may so differ in their last bits).  With a norm they are the
+ * numbers times its weight, and its factor is applied to the results; the
+ * squares are summed in fp32.  An x with a number that is not finite (after the
+ * norm's weight) gives NaN.  Queries, keys and values have to be a multiple of
+ * 16 rows each; n is at most 36864.
  * ammon_prefill_*_w4 below take it for several tokens. */
 size_t ammon_w4_bytes(uint32_t d, uint32_t n);
 /* w [d, n] fp32 or bf16 into out. */
@@ -608,9 +609,9 @@ ammon_status ammon_prefill_qkv_rope_store_w4(ammon_runtime *rt, ammon_stream str
                                              ammon_dtype kv_dtype, uint32_t seq,
                                              const ammon_decode_step *step, const float *table,
                                              void *workspace, size_t workspace_bytes);
-/* For measurements and tests: which kernels W4 products take on this runtime,
- * in place of the library's choice by shape (NULL: that one again), until the
- * next call of this.  tile, of the prompts': "t16", "t16_deep" (not SwiGLU),
+/* For measurements and tests: which kernels W4 products take on this runtime
+ * (that is, on this device: its holders share it), in place of the library's
+ * choice by shape (NULL: that one again), until the next call of this.  tile, of the prompts': "t16", "t16_deep" (not SwiGLU),
  * "t16_x2" (Q24), "t16_x4", "t32_x2" (Q8), "t64" or "long", the last two
  * optionally with the reduction ranges that they split into ("long/1", "/2",
  * "/4", "/8").  way, of one token's: "k8_one", "k8", "k2", "k8_wide" or "flat".
