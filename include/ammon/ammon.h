@@ -611,13 +611,13 @@ ammon_status ammon_prefill_qkv_rope_store_w4(ammon_runtime *rt, ammon_stream str
                                              void *workspace, size_t workspace_bytes);
 /* For measurements and tests: which kernels W4 products take on this runtime
  * (that is, on this device: its holders share it), in place of the library's
- * choice by shape (NULL: that one again), until the next call of this.  tile, of the prompts': "t16", "t16_deep" (not SwiGLU),
- * "t16_x2" (Q24), "t16_x4", "t32_x2" (Q8), "t64" or "long", the last two
- * optionally with the reduction ranges that they split into ("long/1", "/2",
- * "/4", "/8").  way, of one token's: "k8_one", "k8", "k2", "k8_wide" or "flat".
- * A product that the kernel named does not take is refused.  Results differ in
- * the order of fp32 sums.  No product may be under way in another thread
- * meanwhile. */
+ * choice by shape (NULL: that one again), until the next call of this.  tile, of
+ * the prompts': "t16", "t16_deep" (not SwiGLU), "t16_x2" (Q24), "t16_x4",
+ * "t32_x2" (Q8), "t64" or "long", the last two optionally with the reduction
+ * ranges that they split into ("long/1", "/2", "/4", "/8").  way, of one token's:
+ * "k8_one", "k8", "k2", "k8_wide" or "flat".  A product that the kernel named
+ * does not take is refused.  Results differ in the order of fp32 sums.  No
+ * product may be under way in another thread meanwhile. */
 ammon_status ammon_w4_choose(ammon_runtime *rt, const char *tile, const char *way);
 /* ammon_attention_decode for each of `tokens` query rows q [tokens, q_heads,
  * head] at positions step->position + t, which must be below ctx <= seq
